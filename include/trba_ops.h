@@ -1,6 +1,7 @@
 /* INT8 operator API of libtrba_b200: device-resident counterparts of the
  * reference's LinearInt8 (src/linear.rs) and LSTMInt8 / BiLSTMInt8
- * (src/bilstm.rs).
+ * (src/bilstm.rs), and LinearInt4, a linear layer with 4-bit weights for
+ * decoding.
  *
  * The reference keeps the f32 master weights and their int8 copies in host
  * vectors and moves every operand through a fresh device workspace per call.
@@ -57,6 +58,43 @@ int trba_linear_int8_get(trba_linear_int8 *l, float *weight_f32, int8_t *weight_
 /* Replace the f32 weights / bias from the host (NULL = keep) and re-quantise. */
 int trba_linear_int8_set(trba_linear_int8 *l, const float *weight_f32, const float *bias);
 long long trba_linear_int8_param_count(const trba_linear_int8 *l);
+
+/* ---- LinearInt4 (no counterpart in the reference) ----
+ * y [rows, out] = x [rows, in] . W^T + bias for the few rows of a decoding
+ * step (one line, or its beams), where reading the weights is what takes the
+ * time: W[n, k] = (code[n, k] - 8) * scale[n, k / group], 4-bit codes with one
+ * scale per `group` consecutive inputs.  group is 32, 64 or a multiple of
+ * 128; the last group of a row may be short.  Sums are f32 (f32 activations
+ * enter them with all their bits) and y is rounded once, to the type of x.
+ *
+ * A layer keeps its weights on the device that was current when it was
+ * created; forward is refused on another one.  forward only launches kernels:
+ * it may run on several streams at once and be captured into CUDA graphs. */
+typedef struct trba_linear_int4 trba_linear_int4;
+/* From f32 weights [out, in] row-major and bias [out] (NULL = zeros), both on
+ * the host.  scale = max |w| of the group / 7 (1 when all are zero), code - 8
+ * = round(w / scale), halves away from zero (the rule of
+ * LinearInt8::quantize, src/linear.rs:53-59, for 4 bits and groups). */
+trba_linear_int4 *trba_linear_int4_create(int in_features, int out_features, int group, const float *weight_f32,
+                                          const float *bias);
+/* From codes and scales on the device: codes [out, (in + 1) / 2] bytes, the
+ * even input's code in the low half, row stride ld_codes bytes; scales [out,
+ * ceil(in / group)], f32 or f16 (scale_dtype: TRBA_F32 or TRBA_F16 of
+ * trba_decode.h), row stride ld_scales elements; bias f32 [out] or NULL.
+ * Reads them in `stream`'s order and returns when they may be freed. */
+trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_features, int group, const uint8_t *codes,
+                                                long long ld_codes, const void *scales, int scale_dtype,
+                                                long long ld_scales, const float *bias, void *stream);
+void trba_linear_int4_destroy(trba_linear_int4 *l);
+/* x [rows, in] and y [rows, out] on the device, both of `dtype` (TRBA_F32,
+ * TRBA_BF16, TRBA_F16), row strides ldx >= in and ldy >= out in elements; y
+ * must not overlap x.  rows = 0 is an empty call. */
+int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype, long long ldx, int rows, void *y,
+                             long long ldy, void *stream);
+/* Host copies of the state (any pointer may be NULL): codes [out, (in + 1) /
+ * 2] in the order above, scales [out, ceil(in / group)] as f32, bias [out]. */
+int trba_linear_int4_get(const trba_linear_int4 *l, uint8_t *codes, float *scales, float *bias);
+long long trba_linear_int4_param_count(const trba_linear_int4 *l);
 
 /* ---- LSTMInt8 (src/bilstm.rs:13-178) ---- */
 typedef struct trba_lstm_int8 trba_lstm_int8;

@@ -1,0 +1,279 @@
+"""LinearInt4 (include/trba_ops.h, trba_b200.ops): the 4-bit linear layer
+against its f64 oracle (oracle/decode_oracle.py), its quantisation, its
+refusals, and a decoding loop that reads its weights through it."""
+import ctypes as C
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import REPO
+
+sys.path.insert(0, str(REPO / "oracle"))
+import decode_oracle as do  # noqa: E402
+
+from trba_b200 import decode  # noqa: E402
+from trba_b200.ops import LinearInt4  # noqa: E402
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+# ------------------------------------------------------------ oracle (CPU) --
+def test_oracle_quantisation():
+    w = np.array([[7.0, -7.0, 0.5, -0.5, 1.5, 0.49, 3.5], [0.0] * 7, [14.0, 1.0, -1.0, 3.0, -13.1, 0.0, 5.0]], np.float32)
+    q, s = do.int4_quantize(w, 32)
+    assert s.ravel().tolist() == [1.0, 1.0, 2.0] and q.shape == (3, 4)
+    back = do.int4_weights(q, s, 7, 32)
+    assert back.tolist() == [[7, -7, 1, -1, 2, 0, 4], [0] * 7, [14, 2, -2, 4, -14, 0, 6]]
+    rng = np.random.default_rng(0)
+    w = rng.standard_normal((5, 300)).astype(np.float32)
+    q, s = do.int4_quantize(w, 128)
+    assert s.shape == (5, 3)
+    assert (np.abs(do.int4_weights(q, s, 300, 128) - w) <= 0.5001 * np.repeat(s, 128, 1)[:, :300]).all()
+
+
+# ---------------------------------------------------------- refusals (CPU) --
+def test_c_refusals(lib):
+    lib.trba_clear_error()
+
+    def refused(rc, word):
+        assert rc in (-1, None, 0) and word in lib.trba_last_error_string(), lib.trba_last_error_string()
+        assert rc != 0 or rc is None
+        lib.trba_clear_error()
+
+    p = C.c_void_p(64)
+    for ins, outs, group in ((0, 4, 32), (4, 0, 32), (4, 4, 0), (4, 4, 16), (4, 4, 48), (4, 4, 129), (4, 4, -32)):
+        refused(lib.trba_linear_int4_create(ins, outs, group, p, None), b"bad arguments")
+        refused(lib.trba_linear_int4_create_codes(ins, outs, group, p, 1 << 20, p, 0, 1 << 20, None, None), b"bad arguments")
+    refused(lib.trba_linear_int4_create(4, 4, 32, None, None), b"bad arguments")
+    for bad in ((None, 2, p, 0, 1), (p, 1, p, 0, 1), (p, 2, None, 0, 1), (p, 2, p, 1, 1), (p, 2, p, 0, 0)):
+        refused(lib.trba_linear_int4_create_codes(4, 4, 32, *bad, None, None), b"bad arguments")
+    refused(lib.trba_linear_int4_forward(None, p, 0, 4, 1, p, 4, None), b"bad arguments")
+    assert lib.trba_linear_int4_get(None, None, None, None) == -1 and lib.trba_linear_int4_param_count(None) == -1
+    lib.trba_linear_int4_destroy(None)
+    assert lib.trba_last_error() == 0
+
+
+def test_python_refusals():
+    w = np.zeros((4, 6), np.float32)
+    for kw in (dict(group=16), dict(group=100), dict(in_features=0), dict(out_features=-1)):
+        with pytest.raises(ValueError, match="LinearInt4"):
+            LinearInt4(**{**dict(in_features=6, out_features=4, weight_f32=w), **kw})
+    q, s = torch.zeros(4, 3, dtype=torch.uint8), torch.zeros(4, 1)
+    for exc, word, args, kw in (
+            (ValueError, "CUDA", (q, s), {}), (ValueError, "uint8", (q.int(), s), {}), (ValueError, "uint8", (q[:, :2], s), {}),
+            (ValueError, "scales", (q, s.double()), {}), (ValueError, "scales", (q, s[:3]), {}), (ValueError, "scales", (q, s[:, :0]), {}),
+            (ValueError, "bias", (q, s), dict(bias=torch.zeros(3))), (ValueError, "group", (q, s), dict(group=31)),
+            (TypeError, "torch tensor", (q.numpy(), s), {})):
+        with pytest.raises(exc, match=word):
+            LinearInt4.from_codes(*args, **{**dict(in_features=6, group=32), **kw})
+
+
+# ------------------------------------------------------------------- GPU --
+def layer(outs, ins, group, scales, seed, bias=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randint(0, 256, (outs, -(-ins // 2)), generator=g, device="cuda", dtype=torch.uint8)
+    s = torch.rand(outs, -(-ins // group), generator=g, device="cuda").add_(0.05).mul_(0.1).to(DTYPES[scales])
+    b = torch.randn(outs, generator=g, device="cuda") if bias else None
+    return LinearInt4.from_codes(q, s, in_features=ins, group=group, bias=b), q, s, b
+
+
+# |error|: products of a code and an activation are exact in f32; adding them
+# up 16 at a time, ins / 16 additions and at most 20 more (scales, warps,
+# bias), each off by at most 2^-23 of the sum of magnitudes (a tensor core
+# truncates), and half a step of the output's type.
+def check(y, x, q, s, b, ins, group):
+    w = do.int4_weights(q.cpu().numpy(), s.float().cpu().numpy(), ins, group)
+    xx = x.double().cpu().numpy().reshape(-1, ins)
+    want, size = xx @ w.T, np.abs(xx) @ np.abs(w).T
+    if b is not None:
+        want, size = want + b.double().cpu().numpy(), size + np.abs(b.double().cpu().numpy())
+    got = y.double().cpu().numpy().reshape(want.shape)
+    tol = (ins / 16 + 20) * 2.0 ** -23 * size + torch.finfo(y.dtype).eps / 2 * np.abs(want)
+    if y.dtype == torch.float16:
+        tol += 2.0 ** -25  # half a step of its subnormals
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("outs,ins,group", [(1, 1, 32), (3, 2, 64), (7, 31, 32), (16, 33, 32), (17, 64, 64), (130, 256, 128),
+                                            (64, 127, 64), (33, 129, 128), (100, 383, 384), (1000, 512, 64), (50, 1000, 256),
+                                            (129, 4099, 32), (20, 16384, 128), (2600, 130, 128), (31, 2048, 2048)])
+def test_forward_matches_oracle(outs, ins, group, dtype, lib, cuda):
+    for k, rows in enumerate((1, 2, 3, 5, 8, 9, 17, 40, 64, 131)):
+        lin, q, s, b = layer(outs, ins, group, ("f32", "f16")[k & 1], outs + rows, bias=k != 3)
+        g = torch.Generator(device="cuda").manual_seed(rows)
+        x = (torch.randn(rows, ins, generator=g, device="cuda") * torch.exp(torch.randn(ins, generator=g, device="cuda"))).to(DTYPES[dtype])
+        y = lin.forward(x)
+        assert y.shape == (rows, outs) and y.dtype == x.dtype
+        check(y, x, q, s, b, ins, group)
+        assert torch.equal(y, lin.forward(x))  # the same bits every time
+        lin.close()
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_rows_do_not_depend_on_each_other(dtype, cuda):
+    """A row of infinities or NaN stays in its row; a zero row gives the bias."""
+    outs, ins = 70, 300
+    lin, q, s, b = layer(outs, ins, 64, "f32", 4)
+    x = torch.randn(11, ins, device="cuda").to(DTYPES[dtype])
+    x[2], x[5, 7], x[6, 9], x[9] = float("nan"), float("inf"), float("-inf"), 0.0
+    y = lin.forward(x)
+    ok = [0, 1, 3, 4, 7, 8, 10]
+    check(y[ok], x[ok], q, s, b, ins, 64)
+    assert torch.equal(y[9], b.to(y.dtype)) and y[2].isnan().all()
+    for row, col, sign in ((5, 7, 1.0), (6, 9, -1.0)):
+        code = ((q[:, col // 2] >> (4 * (col & 1))) & 15).int() - 8
+        want = torch.where(code == 0, float("nan"), code.sign() * sign * float("inf"))
+        assert torch.equal(y[row].float().nan_to_num(7.0, 1.0, -1.0), want.nan_to_num(7.0, 1.0, -1.0))
+
+
+@pytest.mark.gpu
+def test_extreme_f32_activations(cuda):
+    """f32 activations keep all their bits: the largest, tiny ones, and ones that cancel."""
+    outs, ins = 40, 256
+    lin, q, s, _ = layer(outs, ins, 32, "f32", 6, bias=False)
+    x = torch.zeros(5, ins, device="cuda")
+    x[0, 3] = torch.finfo(torch.float32).max / 64
+    x[1, 5] = 3.3e-30
+    x[2] = 1.0 + torch.arange(ins, device="cuda") * 2.0 ** -23
+    x[3] = torch.randn(ins, device="cuda")
+    x[4] = 16777215.0
+    check(lin.forward(x), x, q, s, None, ins, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("off,ldx,ldy", [(0, 200, 66), (1, 201, 67), (3, 208, 72), (8, 256, 128)])
+def test_strides_and_leading_dimensions(off, ldx, ldy, dtype, cuda):
+    t, rows, ins, outs = DTYPES[dtype], 13, 200, 66
+    lin, q, s, b = layer(outs, ins, 64, "f16", off)
+    buf = torch.full((rows * ldx + off + 8,), float("nan"), dtype=t, device="cuda")
+    x = buf[off:off + rows * ldx].view(rows, ldx)[:, :ins]
+    x.copy_(torch.randn(rows, ins, device="cuda"))
+    ybuf = torch.full((rows * ldy + off + 8,), 9.0, dtype=t, device="cuda")
+    y = ybuf[off:off + rows * ldy].view(rows, ldy)
+    lin.forward(x, out=y[:, :outs])
+    check(y[:, :outs], x, q, s, b, ins, 64)
+    assert (y[:, outs:] == 9).all() and (ybuf[:off] == 9).all() and (ybuf[off + rows * ldy:] == 9).all()
+    want = y[:, :outs].clone()
+    assert torch.equal(lin.forward(x.contiguous()), want)
+    assert torch.equal(lin.forward(x.contiguous().view(1, rows, ins))[0], want)
+    assert torch.equal(lin.forward(x.T.contiguous().T), want)
+    assert torch.equal(lin.forward(x[4]), want[4]) and lin.forward(x[:0]).shape == (0, outs)
+
+
+@pytest.mark.gpu
+def test_quantised_layer(lib, cuda):
+    rng = np.random.default_rng(5)
+    for outs, ins, group in ((33, 300, 128), (130, 255, 64), (7, 1, 32), (64, 4096, 4096)):
+        w = rng.standard_normal((outs, ins)).astype(np.float32)
+        w[0, :32] = 0
+        b = rng.standard_normal(outs).astype(np.float32)
+        lin = LinearInt4(ins, outs, w, b, group=group)
+        st = lin.state()
+        q, s = do.int4_quantize(w, group)
+        assert np.array_equal(st["scales"], s) and np.array_equal(st["codes"], q) and np.array_equal(st["bias"], b)
+        assert lin.param_count() == outs * ins + outs
+        x = torch.randn(4, ins, device="cuda")
+        check(lin.forward(x), x, torch.from_numpy(q), torch.from_numpy(s), torch.from_numpy(b), ins, group)
+    lin, q, s, b = layer(19, 77, 32, "f16", 1)
+    st = lin.state()
+    codes = q.cpu().numpy()
+    codes[:, -1] = (codes[:, -1] & 15) | (st["codes"][:, -1] & 0xF0)  # behind the last input: no code
+    assert np.array_equal(st["codes"], codes) and np.array_equal(st["scales"], s.float().cpu().numpy())
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_forward_refusals(lib, cuda):
+    lin, *_ = layer(8, 40, 32, "f32", 0)
+    x = torch.zeros(2, 40, device="cuda")
+    for exc, word, args, kw in ((TypeError, "float32", (x.double(),), {}), (ValueError, "in_features", (x[:, :39],), {}),
+                                (ValueError, "CUDA", (x.cpu(),), {}), (ValueError, "out must be", (x,), dict(out=x)),
+                                (ValueError, "apart", (x,), dict(out=torch.zeros(1, 8, device="cuda").expand(2, 8))),
+                                (TypeError, "torch tensor", (x.cpu().numpy(),), {})):
+        with pytest.raises(exc, match=word):
+            lin.forward(*args, **kw)
+    lib.trba_clear_error()
+    p = C.c_void_p(x.data_ptr())
+    for args, word in (((None, 0, 40, 1, p, 8), b"bad arguments"), ((p, 0, 39, 1, p, 8), b"bad arguments"), ((p, 0, 40, -1, p, 8), b"bad arguments"),
+                       ((p, 0, 40, 1, p, 7), b"bad arguments"), ((p, 3, 40, 1, p, 8), b"element type"),
+                       ((C.c_void_p(x.data_ptr() + 2), 0, 40, 1, p, 8), b"not aligned")):
+        assert lib.trba_linear_int4_forward(lin.h, *args, None) == -1 and word in lib.trba_last_error_string()
+        lib.trba_clear_error()
+    assert lib.trba_linear_int4_forward(lin.h, None, 0, 40, 0, None, 8, None) == 0
+    lin.close()
+    lin.close()
+
+
+@pytest.mark.gpu
+def test_captured_on_two_streams(cuda):
+    """Two graphs of one layer run at once and on new inputs."""
+    lin, q, s, b = layer(300, 1111, 64, "f16", 8)
+    xs = [torch.randn(5, 1111, device="cuda").bfloat16() for _ in range(4)]
+    want = [lin.forward(x) for x in xs]
+    graphs = []
+    for k in range(2):
+        buf = xs[k].clone()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = lin.forward(buf)
+        graphs.append((g, buf, y, torch.cuda.Stream()))
+    for r in range(2):
+        for k, (g, buf, y, st) in enumerate(graphs):
+            with torch.cuda.stream(st):
+                buf.copy_(xs[2 * r + k])
+                g.replay()
+        torch.cuda.synchronize()
+        for k, (_, _, y, _) in enumerate(graphs):
+            assert torch.equal(y, want[2 * r + k])
+    st = torch.cuda.Stream()
+    y = lin.forward(xs[0], stream=st)
+    st.synchronize()
+    assert torch.equal(y, want[0])
+
+
+@pytest.mark.gpu
+def test_beam_search_through_the_layer(lib, cuda):
+    """The operators as they are used together: an LSTM decoder whose gates and
+    vocabulary are 4-bit layers, searched with beams; every step's logits
+    against f64, every choice against the oracle on those logits."""
+    from test_decode import check_step
+    L, K, V, H, T, eos = 3, 4, 131, 96, 9, 2
+    rng = np.random.default_rng(12)
+    wg, wo = rng.standard_normal((4 * H, 2 * H)).astype(np.float32) * 0.2, rng.standard_normal((V, H)).astype(np.float32)
+    gates = LinearInt4(2 * H, 4 * H, wg, rng.standard_normal(4 * H).astype(np.float32), group=64)
+    gen = LinearInt4(H, V, wo, None, group=32)
+    emb = torch.randn(V, H, device="cuda")
+    wo_q = do.int4_quantize(wo, 32)
+    h = torch.zeros(L * K, H, device="cuda")
+    c = torch.zeros_like(h)
+    scores = torch.full((L, K), float("-inf"), device="cuda")
+    scores[:, 0] = 0
+    fin, tokens = torch.zeros(L, K, dtype=torch.bool, device="cuda"), torch.ones(L, K, dtype=torch.int32, device="cuda")
+    hist = []
+    for _ in range(T):
+        i, f, g, o = gates.forward(torch.cat([emb[tokens.view(-1).long()], h], 1)).chunk(4, 1)
+        c = torch.sigmoid(f) * c + torch.sigmoid(i) * torch.tanh(g)
+        h = torch.sigmoid(o) * torch.tanh(c)
+        logits = gen.forward(h)
+        check(logits, h, torch.from_numpy(wo_q[0]), torch.from_numpy(wo_q[1]), None, H, 32)
+        step = decode.beam_select(logits, scores, fin, eos=eos)
+        check_step(step, logits, scores, fin, eos)
+        before = h
+        h, c = decode.beam_reorder([h, c], step.parents)
+        assert torch.equal(h.view(L, K, H)[1, 2], before.view(L, K, H)[1, step.parents[1, 2]])
+        scores, tokens, fin = step.scores, step.tokens, step.finished
+        hist.append(step)
+    seq, n = decode.beam_sequences(torch.stack([s.tokens for s in hist]), torch.stack([s.parents for s in hist]), eos=eos)
+    want = do.beam_sequences(*(np.stack([x.cpu().numpy() for x in xs]) for xs in
+                               ([s.tokens for s in hist], [s.parents for s in hist])), eos, 0)
+    assert np.array_equal(seq.cpu().numpy(), want[0]) and np.array_equal(n.cpu().numpy(), want[1])
+    assert lib.trba_last_error() == 0

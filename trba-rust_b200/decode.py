@@ -1,0 +1,306 @@
+"""Beam-search operators on torch CUDA tensors (include/trba_decode.h).
+
+    step = beam_select(logits, scores, finished, eos=2)   # scores, tokens, parents, finished
+    h, c = beam_reorder([h, c], step.parents)             # the states follow their beams
+    seqs, lengths = beam_sequences(tokens, parents, eos=2)
+
+Work is queued on torch's current stream of the tensors' device, or on
+``stream`` (a torch.cuda.Stream); outputs belong to that stream.  Arguments
+are checked here: a ValueError or TypeError means that nothing ran.
+"""
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple, Sequence
+
+import torch
+
+from .ffi import lib
+
+MAX_BEAMS = 32
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class BeamStep(NamedTuple):
+    scores: torch.Tensor    # [lines, beams] float32
+    tokens: torch.Tensor    # [lines, beams] int32
+    parents: torch.Tensor   # [lines, beams] int32
+    finished: torch.Tensor  # [lines, beams] bool
+
+
+def _fail(L, what, rc):
+    raise RuntimeError(f"{what} failed ({rc}): " + L.trba_last_error_string().decode())
+
+
+class on_stream:
+    """Makes `stream` (None: the current one) and the tensors' device current
+    for one call; `.ptr` is the stream handle."""
+    __slots__ = ("device", "stream", "ptr", "ctx")
+
+    def __init__(self, device: torch.device, stream):
+        self.device, self.stream, self.ctx = device, stream, None
+
+    def __enter__(self):
+        index = self.device.index
+        if self.stream is not None:
+            if self.stream.device != self.device:
+                raise ValueError(f"stream is on {self.stream.device}, the tensors are on {self.device}")
+            self.ctx = torch.cuda.stream(self.stream)
+            self.ctx.__enter__()
+        elif index != torch.cuda.current_device():
+            self.ctx = torch.cuda.device(index)
+            self.ctx.__enter__()
+        self.ptr = torch.cuda.current_stream(index).cuda_stream
+        return self
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _check_tensors(**tensors):
+    for name, t in tensors.items():
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+
+
+def _check_cuda(name, t, device=None):
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _check_device(**tensors) -> torch.device:
+    """The one CUDA device that all tensors are on."""
+    device = None
+    for name, t in tensors.items():
+        if t is not None:
+            _check_cuda(name, t, device)
+            device = t.device
+    return device
+
+
+def _check_beams(beams):
+    if not 1 <= beams <= MAX_BEAMS:
+        raise ValueError(f"1 to {MAX_BEAMS} beams are supported, got {beams}")
+
+
+def _check_out(name, t, shape, dtype, device):
+    _check_tensors(**{name: t})
+    _check_cuda(name, t, device)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None, *, eos: int = -1,
+                out: BeamStep | None = None, stream=None) -> BeamStep:
+    """The best `beams` continuations of every line by running score plus log
+    softmax of the logits, best first, ties to the lowest (beam, token).
+
+    logits [lines * beams, vocab] or [lines, beams, vocab], float32, bfloat16
+    or float16, any row stride; scores [lines, beams] float32, -inf for a dead
+    beam; finished [lines, beams] bool or uint8, or None.  A finished beam
+    continues with `eos` at an unchanged score.  A line with too few
+    continuations above -inf fills up with score -inf, token eos, parent = the
+    slot.  A NaN logit counts as -inf.  `out`: buffers to write into; its
+    scores and finished may be the inputs'."""
+    _check_tensors(scores=scores, logits=logits, finished=finished)
+    code = DTYPE_CODES.get(logits.dtype)
+    if code is None:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if scores.dim() != 2 or scores.dtype != torch.float32:
+        raise ValueError("scores must be a float32 tensor [lines, beams]")
+    lines, beams = scores.shape
+    _check_beams(beams)
+    vocab = logits.shape[-1]
+    if logits.dim() == 3:
+        if logits.shape[0] != lines or logits.shape[1] != beams:
+            raise ValueError(f"logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
+        if lines > 1 and logits.stride(0) != beams * logits.stride(1):
+            raise ValueError("logits must have one stride over all (line, beam) rows")
+        ld = logits.stride(1) if beams > 1 else logits.stride(0)
+    elif logits.dim() == 2:
+        if logits.shape[0] != lines * beams:
+            raise ValueError(f"logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
+        ld = logits.stride(0)
+    else:
+        raise ValueError("logits must be [lines * beams, vocab] or [lines, beams, vocab]")
+    if vocab < 1 or beams * vocab >= 1 << 31:
+        raise ValueError("vocab must be positive and beams * vocab below 2**31")
+    if vocab > 1 and logits.stride(-1) != 1:
+        raise ValueError("the logits of a row must be contiguous")
+    if lines * beams > 1:
+        if ld < vocab:
+            raise ValueError("logits rows overlap")
+    else:
+        ld = vocab
+    if not -1 <= eos < vocab:
+        raise ValueError(f"eos must be -1 or in [0, {vocab}), got {eos}")
+    if finished is not None:
+        if eos < 0:
+            raise ValueError("finished beams need an end token (eos)")
+        if finished.shape != scores.shape or finished.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("finished must be a bool or uint8 tensor [lines, beams]")
+    device = _check_device(scores=scores, logits=logits, finished=finished)
+    with on_stream(device, stream) as s:
+        scores, fin = scores.contiguous(), None
+        if finished is not None:
+            finished = finished.contiguous()
+            fin = finished.data_ptr()
+        if out is None:
+            shape = (lines, beams)
+            out = BeamStep(torch.empty(shape, dtype=torch.float32, device=device),
+                           torch.empty(shape, dtype=torch.int32, device=device),
+                           torch.empty(shape, dtype=torch.int32, device=device),
+                           torch.empty(shape, dtype=torch.bool, device=device))
+        else:
+            out = BeamStep(*out)
+            for name, t, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32, torch.bool)):
+                _check_out(f"out.{name}", t, (lines, beams), dtype, device)
+        if lines:
+            L = lib()
+            rc = L.trba_beam_select(logits.data_ptr(), code, ld, scores.data_ptr(), fin, lines, beams, vocab, eos,
+                                    out.scores.data_ptr(), out.tokens.data_ptr(), out.parents.data_ptr(),
+                                    out.finished.data_ptr(), s.ptr)
+            if rc:
+                _fail(L, "beam_select", rc)
+    return out
+
+
+def _collapse(shape, src, dst, size):
+    """(count, src stride, dst stride) triples, in bytes, outermost first, with
+    neighbours merged where both tensors walk on without a gap."""
+    dims = []
+    for n, a, b in zip(shape, src, dst):
+        if n == 1:
+            continue
+        a, b = a * size, b * size
+        if dims and dims[-1][1] == n * a and dims[-1][2] == n * b:
+            dims[-1] = (dims[-1][0] * n, a, b)
+        else:
+            dims.append((n, a, b))
+    return dims
+
+
+def _state(src, dst, dim):
+    """The ten fields of a trba_beam_state for one tensor and its output."""
+    size, shape = src.element_size(), src.shape
+    outer = _collapse(shape[:dim], src.stride()[:dim], dst.stride()[:dim], size)
+    inner = _collapse(shape[dim + 1:], src.stride()[dim + 1:], dst.stride()[dim + 1:], size)
+    nbytes = size
+    if inner and inner[-1][1] == size and inner[-1][2] == size:
+        nbytes *= inner.pop()[0]
+    if len(outer) > 1 or len(inner) > 1:
+        raise ValueError(f"state of shape {tuple(shape)} and strides {src.stride()}: at most one gap before and one "
+                         "after the beam dimension are supported; make it contiguous")
+    o, om = outer[0] if outer else (1, 0, 0), inner[0] if inner else (1, 0, 0)
+    return (src.data_ptr(), dst.data_ptr(), nbytes, src.stride(dim) * size, dst.stride(dim) * size, *om, *o)
+
+
+def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: int = 0,
+                 out: Sequence[torch.Tensor] | None = None, stream=None) -> list[torch.Tensor]:
+    """Row (l, k) of every state becomes row (l, parents[l, k]).
+
+    states: tensors of any type whose dimension `dim` is lines * beams, for
+    instance h and c [lines * beams, hidden], stacked layers [layers, lines *
+    beams, hidden] (dim=1) or the filled part of a cache, cache[:, :, :n];
+    parents [lines, beams] int32 as beam_select returns them.  Returns new
+    tensors, or writes into `out` (the same shapes and types, not overlapping
+    any state: keep two sets and use them in turn)."""
+    states = list(states)
+    _check_tensors(parents=parents, **{f"states[{i}]": t for i, t in enumerate(states)})
+    if parents.dim() != 2 or parents.dtype != torch.int32:
+        raise ValueError("parents must be an int32 tensor [lines, beams]")
+    lines, beams = parents.shape
+    _check_beams(beams)
+    for i, t in enumerate(states):
+        if not -t.dim() <= dim < t.dim():
+            raise ValueError(f"states[{i}] has no dimension {dim}")
+        if t.shape[dim] != lines * beams:
+            raise ValueError(f"states[{i}]: dimension {dim} is {t.shape[dim]}, expected lines * beams = {lines * beams}")
+    if out is not None:
+        out = list(out)
+        if len(out) != len(states):
+            raise ValueError(f"out has {len(out)} tensors for {len(states)} states")
+        for i, (t, o) in enumerate(zip(states, out)):
+            _check_tensors(**{f"out[{i}]": o})
+            if o.shape != t.shape or o.dtype != t.dtype:
+                raise ValueError(f"out[{i}] must have the shape and type of states[{i}]")
+        _check_apart(states, out)
+    device = _check_device(parents=parents)
+    for i, t in enumerate(states):
+        _check_cuda(f"states[{i}]", t, device)
+    for i, t in enumerate(out or ()):
+        _check_cuda(f"out[{i}]", t, device)
+    with on_stream(device, stream) as s:
+        parents = parents.contiguous()
+        if out is None:
+            out = [torch.empty(t.shape, dtype=t.dtype, device=device) for t in states]
+        fields = []
+        n = 0
+        for t, o in zip(states, out):
+            if t.numel():
+                fields += _state(t, o, dim % t.dim())
+                n += 1
+        if n:
+            L = lib()
+            rc = L.trba_beam_reorder(struct.pack(f"={len(fields)}q", *fields), n, parents.data_ptr(), lines, beams,
+                                     s.ptr)
+            if rc:
+                _fail(L, "beam_reorder", rc)
+    return out
+
+
+def _span(t):
+    """First and one-past-last byte that a tensor's elements reach."""
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_apart(states, out):
+    spans = [(_span(t), f"states[{i}]") for i, t in enumerate(states) if t.numel()]
+    for i, o in enumerate(out):
+        if not o.numel():
+            continue
+        if any(st == 0 and n > 1 for n, st in zip(o.shape, o.stride())):
+            raise ValueError(f"out[{i}] is a broadcast view")
+        lo, hi = _span(o)
+        for (a, b), name in spans:
+            if lo < b and a < hi:
+                raise ValueError(f"out[{i}] overlaps {name}: reordering in place is not supported")
+
+
+def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1, pad: int = 0, out=None,
+                   stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(sequences [lines, beams, steps] int32, lengths [lines, beams] int32) of
+    the paths that end in the last step's slots, from the [steps, lines,
+    beams] int32 tokens and parents of all steps: each path's tokens before
+    its first `eos`, then `pad`."""
+    _check_tensors(tokens=tokens, parents=parents)
+    if tokens.dim() != 3 or tokens.dtype != torch.int32 or parents.shape != tokens.shape or parents.dtype != torch.int32:
+        raise ValueError("tokens and parents must be int32 tensors [steps, lines, beams]")
+    steps, lines, beams = tokens.shape
+    _check_beams(beams)
+    for name, v in (("eos", eos), ("pad", pad)):
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{name} must fit in 32 bits, got {v}")
+    device = _check_device(tokens=tokens, parents=parents)
+    with on_stream(device, stream) as s:
+        tokens, parents = tokens.contiguous(), parents.contiguous()
+        if out is None:
+            out = (torch.empty((lines, beams, steps), dtype=torch.int32, device=device),
+                   torch.empty((lines, beams), dtype=torch.int32, device=device))
+        else:
+            seq, lengths = out
+            _check_out("out[0]", seq, (lines, beams, steps), torch.int32, device)
+            _check_out("out[1]", lengths, (lines, beams), torch.int32, device)
+            out = (seq, lengths)
+        if lines:
+            L = lib()
+            rc = L.trba_beam_sequences(tokens.data_ptr(), parents.data_ptr(), steps, lines, beams, eos, pad,
+                                       out[0].data_ptr(), out[1].data_ptr(), s.ptr)
+            if rc:
+                _fail(L, "beam_sequences", rc)
+    return out

@@ -7,6 +7,9 @@ rand::thread_rng), and all state lives on the device.
     lin = LinearInt8(in_features, out_features, weight_f32, bias)
     out = lin.forward(inp_int8)                   # [rows*out] int32
     clip = lin.backward(inp_f32, grad_out, lr, mom)
+
+LinearInt4, beside them, is a linear layer with 4-bit weights for decoding; it
+works on torch CUDA tensors.
 """
 from __future__ import annotations
 
@@ -103,6 +106,132 @@ class LinearInt8:
 
     def param_count(self) -> int:
         return int(self.L.trba_linear_int8_param_count(self.h))
+
+
+class LinearInt4:
+    """Linear layer with 4-bit weights and one scale per `group` inputs, for
+    the few rows of a decoding step (include/trba_ops.h):
+
+        lin = LinearInt4(in_features, out_features, weight_f32, bias, group=128)
+        y = lin.forward(x)     # torch CUDA tensors, [rows, in] -> [rows, out]
+
+    No counterpart in the reference."""
+
+    def __init__(self, in_features: int, out_features: int, weight_f32: np.ndarray, bias: np.ndarray | None = None,
+                 group: int = 128):
+        """Quantises f32 weights [out, in] (host): per group, scale = max |w| /
+        7 and code - 8 = round(w / scale)."""
+        self._check_sizes(in_features, out_features, group)
+        w = np.ascontiguousarray(weight_f32, np.float32).reshape(out_features * in_features)
+        b = None if bias is None else np.ascontiguousarray(bias, np.float32).reshape(out_features)
+        self._own(in_features, out_features, group,
+                  lib().trba_linear_int4_create(in_features, out_features, group, _p(w), None if b is None else _p(b)))
+
+    @staticmethod
+    def _check_sizes(in_features, out_features, group):
+        if in_features < 1 or out_features < 1:
+            raise ValueError(f"LinearInt4: sizes must be positive, got {in_features} -> {out_features}")
+        if group not in (32, 64) and (group < 128 or group % 128):
+            raise ValueError(f"LinearInt4: group must be 32, 64 or a multiple of 128, got {group}")
+
+    def _own(self, in_features, out_features, group, handle):
+        import torch
+        self.L = lib()
+        self.in_features, self.out_features, self.group, self.h = in_features, out_features, group, handle
+        if not handle:
+            raise _err(self.L, "LinearInt4")
+        self.device = torch.device("cuda", torch.cuda.current_device())
+
+    @classmethod
+    def from_codes(cls, codes, scales, *, in_features: int, group: int = 128, bias=None) -> "LinearInt4":
+        """From quantised weights on the GPU: codes [out, ceil(in / 2)] uint8,
+        the even input's code in the low half; scales [out, ceil(in / group)]
+        float32 or float16; bias [out] float32 or None.  W = (code - 8) *
+        scale.  The tensors are copied."""
+        import torch
+        from .decode import DTYPE_CODES, _check_device, _check_tensors, on_stream
+        _check_tensors(codes=codes, scales=scales, bias=bias)
+        if in_features < 1 or codes.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[1] != -(-in_features // 2):
+            raise ValueError(f"codes must be a uint8 tensor [out, {-(-in_features // 2)}]")
+        out_features = codes.shape[0]
+        cls._check_sizes(in_features, out_features, group)
+        if scales.dtype not in (torch.float32, torch.float16) or tuple(scales.shape) != (out_features,
+                                                                                       -(-in_features // group)):
+            raise ValueError(f"scales must be float32 or float16 [{out_features}, {-(-in_features // group)}]")
+        if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (out_features,)):
+            raise ValueError(f"bias must be float32 [{out_features}]")
+        device = _check_device(codes=codes, scales=scales, bias=bias)
+        self = cls.__new__(cls)
+        with on_stream(device, None) as s:
+            codes, scales = codes.contiguous(), scales.contiguous()
+            bias = None if bias is None else bias.contiguous()
+            self._own(in_features, out_features, group, lib().trba_linear_int4_create_codes(
+                in_features, out_features, group, codes.data_ptr(), codes.shape[1], scales.data_ptr(),
+                DTYPE_CODES[scales.dtype], scales.shape[1], None if bias is None else bias.data_ptr(), s.ptr))
+        return self
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.L.trba_linear_int4_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def forward(self, x, out=None, stream=None):
+        """[rows, in] -> [rows, out] of the same type (float32, bfloat16 or
+        float16); leading dimensions of x are rows.  Runs on torch's current
+        stream, or on `stream` (a torch.cuda.Stream)."""
+        import torch
+        from .decode import DTYPE_CODES, _check_cuda, _check_tensors, on_stream
+        _check_tensors(x=x, out=out)
+        code = DTYPE_CODES.get(x.dtype)
+        if code is None:
+            raise TypeError(f"LinearInt4::forward: x must be float32, bfloat16 or float16, got {x.dtype}")
+        if x.dim() < 1 or x.shape[-1] != self.in_features:
+            raise ValueError(f"LinearInt4::forward: x {tuple(x.shape)} does not end in in_features {self.in_features}")
+        shape = x.shape[:-1] + (self.out_features,)
+        _check_cuda("x", x, self.device)
+        with on_stream(self.device, stream) as s:
+            if x.dim() != 2:
+                x = x.reshape(-1, self.in_features)
+            rows = x.shape[0]
+            if (self.in_features > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < self.in_features):
+                x = x.contiguous()
+            if out is None:
+                out = torch.empty(shape, dtype=x.dtype, device=self.device)
+                ldy = self.out_features
+            else:
+                _check_cuda("out", out, self.device)
+                if out.shape != shape or out.dtype != x.dtype:
+                    raise ValueError(f"LinearInt4::forward: out must be {x.dtype} {tuple(shape)}")
+                if out.dim() != 2 and not out.is_contiguous():
+                    raise ValueError("LinearInt4::forward: out must be contiguous")
+                ldy = out.stride(0) if out.dim() == 2 and rows > 1 else self.out_features
+                if ldy < self.out_features or (self.out_features > 1 and out.stride(-1) != 1):
+                    raise ValueError("LinearInt4::forward: the rows of out must be contiguous and apart")
+            if rows:
+                ldx = x.stride(0) if rows > 1 else self.in_features
+                rc = self.L.trba_linear_int4_forward(self.h, x.data_ptr(), code, ldx, rows, out.data_ptr(), ldy, s.ptr)
+                if rc:
+                    raise _err(self.L, "LinearInt4::forward")
+        return out
+
+    def state(self) -> dict:
+        """Host copies: codes [out, ceil(in / 2)] uint8, scales [out, groups]
+        float32, bias [out] float32."""
+        n, g = self.out_features, -(-self.in_features // self.group)
+        q, s = np.empty((n, -(-self.in_features // 2)), np.uint8), np.empty((n, g), np.float32)
+        b = np.empty(n, np.float32)
+        if self.L.trba_linear_int4_get(self.h, _p(q), _p(s), _p(b)) != 0:
+            raise _err(self.L, "LinearInt4 state")
+        return {"codes": q, "scales": s, "bias": b}
+
+    def param_count(self) -> int:
+        return int(self.L.trba_linear_int4_param_count(self.h))
 
 
 class LSTMInt8:
