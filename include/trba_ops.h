@@ -88,7 +88,7 @@ trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_feature
 void trba_linear_int4_destroy(trba_linear_int4 *l);
 /* x [rows, in] and y [rows, out] on the device, both of `dtype` (TRBA_F32,
  * TRBA_BF16, TRBA_F16), row strides ldx >= in and ldy >= out in elements; y
- * must not overlap x.  rows = 0 is an empty call. */
+ * must not overlap x.  0 (an empty call) to 2^20 rows. */
 int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype, long long ldx, int rows, void *y,
                              long long ldy, void *stream);
 /* Host copies of the state (any pointer may be NULL): codes [out, (in + 1) /
