@@ -2,11 +2,11 @@
 // decoding step (include/trba_ops.h, LinearInt4).  No counterpart in the
 // reference; the quantisation rule is LinearInt8's (src/linear.rs:53-59) for
 // 4 bits and groups.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <cstdlib>
 #include <new>
 
 #include "common.cuh"
@@ -36,8 +36,6 @@ struct trba_linear_int4 {
 
 namespace trba {
 namespace {
-
-namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -111,6 +109,8 @@ __global__ void __launch_bounds__(256) int4_natural_kernel(const uint32_t *__res
 }
 
 // ----------------------------------------------------------------- forward --
+constexpr int kDepth = 6;  // stages of a warp's ring
+
 // y^T = W x^T on the tensor cores: A is a 16-output tile of the weights, the
 // codes turned into exact bf16 or f16 integers in registers, B the
 // activations from shared memory, eight columns at a time.  An f32
@@ -118,17 +118,18 @@ __global__ void __launch_bounds__(256) int4_natural_kernel(const uint32_t *__res
 // products with the codes are exact in all types, and a group's sum is
 // accumulated in f32 before its scale multiplies it.
 //
-// What bounds it: at one row, reading the codes (half a byte a weight).  The
-// legacy mma is enough for that: a 1 KB block of codes costs 8 mma per eight
-// columns and about 90 integer and conversion instructions.
+// What bounds it: at few rows, reading the codes (half a byte a weight).  The
+// warp-level mma is enough for that: a 1 KB block of codes costs 8 mma per
+// eight columns and about 90 integer and conversion instructions.
 //
-// A CTA is 8 warps, wn tiles by wk interleaved parts of its inputs; a
-// cluster of `cs` CTAs splits the inputs once more and adds its parts through
-// distributed shared memory, so there is no workspace and the order of every
-// sum is fixed.  Each warp streams its blocks through its own ring of
-// cp.async stages, which are in flight while the activations are staged.
-constexpr int kWarps = 8, kDepth = 6;
-
+// One CTA a SM for the whole product: its tiles are a contiguous share of all
+// of them, its warps are `wn` units of MT tiles by `wk` interleaved parts of
+// the inputs.  Every warp streams its blocks, over all its tiles, through a
+// ring of cp.async stages of its own, so that loads stay in flight while
+// activations are staged, sums are joined and outputs written.  Activations
+// are staged in slabs of inputs, each once a CTA, all tiles running over one
+// slab before the next; sums wait in shared memory in between.  The order of
+// every sum is fixed.
 struct Args {
     const uint8_t *codes, *scales;
     const float *bias;
@@ -136,11 +137,13 @@ struct Args {
     void *y;
     i64 ldx, ldy;
     int in, out, rows, dtype;
-    int tiles, chunks, group, gpc, groups_pad, scale_f16;
-    int wn, cs;          // wk = kWarps / wn
-    int slab;            // chunks whose activations are staged at once, a multiple of wk
+    int tiles, chunks, gpc, groups_pad, scale_f16;
+    int cpg;             // chunks a group has (1 for groups of up to 128)
+    int wn;              // wk = warps / wn
+    int slab;            // chunks whose activations are staged at once
     int block_rows;      // rows a CTA takes
-    int cols;            // columns they make (3 a row for f32)
+    int packed;          // f32: columns 3 r + p of a single column tile (else p * rows + r)
+    int xs_at, red_at, sums_at;  // shared memory: ring, activations, partial sums, sums between slabs
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
@@ -151,15 +154,16 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
 }
 
 template <bool F16>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+    const float z0 = first ? 0.0f : c[0], z1 = first ? 0.0f : c[1], z2 = first ? 0.0f : c[2], z3 = first ? 0.0f : c[3];
     if (F16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
 }
 
 // Codes at bits 4 j and 4 j + 16 of a word as a pair of floats, code - 8: the
@@ -179,41 +183,68 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Eight activations of one row from k on (zero behind `in`) as 16-bit columns.
-__device__ __forceinline__ void stage8(const Args &a, int row, int k, uint8_t *dst, int pitch) {
+// Eight f32 or 16-bit activations of one row, zero behind the last input.
+struct Eight {
+    uint4 lo, hi;  // 16-bit types use lo only
+};
+__device__ __forceinline__ Eight load8(const Args &a, i64 row, int k) {
+    Eight v;
+    v.lo = v.hi = make_uint4(0, 0, 0, 0);
     if (a.dtype != TRBA_F32) {
         const uint16_t *src = static_cast<const uint16_t *>(a.x) + row * a.ldx + k;
-        uint4 v = make_uint4(0, 0, 0, 0);
         if (k + 8 <= a.in && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-            v = *reinterpret_cast<const uint4 *>(src);
+            v.lo = *reinterpret_cast<const uint4 *>(src);
+        } else if (k >= 8 && k + 16 <= a.in) {  // the two aligned blocks it lies in are all of this row
+            const uintptr_t at = reinterpret_cast<uintptr_t>(src);
+            const uint4 *p = reinterpret_cast<const uint4 *>(at & ~(uintptr_t)15);
+            const uint4 q0 = p[0], q1 = p[1];
+            const uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+            const int by = ((int)at & 15) >> 2, sh = ((int)at & 2) * 8;
+            uint32_t s[5];
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+                s[i] = by == 0 ? w[i] : by == 1 ? w[min(i + 1, 7)] : by == 2 ? w[min(i + 2, 7)] : w[min(i + 3, 7)];
+            v.lo = make_uint4(__funnelshift_r(s[0], s[1], sh), __funnelshift_r(s[1], s[2], sh),
+                              __funnelshift_r(s[2], s[3], sh), __funnelshift_r(s[3], s[4], sh));
         } else {
             uint16_t h[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[i] = k + i < a.in ? src[i] : (uint16_t)0;
-            v.x = h[0] | (uint32_t)h[1] << 16, v.y = h[2] | (uint32_t)h[3] << 16;
-            v.z = h[4] | (uint32_t)h[5] << 16, v.w = h[6] | (uint32_t)h[7] << 16;
+            v.lo = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                              h[6] | (uint32_t)h[7] << 16);
         }
-        *reinterpret_cast<uint4 *>(dst) = v;
+    } else {
+        const uint32_t *src = static_cast<const uint32_t *>(a.x) + row * a.ldx + k;
+        if (k + 8 <= a.in && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+            v.lo = reinterpret_cast<const uint4 *>(src)[0];
+            v.hi = reinterpret_cast<const uint4 *>(src)[1];
+        } else {
+            uint32_t f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = k + i < a.in ? src[i] : 0u;
+            v.lo = make_uint4(f[0], f[1], f[2], f[3]);
+            v.hi = make_uint4(f[4], f[5], f[6], f[7]);
+        }
+    }
+    return v;
+}
+
+// Stores them as one 16-bit column, or as three bf16 columns, `apart` bytes
+// from each other, that add up to the f32 values: truncated to 8 bits three
+// times (an infinity or NaN goes into the first alone).
+__device__ __forceinline__ void store8(const Args &a, const Eight &v, uint8_t *dst, int apart) {
+    if (a.dtype != TRBA_F32) {
+        *reinterpret_cast<uint4 *>(dst) = v.lo;
         return;
     }
-    const float *src = static_cast<const float *>(a.x) + row * a.ldx + k;
-    float f[8];
-    if (k + 8 <= a.in && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        const float4 lo = reinterpret_cast<const float4 *>(src)[0], hi = reinterpret_cast<const float4 *>(src)[1];
-        f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = k + i < a.in ? src[i] : 0.0f;
-    }
+    const uint32_t f[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
     uint32_t part[3][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // truncated to 8 bits three times: hi + mid + lo is the value; an
-        // infinity or NaN goes in whole
-        const bool finite = fabsf(f[i]) <= 3.402823466e38f;
-        const uint32_t h = finite ? __float_as_uint(f[i]) & 0xffff0000u
-                                  : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(f[i])) << 16;
-        const float r1 = finite ? f[i] - __uint_as_float(h) : 0.0f;
+        const float x = __uint_as_float(f[i]);
+        const bool finite = fabsf(x) <= 3.402823466e38f;
+        const uint32_t h = finite ? f[i] & 0xffff0000u : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(x)) << 16;
+        const float r1 = finite ? x - __uint_as_float(h) : 0.0f;
         const uint32_t m = __float_as_uint(r1) & 0xffff0000u;
         const uint32_t l = __float_as_uint(r1 - __uint_as_float(m)) & 0xffff0000u;
         const uint32_t q[3] = {h, m, l};
@@ -222,147 +253,248 @@ __device__ __forceinline__ void stage8(const Args &a, int row, int k, uint8_t *d
     }
 #pragma unroll
     for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<uint4 *>(dst + (i64)p * pitch) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+        *reinterpret_cast<uint4 *>(dst + p * apart) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
 }
 
-// WG: words (32 inputs) a group has in a chunk; NT: tiles of eight columns.
-template <bool F16, int WG, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_forward_kernel(const __grid_constant__ Args a) {
+// WG: words (32 inputs) a group has in a chunk; NT: tiles of eight columns;
+// MT: tiles of 16 outputs a warp takes at once, so that it reads the
+// activations from shared memory once for all of them; W: warps.
+template <bool F16, int WG, int NT, int MT, int W>
+__global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int wk_n = kWarps / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
-    const int rank = blockIdx.x % a.cs, tile = (blockIdx.x / a.cs) * a.wn + wn;
-    const int per = ((a.chunks + a.cs - 1) / a.cs + wk_n - 1) / wk_n * wk_n;  // chunks of a CTA
-    const int c0 = rank * per, nc = max(0, min(a.chunks, c0 + per) - c0);
+    const int wk_n = W / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
+    const int units = (a.tiles + MT - 1) / MT;
+    const int u0 = (int)((i64)units * blockIdx.x / gridDim.x) + wn;
+    const int u1 = (int)((i64)units * (blockIdx.x + 1) / gridDim.x);
     const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
-    const int split = a.dtype == TRBA_F32 ? 3 : 1, cols = rows * split;
-    const int es = a.scale_f16 ? 2 : 4, sb = 16 * a.gpc * es, slot = 1024 + sb;
+    const int split = a.dtype == TRBA_F32 ? 3 : 1;
+    const int es = a.scale_f16 ? 2 : 4, sb = 16 * a.gpc * es, part = 1024 + sb, slot = MT * part;
     const int pitch = a.slab * 256 + 64;  // 64 mod 128: eight lanes' 16-byte reads meet 32 different banks
     uint8_t *ring = smem + warp * kDepth * slot;
-    uint8_t *xs = smem + kWarps * kDepth * slot;
-    const uint32_t ring_s = smem_addr(ring);
-    const int mine = tile < a.tiles && wk < nc ? (nc - wk + wk_n - 1) / wk_n : 0;
-    const uint8_t *src = a.codes + ((i64)tile * a.chunks + c0 + wk) * 1024;
-    const uint8_t *ssrc = a.scales + (i64)tile * a.groups_pad * 16 * es;
+    uint8_t *xs = smem + a.xs_at;
 
-    auto issue = [&](int i) {
-        if (i < mine) {
-            const uint32_t dst = ring_s + (i % kDepth) * slot;
-            const uint8_t *p = src + (i64)i * wk_n * 1024;
-            cp16(dst + lane * 16, p + lane * 16);
-            cp16(dst + 512 + lane * 16, p + 512 + lane * 16);
-            if (lane * 16 < sb) {
-                const int chunk = c0 + wk + i * wk_n;
-                const int g = WG < 4 ? chunk * (4 / WG) : (int)((i64)chunk * 128 / a.group);
-                cp16(dst + 1024 + lane * 16, ssrc + (i64)g * 16 * es + lane * 16);
+    // the stream of this warp's blocks: for each slab, for each of its units, every wk_n-th chunk
+    int pu = u0, pend = min(a.slab, a.chunks), pc = wk, pbase = 0;
+    const uint8_t *psrc = a.codes, *pscale = a.scales;
+    bool fresh = true;
+    uint32_t dst = smem_addr(ring) + lane * 16;
+    const uint32_t dst_end = dst + kDepth * slot;
+    auto issue = [&]() {
+        while (pc >= pend || pu >= u1) {
+            if (pu < u1) {
+                pu += a.wn;
             }
+            if (pu >= u1) {
+                if (pend >= a.chunks || u0 >= u1) {
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    return;
+                }
+                pu = u0;
+                pbase = pend;
+                pend = min(pend + a.slab, a.chunks);
+            }
+            pc = pbase + wk;
+            fresh = true;
         }
+        if (fresh) {
+            psrc = a.codes + ((i64)pu * MT * a.chunks + pc) * 1024 + lane * 16;
+            pscale = a.scales + (i64)pu * MT * a.groups_pad * 16 * es + lane * 16;
+            fresh = false;
+        }
+        const int g = WG < 4 ? pc * (4 / WG) : a.cpg == 1 ? pc : pc / a.cpg;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (m && pu * MT + m >= a.tiles) break;  // (the sums of a tile that is not there are not stored)
+            const uint8_t *p = psrc + (i64)m * a.chunks * 1024;
+            cp16(dst + m * part, p);
+            cp16(dst + m * part + 512, p + 512);
+            if (lane * 16 < sb) cp16(dst + m * part + 1024, pscale + ((i64)m * a.groups_pad + g) * 16 * es);
+        }
+        psrc += wk_n * 1024;
+        pc += wk_n;
+        dst += slot;
+        if (dst == dst_end) dst -= kDepth * slot;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int i = 0; i < kDepth - 1; ++i) issue(i);
+    for (int i = 0; i < kDepth - 1; ++i) issue();
 
-    float tot[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
     const int g = lane >> 2, t = lane & 3;
-    int i = 0;
-    for (int s0 = 0; s0 < nc; s0 += a.slab) {
-        const int sc = min(a.slab, nc - s0);
+    // a column of mma depends on its own activations alone: lanes behind the
+    // last column read it again
+    const uint8_t *xcol[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        int col = n * 8 + g;
+        if (split == 1 || a.packed) {
+            col = min(col, rows * split - 1);
+        } else {
+            constexpr int kPer = (NT + 2) / 3;
+            col = (n / kPer) * rows + min((n % kPer) * 8 + g, rows - 1);
+        }
+        xcol[n] = xs + col * pitch + t * 16;
+    }
+    const uint8_t *blk = ring;
+    int turn = 0;  // partial-sum buffers are used in turn
+    for (int s0 = 0; s0 < a.chunks; s0 += a.slab) {
+        const int sc = min(a.slab, a.chunks - s0), n8 = sc * 16;
         if (s0) __syncthreads();
-        for (int e = threadIdx.x; e < rows * sc * 16; e += kWarps * 32) {
-            const int r = e / (sc * 16), k8 = e - r * sc * 16;
-            stage8(a, row0 + r, (c0 + s0) * 128 + k8 * 8, xs + (i64)r * split * pitch + k8 * 16, pitch);
+        // four loads in flight a thread
+        for (int e0 = threadIdx.x; e0 < rows * n8; e0 += 4 * W * 32) {
+            Eight v[4];
+            int r[4], k[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int e = e0 + u * W * 32;
+                r[u] = e / n8, k[u] = e - r[u] * n8;
+                if (r[u] < rows) v[u] = load8(a, row0 + r[u], s0 * 128 + k[u] * 8);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (r[u] < rows)
+                    store8(a, v[u], xs + (a.packed ? 3 * r[u] : r[u]) * pitch + k[u] * 16,
+                           a.packed ? pitch : rows * pitch);
         }
         __syncthreads();
-        for (; i < mine && wk + i * wk_n < s0 + sc; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
-            __syncwarp();
-            issue(i + kDepth - 1);
-            const uint8_t *blk = ring + (i % kDepth) * slot;
-            const uint4 lo = *reinterpret_cast<const uint4 *>(blk + lane * 16);
-            const uint4 hi = *reinterpret_cast<const uint4 *>(blk + 512 + lane * 16);
-            const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-            const uint8_t *xk = xs + (wk + i * wk_n - s0) * 256 + t * 16;
-            float c[NT][4];
+        for (int u = u0; u < u1; u += a.wn, turn ^= 1) {
+            float tot[MT][NT][4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if (w % WG == 0) {
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
+                for (int n = 0; n < NT; ++n) tot[m][n][0] = tot[m][n][1] = tot[m][n][2] = tot[m][n][3] = 0.0f;
+            for (int ck = wk; ck < sc; ck += wk_n) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+                __syncwarp();
+                issue();
+                const int xo = ck * 256;
+                uint32_t wl[MT][4], wh[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const uint4 lo = *reinterpret_cast<const uint4 *>(blk + m * part + lane * 16);
+                    const uint4 hi = *reinterpret_cast<const uint4 *>(blk + m * part + 512 + lane * 16);
+                    wl[m][0] = lo.x, wl[m][1] = lo.y, wl[m][2] = lo.z, wl[m][3] = lo.w;
+                    wh[m][0] = hi.x, wh[m][1] = hi.y, wh[m][2] = hi.z, wh[m][3] = hi.w;
                 }
-                uint32_t a0[4], a1[4];
-                a0[0] = code_pair<F16>(wl[w]), a0[1] = code_pair<F16>(wh[w]);
-                a0[2] = code_pair<F16>(wl[w] >> 4), a0[3] = code_pair<F16>(wh[w] >> 4);
-                a1[0] = code_pair<F16>(wl[w] >> 8), a1[1] = code_pair<F16>(wh[w] >> 8);
-                a1[2] = code_pair<F16>(wl[w] >> 12), a1[3] = code_pair<F16>(wh[w] >> 12);
+                float c[MT][NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint4 b = make_uint4(0, 0, 0, 0);
-                    if (n * 8 + g < cols) b = *reinterpret_cast<const uint4 *>(xk + (n * 8 + g) * pitch + w * 64);
-                    mma<F16>(c[n], a0, b.x, b.y);
-                    mma<F16>(c[n], a1, b.z, b.w);
-                }
-                if (w % WG == WG - 1) {
-                    float s0f, s1f;
-                    const uint8_t *sp = blk + 1024 + (w / WG) * 16 * es;
-                    if (a.scale_f16) {
-                        s0f = __half2float(reinterpret_cast<const __half *>(sp)[g]);
-                        s1f = __half2float(reinterpret_cast<const __half *>(sp)[g + 8]);
-                    } else {
-                        s0f = reinterpret_cast<const float *>(sp)[g];
-                        s1f = reinterpret_cast<const float *>(sp)[g + 8];
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t a0[MT][4], a1[MT][4];
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        a0[m][0] = code_pair<F16>(wl[m][w]), a0[m][1] = code_pair<F16>(wh[m][w]);
+                        a0[m][2] = code_pair<F16>(wl[m][w] >> 4), a0[m][3] = code_pair<F16>(wh[m][w] >> 4);
+                        a1[m][0] = code_pair<F16>(wl[m][w] >> 8), a1[m][1] = code_pair<F16>(wh[m][w] >> 8);
+                        a1[m][2] = code_pair<F16>(wl[m][w] >> 12), a1[m][3] = code_pair<F16>(wh[m][w] >> 12);
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        tot[n][0] = fmaf(s0f, c[n][0], tot[n][0]);
-                        tot[n][1] = fmaf(s0f, c[n][1], tot[n][1]);
-                        tot[n][2] = fmaf(s1f, c[n][2], tot[n][2]);
-                        tot[n][3] = fmaf(s1f, c[n][3], tot[n][3]);
+                        const uint4 b = *reinterpret_cast<const uint4 *>(xcol[n] + xo + w * 64);
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            mma<F16>(c[m][n], a0[m], b.x, b.y, w % WG == 0);
+                            mma<F16>(c[m][n], a1[m], b.z, b.w, false);
+                        }
                     }
+                    if (w % WG == WG - 1) {
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            float s0f, s1f;
+                            const uint8_t *sp = blk + m * part + 1024 + (w / WG) * 16 * es;
+                            if (a.scale_f16) {
+                                s0f = __half2float(reinterpret_cast<const __half *>(sp)[g]);
+                                s1f = __half2float(reinterpret_cast<const __half *>(sp)[g + 8]);
+                            } else {
+                                s0f = reinterpret_cast<const float *>(sp)[g];
+                                s1f = reinterpret_cast<const float *>(sp)[g + 8];
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                tot[m][n][0] = fmaf(s0f, c[m][n][0], tot[m][n][0]);
+                                tot[m][n][1] = fmaf(s0f, c[m][n][1], tot[m][n][1]);
+                                tot[m][n][2] = fmaf(s1f, c[m][n][2], tot[m][n][2]);
+                                tot[m][n][3] = fmaf(s1f, c[m][n][3], tot[m][n][3]);
+                            }
+                        }
+                    }
+                }
+                blk += slot;
+                if (blk == ring + kDepth * slot) blk = ring;
+            }
+            // join the wk_n warps of the unit; two buffers in turn, so that a
+            // buffer is written again only after the next unit's barrier
+            constexpr int kFrag = MT * NT;  // float4 of a lane
+            if (wk_n > 1) {
+                float4 *red = reinterpret_cast<float4 *>(smem + a.red_at) +
+                              ((i64)(turn * a.wn + wn) * (wk_n - 1)) * kFrag * 32 + lane;
+                if (wk > 0) {
+#pragma unroll
+                    for (int f = 0; f < kFrag; ++f) {
+                        const float *v = tot[f / NT][f % NT];
+                        red[((wk - 1) * kFrag + f) * 32] = make_float4(v[0], v[1], v[2], v[3]);
+                    }
+                }
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + wn), "r"(wk_n * 32) : "memory");
+                if (wk > 0) continue;
+                for (int k = 0; k < wk_n - 1; ++k)
+#pragma unroll
+                    for (int f = 0; f < kFrag; ++f) {
+                        const float4 v = red[(k * kFrag + f) * 32];
+                        float *o = tot[f / NT][f % NT];
+                        o[0] += v.x, o[1] += v.y, o[2] += v.z, o[3] += v.w;
+                    }
+            }
+            if (a.slab < a.chunks) {
+                float4 *sums = reinterpret_cast<float4 *>(smem + a.sums_at) + (i64)(u - (u0 - wn)) * kFrag * 32 + lane;
+#pragma unroll
+                for (int f = 0; f < kFrag; ++f) {
+                    float *o = tot[f / NT][f % NT];
+                    if (s0) {
+                        const float4 v = sums[f * 32];
+                        o[0] += v.x, o[1] += v.y, o[2] += v.z, o[3] += v.w;
+                    }
+                    if (s0 + sc < a.chunks) sums[f * 32] = make_float4(o[0], o[1], o[2], o[3]);
+                }
+                if (s0 + sc < a.chunks) continue;
+            }
+            // outputs u * MT * 16 + 16 m + g and + 8 of the rows in this lane's columns
+            auto put = [&](int r, int n, float v) {
+                if (r >= rows || n >= a.out) return;
+                v += a.bias[n];
+                const i64 at = (row0 + r) * a.ldy + n;
+                if (a.dtype == TRBA_F32) static_cast<float *>(a.y)[at] = v;
+                else if (a.dtype == TRBA_BF16) static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(v);
+                else static_cast<__half *>(a.y)[at] = __float2half_rn(v);
+            };
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int n0 = (u * MT + m) * 16 + g;
+                if (split == 1) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8, tot[m][n][q]);
+                } else if (NT == 1) {  // packed: columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float v[3];
+#pragma unroll
+                            for (int p = 0; p < 3; ++p)
+                                v[p] = __shfl_sync(kFull, tot[m][0][2 * h + ((3 * r + p) & 1)], 4 * g + (3 * r + p) / 2);
+                            if (t == r) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
+                        }
+                } else if (NT % 3 == 0) {
+#pragma unroll
+                    for (int n = 0; n < NT / 3; ++n)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8,
+                                tot[m][n][q] + (tot[m][n + NT / 3][q] + tot[m][n + 2 * (NT / 3)][q]));
                 }
             }
         }
     }
-    // partial sums [wk][output][column] over the ring and the activations
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    constexpr int kCols = NT * 8 + 1;
-    float *red = reinterpret_cast<float *>(smem);
-    const int outs = a.wn * 16;
-    {
-        float *p = red + ((i64)wk * outs + wn * 16 + g) * kCols + 2 * t;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            p[n * 8] = tot[n][0], p[n * 8 + 1] = tot[n][1];
-            p[8 * kCols + n * 8] = tot[n][2], p[8 * kCols + n * 8 + 1] = tot[n][3];
-        }
-    }
-    __syncthreads();
-    if (a.cs > 1) {
-        for (int e = threadIdx.x; e < outs * kCols; e += kWarps * 32)
-            for (int k = 1; k < wk_n; ++k) red[e] += red[(i64)k * outs * kCols + e];
-        cg::this_cluster().sync();
-    }
-    const int n0 = (blockIdx.x / a.cs) * outs;
-    for (int e = threadIdx.x + rank * kWarps * 32; e < rows * outs; e += kWarps * 32 * a.cs) {
-        const int r = e / outs, o = e - r * outs;
-        if (n0 + o >= a.out) continue;
-        float v[3] = {0.0f, 0.0f, 0.0f};
-        for (int p = 0; p < split; ++p) {
-            const int at = o * kCols + r * split + p;
-            if (a.cs > 1) {
-                for (int k = 0; k < a.cs; ++k) v[p] += *cg::this_cluster().map_shared_rank(red + at, k);
-            } else {
-                for (int k = 0; k < wk_n; ++k) v[p] += red[(i64)k * outs * kCols + at];
-            }
-        }
-        const float sum = v[0] + (v[1] + v[2]) + a.bias[n0 + o];
-        const i64 at = (row0 + r) * a.ldy + n0 + o;
-        if (a.dtype == TRBA_F32) static_cast<float *>(a.y)[at] = sum;
-        else if (a.dtype == TRBA_BF16) static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(sum);
-        else static_cast<__half *>(a.y)[at] = __float2half_rn(sum);
-    }
-    if (a.cs > 1) cg::this_cluster().sync();  // no CTA leaves while its sums are read
 }
 
 int launched() {
@@ -372,46 +504,40 @@ int launched() {
     return (int)e;
 }
 
-constexpr int kMaxCols = 64;
-constexpr int kSlabBytes = 48 * 1024;
+constexpr int kMaxSmem = 227 * 1024;
+constexpr int kMaxJoin = 48 * 1024;  // shared memory of the warps' partial sums
 
-template <bool F16, int WG, int NT>
-int launch(const Args &a, int blocks_x, int blocks_y, size_t smem, cudaStream_t st) {
-    auto fn = int4_forward_kernel<F16, WG, NT>;
+template <bool F16, int WG, int NT, int MT, int W>
+int launch(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
+    auto fn = int4_forward_kernel<F16, WG, NT, MT, W>;
     static std::atomic<unsigned long long> sized{0};  // one bit a device: its limit has been raised
     int dev = 0;
     cudaGetDevice(&dev);
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(sized.load(std::memory_order_relaxed) & bit)) {
         const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(fn),
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
         if (e != cudaSuccess) {
             report_error(__FILE__, __LINE__, cudaGetErrorString(e), (int)e);
             return (int)e;
         }
         sized.fetch_or(bit, std::memory_order_relaxed);
     }
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = a.cs, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks_x, blocks_y);
-    cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, fn, a);
+    fn<<<grid, W * 32, smem, st>>>(a);
     return launched();
 }
 
 template <bool F16, int WG>
-int launch_nt(const Args &a, int bx, int by, int cols, size_t smem, cudaStream_t st) {
-    const int nt = (cols + 7) / 8;
-    if (nt <= 1) return launch<F16, WG, 1>(a, bx, by, smem, st);
-    if (nt <= 2) return launch<F16, WG, 2>(a, bx, by, smem, st);
-    if (nt <= 4) return launch<F16, WG, 4>(a, bx, by, smem, st);
-    return launch<F16, WG, 8>(a, bx, by, smem, st);
+int launch_nt(const Args &a, int nt, dim3 grid, size_t smem, cudaStream_t st) {
+    switch (nt) {
+        case 1: return launch<F16, WG, 1, 1, 16>(a, grid, smem, st);
+        case 2: return launch<F16, WG, 2, 1, 16>(a, grid, smem, st);
+        case 3: return launch<F16, WG, 3, 2, 8>(a, grid, smem, st);
+        case 4: return launch<F16, WG, 4, 2, 8>(a, grid, smem, st);
+        case 5: return launch<F16, WG, 5, 2, 8>(a, grid, smem, st);
+        case 6: return launch<F16, WG, 6, 2, 8>(a, grid, smem, st);
+        default: return launch<F16, WG, 8, 2, 8>(a, grid, smem, st);
+    }
 }
 
 int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int rows, void *y, i64 ldy, cudaStream_t st) {
@@ -419,37 +545,65 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
     a.codes = l->codes, a.scales = l->scales, a.bias = l->bias;
     a.x = x, a.y = y, a.ldx = ldx, a.ldy = ldy;
     a.in = l->in, a.out = l->out, a.rows = rows, a.dtype = dtype;
-    a.tiles = l->tiles, a.chunks = l->chunks, a.group = l->group, a.gpc = l->gpc;
+    a.tiles = l->tiles, a.chunks = l->chunks, a.gpc = l->gpc;
+    a.cpg = l->group >= 128 ? l->group / 128 : 1;
     a.groups_pad = l->groups_pad, a.scale_f16 = l->scale_dtype == TRBA_F16;
-    const int split = dtype == TRBA_F32 ? 3 : 1, most = kMaxCols / split;
-    const int blocks_y = (rows + most - 1) / most;
+    // rows of a CTA: up to 64 columns, an f32 row being three (16 rows make six tiles of them)
+    const bool f32 = dtype == TRBA_F32;
+    const int most = f32 ? 16 : 64, blocks_y = (rows + most - 1) / most;
     a.block_rows = (rows + blocks_y - 1) / blocks_y;
-    a.cols = a.block_rows * split;
-    const int target = 2 * sm_count();
-    a.wn = kWarps;
-    while (a.wn > 1 && (a.tiles + a.wn - 1) / a.wn * blocks_y < target) a.wn >>= 1;
-    const int wk = kWarps / a.wn;
-    const int blocks = (a.tiles + a.wn - 1) / a.wn;
-    a.cs = 1;
-    while (a.cs < 8 && blocks * blocks_y * a.cs < sm_count() && a.chunks >= 2 * a.cs * wk * 2) a.cs *= 2;
-    const int per = ((a.chunks + a.cs - 1) / a.cs + wk - 1) / wk * wk;
-    a.slab = (kSlabBytes / a.cols - 64) / 256 / wk * wk;
-    if (a.slab < wk) a.slab = wk;
-    if (a.slab > per) a.slab = per;
-    const size_t slot = 1024 + 16 * a.gpc * (a.scale_f16 ? 2 : 4);
-    const int nt = a.cols <= 8 ? 1 : a.cols <= 16 ? 2 : a.cols <= 32 ? 4 : 8;
-    size_t smem = kWarps * kDepth * slot + (size_t)a.cols * (a.slab * 256 + 64);
-    const size_t red = (size_t)kWarps * 16 * (nt * 8 + 1) * 4;
-    if (smem < red) smem = red;
-    const int wg = l->group >= 128 ? 4 : l->group / 32, bx = blocks * a.cs;
-    if (dtype == TRBA_F16) {
-        if (wg == 1) return launch_nt<true, 1>(a, bx, blocks_y, a.cols, smem, st);
-        if (wg == 2) return launch_nt<true, 2>(a, bx, blocks_y, a.cols, smem, st);
-        return launch_nt<true, 4>(a, bx, blocks_y, a.cols, smem, st);
+    a.packed = f32 && a.block_rows <= 2;
+    int nt = f32 ? (a.packed ? 1 : a.block_rows <= 8 ? 3 : 6) : (a.block_rows + 7) / 8;
+    if (nt == 7) nt = 8;
+    const int mt = nt <= 2 ? 1 : 2, warps = nt <= 2 ? 16 : 8;
+    const int cols = a.block_rows * (f32 ? 3 : 1);
+    i64 smem = 0;
+    const int units = (a.tiles + mt - 1) / mt;
+    const int frag = mt * nt * 512;  // bytes of one unit's sums
+    const int ring = warps * kDepth * mt * (1024 + 16 * a.gpc * (a.scale_f16 ? 2 : 4));
+    const auto x_bytes = [&](int chunks) { return ((i64)cols * (chunks * 256 + 64) + 127) & ~127ll; };
+    int ctas = units < sm_count() ? units : sm_count();
+    for (;; ctas = ctas * 2 < units ? ctas * 2 : units) {
+        const int share = (units + ctas - 1) / ctas;  // units of a CTA, at most
+        // Units of a CTA that run side by side: the fewest steps of (chunks a
+        // warp streams + the join of the warps that share a unit).
+        long long best = -1;
+        int red = 0;
+        for (int wn = warps; wn >= 1; wn >>= 1) {
+            const int wk = warps / wn, bytes = 2 * wn * (wk - 1) * frag;
+            const long long steps = (share + wn - 1) / wn;
+            const long long cost = steps * (4 * ((a.chunks + wk - 1) / wk) + (wk > 1 ? 4 + wk : 0));
+            if (bytes <= kMaxJoin && (best < 0 || cost < best)) best = cost, a.wn = wn, red = bytes;
+        }
+        if (const char *e = getenv("TUNE_WN")) a.wn = atoi(e), red = 2 * a.wn * (warps / a.wn - 1) * frag;
+        // All activations at once where they fit; else as many chunks as fit
+        // beside the sums that wait between slabs.  Sums that leave no room
+        // for a slab of a few chunks go to more CTAs.
+        const i64 room = kMaxSmem - ring - red;
+        i64 sums = 0;
+        a.slab = a.chunks;
+        if (x_bytes(a.chunks) > room) {
+            sums = (i64)share * frag;
+            a.slab = (int)(((room - sums - 128) / cols - 64) / 256);
+            if (a.slab < 4 && ctas < units) continue;
+        }
+        if (const char *e = getenv("TUNE_SLAB")) a.slab = atoi(e), sums = (i64)share * frag;
+        a.xs_at = ring;
+        a.red_at = a.xs_at + (int)x_bytes(a.slab);
+        a.sums_at = a.red_at + red;
+        smem = a.sums_at + sums;
+        break;
     }
-    if (wg == 1) return launch_nt<false, 1>(a, bx, blocks_y, a.cols, smem, st);
-    if (wg == 2) return launch_nt<false, 2>(a, bx, blocks_y, a.cols, smem, st);
-    return launch_nt<false, 4>(a, bx, blocks_y, a.cols, smem, st);
+    const int wg = l->group >= 128 ? 4 : l->group / 32;
+    const dim3 grid(ctas, blocks_y);
+    if (dtype == TRBA_F16) {
+        if (wg == 1) return launch_nt<true, 1>(a, nt, grid, smem, st);
+        if (wg == 2) return launch_nt<true, 2>(a, nt, grid, smem, st);
+        return launch_nt<true, 4>(a, nt, grid, smem, st);
+    }
+    if (wg == 1) return launch_nt<false, 1>(a, nt, grid, smem, st);
+    if (wg == 2) return launch_nt<false, 2>(a, nt, grid, smem, st);
+    return launch_nt<false, 4>(a, nt, grid, smem, st);
 }
 
 template <class S>
