@@ -15,22 +15,22 @@
 
 // Weight layout, made once when a layer is created: outputs in tiles of 16,
 // inputs in chunks of 128, so that a warp streams one tile's chunks as
-// consecutive 1 KB blocks with fully coalesced 16-byte loads that are already
-// the A fragments of mma.m16n8k16.  In a block, lane l = 4 g + t has 16 bytes
-// of row g (first 512 bytes) and 16 of row g + 8; their word w holds the
-// codes of inputs 32 w + 8 t .. + 7, so the four lanes of a row cover 32
-// consecutive inputs a word and every group size from 32 on ends between
-// words.  Inside a word, codes 2 j and 2 j + 1 sit 16 bits apart at bit 4 j:
-// one shift, mask and or makes them a pair of 16-bit floats.  Scales: [tile]
-// [group][16 rows].  Codes behind the last input or output are 8 (zero).
+// consecutive blocks whose 16-byte pieces are already the A fragments of
+// mma.m16n8k16.  A block is 1 KB of codes and the scales of its 16 rows.  In
+// the codes, lane l = 4 g + t has 16 bytes of row g (first 512 bytes) and 16
+// of row g + 8; their word w holds the codes of inputs 32 w + 8 t .. + 7, so
+// the four lanes of a row cover 32 consecutive inputs a word and every group
+// size from 32 on ends between words.  Inside a word, codes 2 j and 2 j + 1
+// sit 16 bits apart at bit 4 j: one shift, mask and or makes them a pair of
+// 16-bit floats.  Scales: [128 / group][16 rows]; a group of several chunks
+// has its scale once a chunk (at most 6% more to read), so that all blocks
+// look the same.  Codes behind the last input or output are 8 (zero).
 struct trba_linear_int4 {
     int in = 0, out = 0, group = 0, groups = 0, device = 0, scale_dtype = 0;
     int tiles = 0, chunks = 0;
-    int gpc = 0;                // groups a chunk touches (1 for groups of 128 and more)
-    int groups_pad = 0;         // groups a tile has room for
-    uint8_t *base = nullptr;    // one allocation: codes, scales, bias
-    uint8_t *codes = nullptr;   // [tiles][chunks][1024]
-    uint8_t *scales = nullptr;  // [tiles][groups_pad][16] f32 or f16
+    int gpc = 0;                // scales of a row in a chunk (1 for groups of 128 and more)
+    int block = 0;              // bytes of a block: 1024 + 16 gpc scales
+    uint8_t *base = nullptr;    // one allocation: blocks [tiles][chunks], bias
     float *bias = nullptr;      // [out]
 };
 
@@ -65,51 +65,63 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const float *__restr
     }
 }
 
-// Natural codes [out][pitch] and scales [out][groups] -> the layout above, one
-// thread a 4-byte word of codes and one a scale.
+// Natural codes [out][pitch] and scales [out][groups] -> the layout above: a
+// warp a block, a lane 8 words of codes, then the scales.
 template <class S>
 __global__ void __launch_bounds__(256) int4_layout_kernel(const uint8_t *__restrict__ codes, i64 pitch,
                                                           const S *__restrict__ scales, i64 ld_scales, int in, int out,
-                                                          int groups, int groups_pad, int tiles, int chunks,
-                                                          uint32_t *__restrict__ words, S *__restrict__ dst) {
-    const i64 n_words = (i64)tiles * chunks * 256, n_scales = (i64)tiles * groups_pad * 16;
-    GRID_LOOP(e, n_words + n_scales) {
-        if (e < n_words) {
-            const int w = (int)(e & 3), l = (int)(e >> 2) & 31, half = (int)(e >> 7) & 1;
-            const i64 block = e >> 8, tile = block / chunks;
-            const int n = (int)tile * 16 + half * 8 + (l >> 2);
-            const int k0 = (int)(block - tile * chunks) * 128 + w * 32 + (l & 3) * 8;
-            uint32_t v = 0;
-            for (int c = 0; c < 8; ++c) {
-                const int k = k0 + c;
-                const uint32_t q = n < out && k < in ? (codes[n * pitch + (k >> 1)] >> (4 * (k & 1))) & 15u : 8u;
-                v |= q << (4 * (c >> 1) + 16 * (c & 1));
+                                                          int group, int groups, int gpc, int tiles, int chunks,
+                                                          int block, uint8_t *__restrict__ dst) {
+    const int lane = threadIdx.x & 31;
+    const i64 step = (i64)gridDim.x * 8;
+    for (i64 e = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); e < (i64)tiles * chunks; e += step) {
+        const i64 tile = e / chunks;
+        const int chunk = (int)(e - tile * chunks);
+        uint8_t *out_block = dst + e * block;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const i64 n = tile * 16 + half * 8 + (lane >> 2);
+            uint32_t v[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int k0 = chunk * 128 + w * 32 + (lane & 3) * 8;
+                v[w] = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const int k = k0 + c;
+                    const uint32_t q = n < out && k < in ? (codes[n * pitch + (k >> 1)] >> (4 * (k & 1))) & 15u : 8u;
+                    v[w] |= q << (4 * (c >> 1) + 16 * (c & 1));
+                }
             }
-            words[e] = v;
-        } else {
-            const i64 f = e - n_words, tg = f >> 4, tile = tg / groups_pad;
-            const int n = (int)tile * 16 + (int)(f & 15), g = (int)(tg - tile * groups_pad);
-            dst[f] = n < out && g < groups ? scales[n * ld_scales + g] : S(0.0f);
+            reinterpret_cast<uint4 *>(out_block + half * 512)[lane] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        for (int f = lane; f < gpc * 16; f += 32) {
+            const i64 n = tile * 16 + (f & 15), g = ((i64)chunk * 128 + (i64)(f >> 4) * 32 * (4 / gpc)) / group;
+            reinterpret_cast<S *>(out_block + 1024)[f] = n < out && g < groups ? scales[n * ld_scales + g] : S(0.0f);
         }
     }
 }
 
 // The reverse, for the host copies of the state.
-__global__ void __launch_bounds__(256) int4_natural_kernel(const uint32_t *__restrict__ words, int in, int out,
-                                                           int chunks, uint8_t *__restrict__ codes) {
+__global__ void __launch_bounds__(256) int4_natural_kernel(const uint8_t *__restrict__ base, int in, int out,
+                                                           int chunks, int block, uint8_t *__restrict__ codes) {
     const int pitch = (int)(((i64)in + 1) / 2);
     GRID_LOOP(e, (i64)out * pitch) {
         const i64 n = e / pitch;
         const int k = (int)(e - n * pitch) * 2;
         const int half = (int)(n >> 3) & 1, l = (int)(n & 7) * 4 + ((k >> 3) & 3), w = (k >> 5) & 3;
-        const uint32_t v = words[(((n >> 4) * chunks + (k >> 7)) * 2 + half) * 128 + l * 4 + w];
+        const uint32_t v = reinterpret_cast<const uint32_t *>(base + ((n >> 4) * chunks + (k >> 7)) * block)[half * 128 + l * 4 + w];
         const int c = k & 7;
         codes[e] = (uint8_t)(((v >> (2 * c)) & 15u) | (((v >> (2 * c + 16)) & 15u) << 4));
     }
 }
 
 // ----------------------------------------------------------------- forward --
-constexpr int kDepth = 6;  // stages of a warp's ring
+constexpr int kPair = 2;  // blocks of a stage
+// One column tile needs few registers: 32 warps hide more latency.  Stages of
+// a warp's ring: 64 KB are in flight a SM either way.
+constexpr int warps_of(int nt) { return nt == 1 ? 32 : 16; }
+constexpr int depth_of(int warps) { return warps == 32 ? 2 : 3; }
 
 // y^T = W x^T on the tensor cores: A is a 16-output tile of the weights, the
 // codes turned into exact bf16 or f16 integers in registers, B the
@@ -123,7 +135,7 @@ constexpr int kDepth = 6;  // stages of a warp's ring
 // eight columns and about 90 integer and conversion instructions.
 //
 // One CTA a SM for the whole product: its tiles are a contiguous share of all
-// of them, its warps are `wn` units of MT tiles by `wk` interleaved parts of
+// of them, its warps are `wn` tiles by `wk` parts of
 // the inputs.  Every warp streams its blocks, over all its tiles, through a
 // ring of cp.async stages of its own, so that loads stay in flight while
 // activations are staged, sums are joined and outputs written.  Activations
@@ -131,21 +143,22 @@ constexpr int kDepth = 6;  // stages of a warp's ring
 // slab before the next; sums wait in shared memory in between.  The order of
 // every sum is fixed.
 struct Args {
-    const uint8_t *codes, *scales;
+    const uint8_t *blocks;
     const float *bias;
     const void *x;
     void *y;
     i64 ldx, ldy;
     int in, out, rows, dtype;
-    int tiles, chunks, gpc, groups_pad, scale_f16;
-    int cpg;             // chunks a group has (1 for groups of up to 128)
-    int wn;              // wk = warps / wn
+    int tiles, chunks, gpc;
+    int wn;              // wk = W / wn
     int slab;            // chunks whose activations are staged at once
     int block_rows;      // rows a CTA takes
     int packed;          // f32: columns 3 r + p of a single column tile (else p * rows + r)
     int xs_at, red_at, sums_at;  // shared memory: ring, activations, partial sums, sums between slabs
 };
 
+__device__ __forceinline__ float scale_f32(float v) { return v; }
+__device__ __forceinline__ float scale_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -166,21 +179,47 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
 }
 
-// Codes at bits 4 j and 4 j + 16 of a word as a pair of floats, code - 8: the
-// code is or-ed into the mantissa of 128 (bf16) or 1024 (f16), where one step
-// is 1, and 136 or 1032 is subtracted; both exact.
-template <bool F16>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+// (w & mask) | bits in one instruction (left to itself the compiler takes two)
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
     uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+__device__ __forceinline__ uint32_t bf162_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+
+// The four pairs of a word (codes at bits 4 j and 4 j + 16) as floats, exact,
+// with one shift a word.
+// f16: the code is or-ed into the mantissa of 1024 at either of two places,
+// the upper one worth 16 times as much: code - 8.
+// bf16 has room for one place behind 128.  The place above it needs no
+// magic number: the bits of exponent 0 and of exponent 1 count in the same
+// steps of 2^-133, so a code at bits 4 .. 7 is code * 2^-129 and times 2^127
+// a quarter of itself.  All pairs come as (code - 8) / 4; kUnit undoes it.
+template <bool F16>
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t &p0, uint32_t &p1, uint32_t &p2, uint32_t &p3) {
+    const uint32_t v = w >> 8;
     if (F16) {
-        r = (w & 0x000f000fu) | 0x64006400u;
-        const __half2 v = __hsub2(*reinterpret_cast<__half2 *>(&r), __half2half2(__ushort_as_half(0x6408)));
-        return *reinterpret_cast<const uint32_t *>(&v);
+        const __half2 low = __half2half2(__ushort_as_half(0x6408)),   // 1032
+            sixteenth = __half2half2(__ushort_as_half(0x2c00)), high = __half2half2(__ushort_as_half(0xd480));  // -72
+        const uint32_t q0 = and_or(w, 0x000f000fu, 0x64006400u), q1 = and_or(w, 0x00f000f0u, 0x64006400u);
+        const uint32_t q2 = and_or(v, 0x000f000fu, 0x64006400u), q3 = and_or(v, 0x00f000f0u, 0x64006400u);
+        p0 = half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&q0), low));
+        p1 = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&q1), sixteenth, high));
+        p2 = half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&q2), low));
+        p3 = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&q3), sixteenth, high));
+    } else {
+        const __nv_bfloat162 quarter = __bfloat162bfloat162(__ushort_as_bfloat16(0x3e80)),
+                             low = __bfloat162bfloat162(__ushort_as_bfloat16(0xc208)),    // -34
+            up = __bfloat162bfloat162(__ushort_as_bfloat16(0x7f00)),                      // 2^127
+            high = __bfloat162bfloat162(__ushort_as_bfloat16(0xc000));                    // -2
+        const uint32_t q0 = and_or(w, 0x000f000fu, 0x43004300u), q1 = w & 0x00f000f0u;
+        const uint32_t q2 = and_or(v, 0x000f000fu, 0x43004300u), q3 = v & 0x00f000f0u;
+        p0 = bf162_bits(__hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&q0), quarter, low));
+        p1 = bf162_bits(__hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&q1), up, high));
+        p2 = bf162_bits(__hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&q2), quarter, low));
+        p3 = bf162_bits(__hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&q3), up, high));
     }
-    r = (w & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 v =
-        __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&r), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
-    return *reinterpret_cast<const uint32_t *>(&v);
 }
 
 // Eight f32 or 16-bit activations of one row, zero behind the last input.
@@ -256,65 +295,59 @@ __device__ __forceinline__ void store8(const Args &a, const Eight &v, uint8_t *d
         *reinterpret_cast<uint4 *>(dst + p * apart) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
 }
 
-// WG: words (32 inputs) a group has in a chunk; NT: tiles of eight columns;
-// MT: tiles of 16 outputs a warp takes at once, so that it reads the
-// activations from shared memory once for all of them; W: warps.
-template <bool F16, int WG, int NT, int MT, int W>
+// S: type of the scales; WG: words (32 inputs) a group has in a chunk; NT:
+// tiles of eight columns; W: warps.
+template <bool F16, class S, int WG, int NT, int W>
 __global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wk_n = W / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
-    const int units = (a.tiles + MT - 1) / MT;
-    const int u0 = (int)((i64)units * blockIdx.x / gridDim.x) + wn;
-    const int u1 = (int)((i64)units * (blockIdx.x + 1) / gridDim.x);
+    const int t0 = (int)((i64)a.tiles * blockIdx.x / gridDim.x) + wn;
+    const int t1 = (int)((i64)a.tiles * (blockIdx.x + 1) / gridDim.x);
     const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
     const int split = a.dtype == TRBA_F32 ? 3 : 1;
-    const int es = a.scale_f16 ? 2 : 4, sb = 16 * a.gpc * es, part = 1024 + sb, slot = MT * part;
+    constexpr int kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S), kSlot = kPair * kBlock, kDepth = depth_of(W);
     const int pitch = a.slab * 256 + 64;  // 64 mod 128: eight lanes' 16-byte reads meet 32 different banks
-    uint8_t *ring = smem + warp * kDepth * slot;
-    uint8_t *xs = smem + a.xs_at;
+    const int ring = warp * kDepth * kSlot;  // offsets in shared memory
 
-    // the stream of this warp's blocks: for each slab, for each of its units, every wk_n-th chunk
-    int pu = u0, pend = min(a.slab, a.chunks), pc = wk, pbase = 0;
-    const uint8_t *psrc = a.codes, *pscale = a.scales;
-    bool fresh = true;
-    uint32_t dst = smem_addr(ring) + lane * 16;
-    const uint32_t dst_end = dst + kDepth * slot;
+    // the stream of this warp's stages: for each slab, for each of its tiles, its part of the chunks
+    int ptile = t0 - a.wn, pslab = t0 < t1 ? 0 : a.chunks, left = 0;
+    const uint8_t *psrc = a.blocks;
+    const uint32_t ring_s = smem_addr(smem) + ring + lane * 16;
+    uint32_t dst = ring_s;
     auto issue = [&]() {
-        while (pc >= pend || pu >= u1) {
-            if (pu < u1) {
-                pu += a.wn;
-            }
-            if (pu >= u1) {
-                if (pend >= a.chunks || u0 >= u1) {
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    return;
+        if (left <= 0) {
+            while (pslab < a.chunks && left <= 0) {  // the next tile, or the next slab's first
+                ptile += a.wn;
+                if (ptile >= t1) {
+                    ptile = t0;
+                    pslab += a.slab;
+                    if (pslab >= a.chunks) break;
                 }
-                pu = u0;
-                pbase = pend;
-                pend = min(pend + a.slab, a.chunks);
+                const int sc = min(a.slab, a.chunks - pslab), c = pslab + sc * wk / wk_n;
+                left = pslab + sc * (wk + 1) / wk_n - c;
+                psrc = a.blocks + ((i64)ptile * a.chunks + c) * kBlock + lane * 16;
             }
-            pc = pbase + wk;
-            fresh = true;
         }
-        if (fresh) {
-            psrc = a.codes + ((i64)pu * MT * a.chunks + pc) * 1024 + lane * 16;
-            pscale = a.scales + (i64)pu * MT * a.groups_pad * 16 * es + lane * 16;
-            fresh = false;
-        }
-        const int g = WG < 4 ? pc * (4 / WG) : a.cpg == 1 ? pc : pc / a.cpg;
+        if (left > 0) {
+            if (left > 1) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (m && pu * MT + m >= a.tiles) break;  // (the sums of a tile that is not there are not stored)
-            const uint8_t *p = psrc + (i64)m * a.chunks * 1024;
-            cp16(dst + m * part, p);
-            cp16(dst + m * part + 512, p + 512);
-            if (lane * 16 < sb) cp16(dst + m * part + 1024, pscale + ((i64)m * a.groups_pad + g) * 16 * es);
+                for (int j = 0; j < (kSlot + 511) / 512; ++j)
+                    if (512 * (j + 1) <= kSlot || lane * 16 < kSlot - 512 * j) cp16(dst + 512 * j, psrc + 512 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < (kBlock + 511) / 512; ++j)
+                    if (512 * (j + 1) <= kBlock || lane * 16 < kBlock - 512 * j) cp16(dst + 512 * j, psrc + 512 * j);
+            }
+            psrc += kSlot;
+            left -= kPair;
+            if (kDepth == 2) {
+                dst = 2 * ring_s + kSlot - dst;
+            } else {
+                dst += kSlot;
+                if (dst == ring_s + kDepth * kSlot) dst = ring_s;
+            }
         }
-        psrc += wk_n * 1024;
-        pc += wk_n;
-        dst += slot;
-        if (dst == dst_end) dst -= kDepth * slot;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     for (int i = 0; i < kDepth - 1; ++i) issue();
@@ -322,7 +355,7 @@ __global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_co
     const int g = lane >> 2, t = lane & 3;
     // a column of mma depends on its own activations alone: lanes behind the
     // last column read it again
-    const uint8_t *xcol[NT];
+    int xcol[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         int col = n * 8 + g;
@@ -332,166 +365,143 @@ __global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_co
             constexpr int kPer = (NT + 2) / 3;
             col = (n / kPer) * rows + min((n % kPer) * 8 + g, rows - 1);
         }
-        xcol[n] = xs + col * pitch + t * 16;
+        xcol[n] = a.xs_at + col * pitch + t * 16;
     }
-    const uint8_t *blk = ring;
+    int blk = ring;
     int turn = 0;  // partial-sum buffers are used in turn
     for (int s0 = 0; s0 < a.chunks; s0 += a.slab) {
         const int sc = min(a.slab, a.chunks - s0), n8 = sc * 16;
         if (s0) __syncthreads();
-        // four loads in flight a thread
-        for (int e0 = threadIdx.x; e0 < rows * n8; e0 += 4 * W * 32) {
-            Eight v[4];
-            int r[4], k[4];
+        constexpr int kLoads = W == 32 ? 2 : 4;  // in flight a thread
+        for (int e0 = threadIdx.x; e0 < rows * n8; e0 += kLoads * W * 32) {
+            Eight v[kLoads];
+            int r[kLoads], k[kLoads];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < kLoads; ++u) {
                 const int e = e0 + u * W * 32;
                 r[u] = e / n8, k[u] = e - r[u] * n8;
                 if (r[u] < rows) v[u] = load8(a, row0 + r[u], s0 * 128 + k[u] * 8);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < kLoads; ++u)
                 if (r[u] < rows)
-                    store8(a, v[u], xs + (a.packed ? 3 * r[u] : r[u]) * pitch + k[u] * 16,
+                    store8(a, v[u], smem + a.xs_at + (a.packed ? 3 * r[u] : r[u]) * pitch + k[u] * 16,
                            a.packed ? pitch : rows * pitch);
         }
         __syncthreads();
-        for (int u = u0; u < u1; u += a.wn, turn ^= 1) {
-            float tot[MT][NT][4];
+        const int cb = sc * wk / wk_n, ce = sc * (wk + 1) / wk_n;
+        for (int u = t0; u < t1; u += a.wn, turn ^= 1) {
+            float tot[NT][4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) tot[m][n][0] = tot[m][n][1] = tot[m][n][2] = tot[m][n][3] = 0.0f;
-            for (int ck = wk; ck < sc; ck += wk_n) {
+            for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
+            for (int xo = cb * 256; xo < ce * 256; xo += kPair * 256) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
                 __syncwarp();
                 issue();
-                const int xo = ck * 256;
-                uint32_t wl[MT][4], wh[MT][4];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint4 lo = *reinterpret_cast<const uint4 *>(blk + m * part + lane * 16);
-                    const uint4 hi = *reinterpret_cast<const uint4 *>(blk + m * part + 512 + lane * 16);
-                    wl[m][0] = lo.x, wl[m][1] = lo.y, wl[m][2] = lo.z, wl[m][3] = lo.w;
-                    wh[m][0] = hi.x, wh[m][1] = hi.y, wh[m][2] = hi.z, wh[m][3] = hi.w;
-                }
-                float c[MT][NT][4];
+                for (int p = 0; p < kPair; ++p) {
+                    if (p && xo + 256 * p >= ce * 256) break;
+                    const uint8_t *bp = smem + blk + p * kBlock;
+                    const uint4 lo = *reinterpret_cast<const uint4 *>(bp + lane * 16);
+                    const uint4 hi = *reinterpret_cast<const uint4 *>(bp + 512 + lane * 16);
+                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+                    const S *sp = reinterpret_cast<const S *>(bp + 1024) + g;
+                    float c[NT][4];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t a0[MT][4], a1[MT][4];
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t a0[4], a1[4];
+                        code_pairs<F16>(wl[w], a0[0], a0[2], a1[0], a1[2]);
+                        code_pairs<F16>(wh[w], a0[1], a0[3], a1[1], a1[3]);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        a0[m][0] = code_pair<F16>(wl[m][w]), a0[m][1] = code_pair<F16>(wh[m][w]);
-                        a0[m][2] = code_pair<F16>(wl[m][w] >> 4), a0[m][3] = code_pair<F16>(wh[m][w] >> 4);
-                        a1[m][0] = code_pair<F16>(wl[m][w] >> 8), a1[m][1] = code_pair<F16>(wh[m][w] >> 8);
-                        a1[m][2] = code_pair<F16>(wl[m][w] >> 12), a1[m][3] = code_pair<F16>(wh[m][w] >> 12);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint4 b = *reinterpret_cast<const uint4 *>(xcol[n] + xo + w * 64);
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            mma<F16>(c[m][n], a0[m], b.x, b.y, w % WG == 0);
-                            mma<F16>(c[m][n], a1[m], b.z, b.w, false);
+                        for (int n = 0; n < NT; ++n) {
+                            const uint4 b = *reinterpret_cast<const uint4 *>(smem + xcol[n] + xo + p * 256 + w * 64);
+                            mma<F16>(c[n], a0, b.x, b.y, w % WG == 0);
+                            mma<F16>(c[n], a1, b.z, b.w, false);
                         }
-                    }
-                    if (w % WG == WG - 1) {
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            float s0f, s1f;
-                            const uint8_t *sp = blk + m * part + 1024 + (w / WG) * 16 * es;
-                            if (a.scale_f16) {
-                                s0f = __half2float(reinterpret_cast<const __half *>(sp)[g]);
-                                s1f = __half2float(reinterpret_cast<const __half *>(sp)[g + 8]);
-                            } else {
-                                s0f = reinterpret_cast<const float *>(sp)[g];
-                                s1f = reinterpret_cast<const float *>(sp)[g + 8];
-                            }
+                        if (w % WG == WG - 1) {
+                            const float s0f = scale_f32(sp[(w / WG) * 16]), s1f = scale_f32(sp[(w / WG) * 16 + 8]);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                tot[m][n][0] = fmaf(s0f, c[m][n][0], tot[m][n][0]);
-                                tot[m][n][1] = fmaf(s0f, c[m][n][1], tot[m][n][1]);
-                                tot[m][n][2] = fmaf(s1f, c[m][n][2], tot[m][n][2]);
-                                tot[m][n][3] = fmaf(s1f, c[m][n][3], tot[m][n][3]);
+                                tot[n][0] = fmaf(s0f, c[n][0], tot[n][0]);
+                                tot[n][1] = fmaf(s0f, c[n][1], tot[n][1]);
+                                tot[n][2] = fmaf(s1f, c[n][2], tot[n][2]);
+                                tot[n][3] = fmaf(s1f, c[n][3], tot[n][3]);
                             }
                         }
                     }
                 }
-                blk += slot;
-                if (blk == ring + kDepth * slot) blk = ring;
+                if (kDepth == 2) {
+                    blk = 2 * ring + kSlot - blk;
+                } else {
+                    blk += kSlot;
+                    if (blk == ring + kDepth * kSlot) blk = ring;
+                }
             }
-            // join the wk_n warps of the unit; two buffers in turn, so that a
-            // buffer is written again only after the next unit's barrier
-            constexpr int kFrag = MT * NT;  // float4 of a lane
+            // join the wk_n warps of the tile; two buffers in turn, so that a
+            // buffer is written again only after the next tile's barrier
             if (wk_n > 1) {
                 float4 *red = reinterpret_cast<float4 *>(smem + a.red_at) +
-                              ((i64)(turn * a.wn + wn) * (wk_n - 1)) * kFrag * 32 + lane;
+                              ((turn * a.wn + wn) * (wk_n - 1)) * NT * 32 + lane;
                 if (wk > 0) {
 #pragma unroll
-                    for (int f = 0; f < kFrag; ++f) {
-                        const float *v = tot[f / NT][f % NT];
-                        red[((wk - 1) * kFrag + f) * 32] = make_float4(v[0], v[1], v[2], v[3]);
-                    }
+                    for (int n = 0; n < NT; ++n)
+                        red[((wk - 1) * NT + n) * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
                 }
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + wn), "r"(wk_n * 32) : "memory");
                 if (wk > 0) continue;
                 for (int k = 0; k < wk_n - 1; ++k)
 #pragma unroll
-                    for (int f = 0; f < kFrag; ++f) {
-                        const float4 v = red[(k * kFrag + f) * 32];
-                        float *o = tot[f / NT][f % NT];
-                        o[0] += v.x, o[1] += v.y, o[2] += v.z, o[3] += v.w;
+                    for (int n = 0; n < NT; ++n) {
+                        const float4 v = red[(k * NT + n) * 32];
+                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
                     }
             }
             if (a.slab < a.chunks) {
-                float4 *sums = reinterpret_cast<float4 *>(smem + a.sums_at) + (i64)(u - (u0 - wn)) * kFrag * 32 + lane;
+                float4 *sums = reinterpret_cast<float4 *>(smem + a.sums_at) + (u - (t0 - wn)) * NT * 32 + lane;
 #pragma unroll
-                for (int f = 0; f < kFrag; ++f) {
-                    float *o = tot[f / NT][f % NT];
+                for (int n = 0; n < NT; ++n) {
                     if (s0) {
-                        const float4 v = sums[f * 32];
-                        o[0] += v.x, o[1] += v.y, o[2] += v.z, o[3] += v.w;
+                        const float4 v = sums[n * 32];
+                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
                     }
-                    if (s0 + sc < a.chunks) sums[f * 32] = make_float4(o[0], o[1], o[2], o[3]);
+                    if (s0 + sc < a.chunks) sums[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
                 }
                 if (s0 + sc < a.chunks) continue;
             }
-            // outputs u * MT * 16 + 16 m + g and + 8 of the rows in this lane's columns
+            // outputs 16 u + g and + 8 of the rows in this lane's columns
+            const int n0 = u * 16 + g;
+            constexpr float kUnit = F16 ? 1.0f : 4.0f;
             auto put = [&](int r, int n, float v) {
                 if (r >= rows || n >= a.out) return;
-                v += a.bias[n];
+                v = fmaf(v, kUnit, a.bias[n]);
                 const i64 at = (row0 + r) * a.ldy + n;
                 if (a.dtype == TRBA_F32) static_cast<float *>(a.y)[at] = v;
                 else if (a.dtype == TRBA_BF16) static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(v);
                 else static_cast<__half *>(a.y)[at] = __float2half_rn(v);
             };
+            if (split == 1) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int n0 = (u * MT + m) * 16 + g;
-                if (split == 1) {
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int q = 0; q < 4; ++q) put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8, tot[n][q]);
+            } else if (NT == 1) {  // packed: columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8, tot[m][n][q]);
-                } else if (NT == 1) {  // packed: columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int r = 0; r < 2; ++r) {
+                        float v[3];
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float v[3];
+                        for (int p = 0; p < 3; ++p)
+                            v[p] = __shfl_sync(kFull, tot[0][2 * h + ((3 * r + p) & 1)], 4 * g + (3 * r + p) / 2);
+                        if (t == r) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
+                    }
+            } else if (NT % 3 == 0) {
 #pragma unroll
-                            for (int p = 0; p < 3; ++p)
-                                v[p] = __shfl_sync(kFull, tot[m][0][2 * h + ((3 * r + p) & 1)], 4 * g + (3 * r + p) / 2);
-                            if (t == r) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
-                        }
-                } else if (NT % 3 == 0) {
+                for (int n = 0; n < NT / 3; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT / 3; ++n)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8,
-                                tot[m][n][q] + (tot[m][n + NT / 3][q] + tot[m][n + 2 * (NT / 3)][q]));
-                }
+                    for (int q = 0; q < 4; ++q)
+                        put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8,
+                            tot[n][q] + (tot[n + NT / 3][q] + tot[n + 2 * (NT / 3)][q]));
             }
         }
     }
@@ -507,9 +517,9 @@ int launched() {
 constexpr int kMaxSmem = 227 * 1024;
 constexpr int kMaxJoin = 48 * 1024;  // shared memory of the warps' partial sums
 
-template <bool F16, int WG, int NT, int MT, int W>
+template <bool F16, class S, int WG, int NT>
 int launch(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
-    auto fn = int4_forward_kernel<F16, WG, NT, MT, W>;
+    auto fn = int4_forward_kernel<F16, S, WG, NT, warps_of(NT)>;
     static std::atomic<unsigned long long> sized{0};  // one bit a device: its limit has been raised
     int dev = 0;
     cudaGetDevice(&dev);
@@ -523,31 +533,42 @@ int launch(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
         }
         sized.fetch_or(bit, std::memory_order_relaxed);
     }
-    fn<<<grid, W * 32, smem, st>>>(a);
+    fn<<<grid, warps_of(NT) * 32, smem, st>>>(a);
     return launched();
 }
 
-template <bool F16, int WG>
+template <bool F16, class S, int WG>
 int launch_nt(const Args &a, int nt, dim3 grid, size_t smem, cudaStream_t st) {
     switch (nt) {
-        case 1: return launch<F16, WG, 1, 1, 16>(a, grid, smem, st);
-        case 2: return launch<F16, WG, 2, 1, 16>(a, grid, smem, st);
-        case 3: return launch<F16, WG, 3, 2, 8>(a, grid, smem, st);
-        case 4: return launch<F16, WG, 4, 2, 8>(a, grid, smem, st);
-        case 5: return launch<F16, WG, 5, 2, 8>(a, grid, smem, st);
-        case 6: return launch<F16, WG, 6, 2, 8>(a, grid, smem, st);
-        default: return launch<F16, WG, 8, 2, 8>(a, grid, smem, st);
+        case 1: return launch<F16, S, WG, 1>(a, grid, smem, st);
+        case 2: return launch<F16, S, WG, 2>(a, grid, smem, st);
+        case 3: return launch<F16, S, WG, 3>(a, grid, smem, st);
+        case 4: return launch<F16, S, WG, 4>(a, grid, smem, st);
+        case 5: return launch<F16, S, WG, 5>(a, grid, smem, st);
+        case 6: return launch<F16, S, WG, 6>(a, grid, smem, st);
+        default: return launch<F16, S, WG, 8>(a, grid, smem, st);
     }
+}
+
+template <bool F16>
+int launch_type(const Args &a, bool scale_f16, int wg, int nt, dim3 grid, size_t smem, cudaStream_t st) {
+    if (scale_f16) {
+        if (wg == 1) return launch_nt<F16, __half, 1>(a, nt, grid, smem, st);
+        if (wg == 2) return launch_nt<F16, __half, 2>(a, nt, grid, smem, st);
+        return launch_nt<F16, __half, 4>(a, nt, grid, smem, st);
+    }
+    if (wg == 1) return launch_nt<F16, float, 1>(a, nt, grid, smem, st);
+    if (wg == 2) return launch_nt<F16, float, 2>(a, nt, grid, smem, st);
+    return launch_nt<F16, float, 4>(a, nt, grid, smem, st);
 }
 
 int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int rows, void *y, i64 ldy, cudaStream_t st) {
     Args a{};
-    a.codes = l->codes, a.scales = l->scales, a.bias = l->bias;
+    a.blocks = l->base, a.bias = l->bias;
     a.x = x, a.y = y, a.ldx = ldx, a.ldy = ldy;
     a.in = l->in, a.out = l->out, a.rows = rows, a.dtype = dtype;
     a.tiles = l->tiles, a.chunks = l->chunks, a.gpc = l->gpc;
-    a.cpg = l->group >= 128 ? l->group / 128 : 1;
-    a.groups_pad = l->groups_pad, a.scale_f16 = l->scale_dtype == TRBA_F16;
+    const bool scale_f16 = l->scale_dtype == TRBA_F16;
     // rows of a CTA: up to 64 columns, an f32 row being three (16 rows make six tiles of them)
     const bool f32 = dtype == TRBA_F32;
     const int most = f32 ? 16 : 64, blocks_y = (rows + most - 1) / most;
@@ -555,21 +576,20 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
     a.packed = f32 && a.block_rows <= 2;
     int nt = f32 ? (a.packed ? 1 : a.block_rows <= 8 ? 3 : 6) : (a.block_rows + 7) / 8;
     if (nt == 7) nt = 8;
-    const int mt = nt <= 2 ? 1 : 2, warps = nt <= 2 ? 16 : 8;
     const int cols = a.block_rows * (f32 ? 3 : 1);
     i64 smem = 0;
-    const int units = (a.tiles + mt - 1) / mt;
-    const int frag = mt * nt * 512;  // bytes of one unit's sums
-    const int ring = warps * kDepth * mt * (1024 + 16 * a.gpc * (a.scale_f16 ? 2 : 4));
+    const int frag = nt * 512;  // bytes of one tile's sums
+    const int warps = warps_of(nt), ring = warps * depth_of(warps) * kPair * l->block;
     const auto x_bytes = [&](int chunks) { return ((i64)cols * (chunks * 256 + 64) + 127) & ~127ll; };
-    int ctas = units < sm_count() ? units : sm_count();
-    for (;; ctas = ctas * 2 < units ? ctas * 2 : units) {
-        const int share = (units + ctas - 1) / ctas;  // units of a CTA, at most
-        // Units of a CTA that run side by side: the fewest steps of (chunks a
-        // warp streams + the join of the warps that share a unit).
+    int ctas = a.tiles < sm_count() ? a.tiles : sm_count();
+    for (;; ctas = ctas * 2 < a.tiles ? ctas * 2 : a.tiles) {
+        const int share = (a.tiles + ctas - 1) / ctas;  // tiles of a CTA, at most
+        // Tiles of a CTA that run side by side: the fewest steps of (chunks a
+        // warp streams + the join of the warps that share a tile).
         long long best = -1;
         int red = 0;
         for (int wn = warps; wn >= 1; wn >>= 1) {
+            if (wn == 16 && warps > 16) continue;  // named barriers 1 + wn go up to 15
             const int wk = warps / wn, bytes = 2 * wn * (wk - 1) * frag;
             const long long steps = (share + wn - 1) / wn;
             const long long cost = steps * (4 * ((a.chunks + wk - 1) / wk) + (wk > 1 ? 4 + wk : 0));
@@ -585,7 +605,7 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
         if (x_bytes(a.chunks) > room) {
             sums = (i64)share * frag;
             a.slab = (int)(((room - sums - 128) / cols - 64) / 256);
-            if (a.slab < 4 && ctas < units) continue;
+            if (a.slab < 4 && ctas < a.tiles) continue;
         }
         if (const char *e = getenv("TUNE_SLAB")) a.slab = atoi(e), sums = (i64)share * frag;
         a.xs_at = ring;
@@ -596,23 +616,15 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
     }
     const int wg = l->group >= 128 ? 4 : l->group / 32;
     const dim3 grid(ctas, blocks_y);
-    if (dtype == TRBA_F16) {
-        if (wg == 1) return launch_nt<true, 1>(a, nt, grid, smem, st);
-        if (wg == 2) return launch_nt<true, 2>(a, nt, grid, smem, st);
-        return launch_nt<true, 4>(a, nt, grid, smem, st);
-    }
-    if (wg == 1) return launch_nt<false, 1>(a, nt, grid, smem, st);
-    if (wg == 2) return launch_nt<false, 2>(a, nt, grid, smem, st);
-    return launch_nt<false, 4>(a, nt, grid, smem, st);
+    return dtype == TRBA_F16 ? launch_type<true>(a, scale_f16, wg, nt, grid, smem, st)
+                             : launch_type<false>(a, scale_f16, wg, nt, grid, smem, st);
 }
 
 template <class S>
 int layout(trba_linear_int4 *l, const uint8_t *codes, i64 pitch, const void *scales, i64 ld_scales, cudaStream_t st) {
-    const i64 n = (i64)l->tiles * l->chunks * 256 + (i64)l->tiles * l->groups_pad * 16;
-    int4_layout_kernel<S><<<grid_for(n), 256, 0, st>>>(codes, pitch, static_cast<const S *>(scales), ld_scales, l->in,
-                                                       l->out, l->groups, l->groups_pad, l->tiles, l->chunks,
-                                                       reinterpret_cast<uint32_t *>(l->codes),
-                                                       reinterpret_cast<S *>(l->scales));
+    int4_layout_kernel<S><<<grid_for((i64)l->tiles * l->chunks * 32), 256, 0, st>>>(
+        codes, pitch, static_cast<const S *>(scales), ld_scales, l->in, l->out, l->group, l->groups, l->gpc, l->tiles,
+        l->chunks, l->block, l->base);
     return launched();
 }
 
@@ -628,19 +640,16 @@ trba_linear_int4 *allocate(int in, int out, int group, int scale_dtype) {
     l->tiles = (out - 1) / 16 + 1;
     l->chunks = (in - 1) / 128 + 1;
     l->gpc = group >= 128 ? 1 : 128 / group;
-    l->groups_pad = group >= 128 ? l->groups : l->chunks * l->gpc;
-    const size_t nc = (size_t)l->tiles * l->chunks * 1024;
-    const size_t ns = (size_t)l->tiles * l->groups_pad * 16 * (scale_dtype == TRBA_F32 ? 4 : 2);
+    l->block = 1024 + 16 * l->gpc * (scale_dtype == TRBA_F32 ? 4 : 2);
+    const size_t nc = (size_t)l->tiles * l->chunks * l->block;
     if (cudaGetDevice(&l->device) != cudaSuccess ||
-        cudaMalloc(&l->base, nc + ns + (size_t)out * 4) != cudaSuccess) {
+        cudaMalloc(&l->base, nc + (size_t)out * 4) != cudaSuccess) {
         cudaGetLastError();
         report_error(__FILE__, __LINE__, "LinearInt4: device allocation failed", -1);
         delete l;
         return nullptr;
     }
-    l->codes = l->base;
-    l->scales = l->base + nc;
-    l->bias = reinterpret_cast<float *>(l->base + nc + ns);
+    l->bias = reinterpret_cast<float *>(l->base + nc);
     return l;
 }
 
@@ -734,8 +743,7 @@ int trba_linear_int4_get(const trba_linear_int4 *l, uint8_t *codes, float *scale
         uint8_t *nat = nullptr;
         e = cudaMalloc(&nat, n);
         if (e == cudaSuccess) {
-            int4_natural_kernel<<<grid_for((i64)n), 256>>>(reinterpret_cast<const uint32_t *>(l->codes), l->in, l->out,
-                                                           l->chunks, nat);
+            int4_natural_kernel<<<grid_for((i64)n), 256>>>(l->base, l->in, l->out, l->chunks, l->block, nat);
             e = (cudaError_t)launched();
             if (e == cudaSuccess) e = cudaMemcpy(codes, nat, n, cudaMemcpyDeviceToHost);
             cudaFree(nat);
@@ -744,15 +752,17 @@ int trba_linear_int4_get(const trba_linear_int4 *l, uint8_t *codes, float *scale
     if (bias && e == cudaSuccess) e = cudaMemcpy(bias, l->bias, (size_t)l->out * 4, cudaMemcpyDeviceToHost);
     if (scales && e == cudaSuccess) {
         const bool f16 = l->scale_dtype == TRBA_F16;
-        const size_t ns = (size_t)l->tiles * l->groups_pad * 16;
-        uint8_t *tmp = new (std::nothrow) uint8_t[ns * (f16 ? 2 : 4)];
+        const size_t sb = l->block - 1024, nb = (size_t)l->tiles * l->chunks;  // the blocks' scales alone
+        uint8_t *tmp = new (std::nothrow) uint8_t[nb * sb];
         TRBA_REQUIRE_RET(tmp, "trba_linear_int4_get: out of host memory", -1);
-        e = cudaMemcpy(tmp, l->scales, ns * (f16 ? 2 : 4), cudaMemcpyDeviceToHost);
+        e = cudaMemcpy2D(tmp, sb, l->base + 1024, l->block, sb, nb, cudaMemcpyDeviceToHost);
         for (int n = 0; n < l->out; ++n)
             for (int g = 0; g < l->groups; ++g) {
-                const size_t at = ((size_t)(n >> 4) * l->groups_pad + g) * 16 + (n & 15);
-                scales[(size_t)n * l->groups + g] = f16 ? __half2float(reinterpret_cast<const __half *>(tmp)[at])
-                                                        : reinterpret_cast<const float *>(tmp)[at];
+                const size_t chunk = (size_t)g * l->group / 128, part = l->group < 128 ? g % l->gpc : 0;
+                const uint8_t *p = tmp + ((size_t)(n >> 4) * l->chunks + chunk) * sb;
+                const size_t at = part * 16 + (n & 15);
+                scales[(size_t)n * l->groups + g] = f16 ? __half2float(reinterpret_cast<const __half *>(p)[at])
+                                                        : reinterpret_cast<const float *>(p)[at];
             }
         delete[] tmp;
     }
