@@ -10,9 +10,9 @@
  * recogniser's own decoder.
  *
  * All pointers are device pointers of the current device.  The functions
- * only launch kernels on `stream`: no allocation, no synchronisation, no
- * workspace, so they may be captured into CUDA graphs and run on several
- * streams at once.  They return 0, -1 for a bad argument or a CUDA error
+ * only launch kernels on `stream`, without allocation or synchronisation, so
+ * they may be captured into CUDA graphs and, each with a workspace of its
+ * own, run on several streams at once.  They return 0, -1 for a bad argument or a CUDA error
  * code; errors also follow the library policy (trba_last_error / abort on
  * error).  Zero lines is an empty call and returns 0. */
 #ifndef TRBA_DECODE_H
@@ -57,11 +57,16 @@ extern "C" {
  * formed and compared in f64 and rounded to f32 at the end (the exponentials
  * are f32, their sums f64).
  *
- * beams 1 .. 32, beams * vocab < 2^31, eos in [0, vocab) or -1 for "no end
- * token" (then finished must be NULL). */
+ * beams 1 .. 32, vocab 1 .. 2^30, beams * vocab < 2^31, lines * beams <
+ * 2^24, eos in [0, vocab) or -1 for "no end token" (then finished must be
+ * NULL).  Long rows need a workspace of trba_beam_select_workspace(...) bytes,
+ * aligned to 16 (0 bytes: none, NULL will do), which calls that may overlap
+ * must not share; what it holds before and after does not matter. */
+long long trba_beam_select_workspace(int dtype, int lines, int beams, int vocab);
 int trba_beam_select(const void *logits, int dtype, long long ld, const float *scores, const uint8_t *finished,
                      int lines, int beams, int vocab, int eos, float *out_scores, int32_t *out_tokens,
-                     int32_t *out_parents, uint8_t *out_finished, void *stream);
+                     int32_t *out_parents, uint8_t *out_finished, void *workspace, long long workspace_bytes,
+                     void *stream);
 
 /* A state tensor whose rows follow the beams, as a strided view
  * [outer][lines * beams][mid][bytes]; strides and sizes in bytes.  A plain

@@ -45,7 +45,7 @@ def _refused(lib, rc, word):
 def test_c_refusals(lib):
     lib.trba_clear_error()
     sel = lambda dtype=0, ld=10, lines=1, beams=2, vocab=10, eos=1, fin=None, p=None: lib.trba_beam_select(  # noqa: E731
-        p, dtype, ld, p, fin, lines, beams, vocab, eos, p, p, p, p, None)
+        p, dtype, ld, p, fin, lines, beams, vocab, eos, p, p, p, p, None, 0, None)
     for kw in (dict(beams=0), dict(beams=33), dict(lines=-1), dict(vocab=0), dict(ld=9), dict(beams=32, vocab=1 << 27, ld=1 << 27)):
         _refused(lib, sel(**kw), b"bad sizes")
     _refused(lib, sel(eos=10), b"eos outside")
@@ -55,6 +55,9 @@ def test_c_refusals(lib):
     _refused(lib, sel(), b"null pointer")
     _refused(lib, sel(p=C.c_void_p(66)), b"not aligned")
     assert sel(lines=0) == 0
+    _refused(lib, sel(vocab=1 << 16, ld=1 << 16, p=C.c_void_p(64)), b"workspace")
+    assert lib.trba_beam_select_workspace(0, 1, 2, 10) == 0 < lib.trba_beam_select_workspace(0, 1, 2, 1 << 16)
+    assert lib.trba_beam_select_workspace(0, 0, 2, 1 << 16) == 0 == lib.trba_beam_select_workspace(3, 1, 2, 1 << 16)
     one = (C.c_int64 * 11)(64, 64, -1, 8, 8, 1, 0, 0, 1, 0, 0)
     par = C.c_void_p(64)
     _refused(lib, lib.trba_beam_reorder(one, 1, par, 1, 2, None), b"negative")

@@ -6,6 +6,9 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "common.cuh"
 #include "trba_decode.h"
 
@@ -31,26 +34,11 @@ __device__ __forceinline__ float to_f32(__half v) {
     return __half2float(v);
 }
 
-// The best entries of a warp, one a lane, best first: larger value, then lower
-// index.  Lanes that hold no entry have (-inf, kNone).
-struct WarpList {
-    float v = -INFINITY;
-    int i = kNone;
-    // Inserts (x, at), the same in every lane, if it is among the best `k`.
-    __device__ __forceinline__ void insert(float x, int at, int lane) {
-        const int pos = __popc(__ballot_sync(kFull, v > x || (v == x && i < at)));
-        const float pv = __shfl_up_sync(kFull, v, 1);
-        const int pi = __shfl_up_sync(kFull, i, 1);
-        if (lane == pos) {
-            v = x;
-            i = at;
-        } else if (lane > pos) {
-            v = pv;
-            i = pi;
-        }
-    }
-};
-
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
@@ -61,98 +49,549 @@ __device__ __forceinline__ double warp_sum(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
 }
+// The value of rank `k` (0: largest) of the warp's 32, by a bitonic sort.
+__device__ __forceinline__ float warp_kth(float v, int k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float w = __shfl_xor_sync(kFull, v, o);
+            v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, w) : fminf(v, w);
+        }
+    return __shfl_sync(kFull, v, k);
+}
+// Unsigned integers in the order of the floats (no NaN).
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned u = __float_as_uint(v);
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(unsigned k) {
+    return __uint_as_float(k ^ ((unsigned)((int)~k >> 31) | 0x80000000u));
+}
 
-constexpr int kSelThreads = 256;
+// A candidate as one number: the larger value first, then the lower index.
+// Values of -inf are no candidates: 0.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key make_key(float x, int at) {
+    return x > -INFINITY ? (Key)ordered(x + 0.0f) << 32 | (unsigned)~at : 0;  // (-0 equals 0)
+}
+__device__ __forceinline__ float key_value(Key k) { return k ? unordered((unsigned)(k >> 32)) : -INFINITY; }
+__device__ __forceinline__ int key_index(Key k) { return (int)~(unsigned)k; }
 
-// One CTA a line, a warp a beam at a time: the row's best `beams` tokens (the
-// order within a row is that of the logits) and its log sum of exponentials;
-// then one warp merges the beams' lists, its lane b at the head of beam b's.
+__device__ __forceinline__ Key exchange(Key v, int o, bool keep_max) {
+    const Key w = __shfl_xor_sync(kFull, v, o);
+    return (v > w) == keep_max ? v : w;
+}
+// The warp's 32 keys in descending order, by a bitonic sort; only the first
+// `count` lanes have keys.
+__device__ __noinline__ Key sort_keys(Key v, int count, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) v = exchange(v, o, ((lane & o) == 0) == ((lane & size) == 0));
+        if (count <= size) break;
+    }
+    return v;
+}
+// The largest 32 of two descending lists, descending.
+__device__ __noinline__ Key merge_keys(Key a, Key b, int lane) {
+    const Key r = __shfl_sync(kFull, b, 31 - lane);
+    Key v = a > r ? a : r;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = exchange(v, o, (lane & o) == 0);
+    return v;
+}
+
+// The scan of a row goes in batches of kSelUnroll groups of 16 bytes a lane,
+// through a ring of cp.async stages in shared memory.  Rows may start at any
+// element: a stage holds the aligned blocks its batch lies in, and a group
+// that straddles two is put together from both.  Groups go by their index in
+// the row, not by their address, so that equal rows have equal sums wherever
+// they start.
+constexpr int kSelUnroll = 4, kStages = 3;
+constexpr int kStageBytes = kSelUnroll * 512 + 16;
+constexpr int kSpans = 16;    // spans of batches whose largest elements are remembered
+constexpr int kBuffer = 64;   // candidates kept before they are sorted in
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Shared memory of a warp's scan.  The candidates and the list of places to
+// look at again use the ring when it is done with, or the spans that a segment
+// still in the ring leaves free.
+struct __align__(16) Scan {
+    uint8_t ring[kStages][kStageBytes];
+    float most[kSpans][32];  // the largest element of each lane in each span
+    __device__ __forceinline__ Key *cand(bool kept) {  // [kBuffer]
+        return kept ? reinterpret_cast<Key *>(most[kStages]) : reinterpret_cast<Key *>(ring);
+    }
+    __device__ __forceinline__ unsigned short *hit(bool kept) {  // span * 32 + lane, [kSpans * 32]
+        return reinterpret_cast<unsigned short *>(cand(kept) + kBuffer);
+    }
+};
+static_assert(kStages * kStageBytes >= kBuffer * 8 + kSpans * 64, "the ring holds candidates and places");
+static_assert((kSpans - kStages) * 128 >= kBuffer * 8 + kStages * 64, "so do the spans a short segment leaves free");
+
+// What a warp found in its segment of a row: the largest logit, the sum of
+// exp(logit - largest) and its best tokens.
+struct Found {
+    double sum;
+    Key best[TRBA_MAX_BEAMS];
+    float top;
+};
+
+
 template <class T>
-__global__ void __launch_bounds__(kSelThreads) beam_select_kernel(
-    const T *__restrict__ logits, i64 ld, const float *scores, const uint8_t *finished, int beams, int vocab, int eos,
-    float *out_scores, int32_t *__restrict__ out_tokens, int32_t *__restrict__ out_parents, uint8_t *out_finished) {
-    __shared__ double s_score[TRBA_MAX_BEAMS][TRBA_MAX_BEAMS];
-    __shared__ int s_tok[TRBA_MAX_BEAMS][TRBA_MAX_BEAMS];
-    __shared__ uint8_t s_fin[TRBA_MAX_BEAMS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const i64 slot0 = (i64)blockIdx.x * beams;
-    for (int b = warp; b < beams; b += kSelThreads / 32) {
-        const float sc = scores[slot0 + b];
-        const bool fin = finished && finished[slot0 + b];
-        const bool dead = !(sc > -INFINITY);
+__device__ __forceinline__ float element(uint32_t w, int half) {
+    float v;
+    if (sizeof(T) == 4) v = __uint_as_float(w);
+    else if (std::is_same<T, __nv_bfloat16>::value) v = __uint_as_float(half ? w & 0xffff0000u : w << 16);
+    else v = __half2float(__ushort_as_half((unsigned short)(w >> (16 * half))));
+    return v;
+}
+
+// Copies the blocks of the elements [base, base + batch) that lie before `end`.
+template <class T>
+__device__ __forceinline__ void fetch_batch(const T *row, int base, int end, int skew, uint8_t *stage, int lane) {
+    const char *src = reinterpret_cast<const char *>(row + base) - skew + lane * 16;
+    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(stage)) + lane * 16;
+    if (base + (kSelUnroll * 32 + 1) * 16 / (int)sizeof(T) <= end) {
+#pragma unroll
+        for (int u = 0; u < kSelUnroll; ++u)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + u * 512), "l"(src + u * 512) : "memory");
+        if (skew && lane == 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + kSelUnroll * 512), "l"(src + kSelUnroll * 512)
+                         : "memory");
+        return;
+    }
+    // the row's end: the last block only as far as the row goes
+#pragma unroll 1
+    for (int u = 0; u <= kSelUnroll; ++u) {
+        if (u == kSelUnroll && (lane > 0 || skew == 0)) break;
+        const int room = (end - base) * (int)sizeof(T) + skew - lane * 16 - u * 512, bytes = min(room, 16);
+        if (bytes > 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + u * 512), "l"(src + u * 512), "r"(bytes)
+                         : "memory");
+    }
+}
+
+// The elements of +inf of a lane in a batch (they share the row): rare.
+template <class T>
+__device__ __noinline__ int count_inf(const T *row, int base, int end, int lane) {
+    constexpr int N = 16 / sizeof(T);
+    int n = 0;
+#pragma unroll 1
+    for (int k = 0; k < kSelUnroll * N; ++k) {
+        const int at = base + (k / N * 32 + lane) * N + k % N;
+        if (at < end && to_f32(row[at]) == INFINITY) ++n;
+    }
+    return n;
+}
+
+// Sorts the first 32 candidates of the buffer into the list of the best.
+__device__ __forceinline__ Key take_32(Key *cand, Key best, int &count, int lane) {
+    __syncwarp();
+    Key mine = lane < count ? cand[lane] : 0;
+    const Key rest = lane + 32 < count ? cand[lane + 32] : 0;
+    __syncwarp();
+    if (lane + 32 < count) cand[lane] = rest;
+    mine = sort_keys(mine, count, lane);
+    count = max(0, count - 32);
+    return __any_sync(kFull, best != 0) ? merge_keys(best, mine, lane) : mine;
+}
+// Appends the lanes' wanted keys to the buffer.
+__device__ __forceinline__ void append(Key *cand, Key key, bool want, int &count, int lane) {
+    const unsigned some = __ballot_sync(kFull, want);
+    if (want) cand[count + __popc(some & ((1u << lane) - 1))] = key;
+    count += __popc(some);
+}
+
+// Lists the places whose largest element is at least `bar`; returns how many.
+__device__ __forceinline__ int list_hits(const Scan &scan, unsigned short *list, int spans, float bar, int lane) {
+    const float least = fmaxf(bar, -3.402823466e38f);  // -inf is never one of the best
+    int hits = 0;
+    __syncwarp();
+#pragma unroll 4
+    for (int q = 0; q < spans; ++q) {
+        const bool hit = scan.most[q][lane] >= least;  // (a lane reads what it wrote itself)
+        const unsigned some = __ballot_sync(kFull, hit);
+        if (hit) list[hits + __popc(some & ((1u << lane) - 1))] = (unsigned short)(q * 32 + lane);
+        hits += __popc(some);
+    }
+    __syncwarp();
+    return hits;
+}
+
+// The elements [c0, c1) of a row (c0 a multiple of 32 groups): the sum of
+// exp(x - m) under a lane's running largest m, f32 within a batch, f64 beyond,
+// and the best `beams`.  The scan itself only remembers each lane's largest
+// element of each span of batches.  The beams-th largest of those is a bar
+// that at least `beams` elements reach, so only the places whose largest
+// reaches it, about as many as there are beams, are looked at again (in the
+// ring if the segment still is, else in the cache).
+template <class T>
+__device__ __forceinline__ void scan_segment(const T *row, int c0, int c1, int beams, int lane, Scan &scan,
+                                             Found &out) {
+    constexpr int N = 16 / sizeof(T), kBatch = kSelUnroll * 32 * N;
+    const int skew = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+    const int batches = (c1 - c0 + kBatch - 1) / kBatch, per = (batches + kSpans - 1) / kSpans;
+#pragma unroll
+    for (int t = 0; t < kStages - 1; ++t) {
+        if (t < batches) fetch_batch<T>(row, c0 + t * kBatch, c1, skew, scan.ring[t], lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    float m = -INFINITY, most = -INFINITY;
+    double sum = 0.0;
+    int spans = 0, in_span = 0;
+#pragma unroll 1
+    for (int t = 0; t < batches; ++t) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        if (t + kStages - 1 < batches)
+            fetch_batch<T>(row, c0 + (t + kStages - 1) * kBatch, c1, skew, scan.ring[(t + kStages - 1) % kStages], lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const int base = c0 + t * kBatch;
+        float x[kSelUnroll][N];
+#pragma unroll
+        for (int u = 0; u < kSelUnroll; ++u) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(scan.ring[t % kStages]) + u * 32 + lane;
+            const uint4 lo = q[0];
+            uint32_t w[4] = {lo.x, lo.y, lo.z, lo.w};
+            if (skew) {
+                const uint4 hi = q[1];
+                const uint32_t all[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                const int by = skew >> 2, sh = (skew & 2) * 8;
+                uint32_t s[5];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) {
+                    const uint32_t a = by & 1 ? all[i + 1] : all[i], b = by & 1 ? all[min(i + 3, 7)] : all[i + 2];
+                    s[i] = by & 2 ? b : a;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(s[i], s[i + 1], sh);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[u][e] = element<T>(w[e * (int)sizeof(T) / 4], e & 1);
+        }
+        if (base + kBatch > c1) {  // the row's last batch
+#pragma unroll
+            for (int u = 0; u < kSelUnroll; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (base + (u * 32 + lane) * N + e >= c1) x[u][e] = -INFINITY;
+        }
+        float all = -INFINITY;  // (of a number and a NaN the number is the larger)
+#pragma unroll
+        for (int u = 0; u < kSelUnroll; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) all = fmaxf(all, x[u][e]);
+        if (all > m) {
+            sum *= (double)exp2_approx((m - all) * kLog2e);  // 0 while m is -inf (and so is the sum)
+            m = all;
+        }
+        most = fmaxf(most, all);
+        if (++in_span == per || t + 1 == batches) {
+            scan.most[spans++][lane] = most;
+            most = -INFINITY;
+            in_span = 0;
+        }
+        if (m == INFINITY) {
+            sum += (double)count_inf<T>(row, base, c1, lane);
+        } else if (m > -INFINITY) {
+            float part[kSelUnroll];
+            bool again = true;
+            while (again) {
+#pragma unroll
+                for (int u = 0; u < kSelUnroll; ++u) {
+                    float y[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) y[e] = exp2_approx((x[u][e] - m) * kLog2e);
+#pragma unroll
+                    for (int o = N / 2; o > 0; o >>= 1)
+#pragma unroll
+                        for (int e = 0; e < o; ++e) y[e] += y[e + o];
+                    part[u] = y[0];
+                }
+                part[0] = (part[0] + part[1]) + (part[2] + part[3]);
+                again = part[0] != part[0];
+                if (again) {  // NaN counts as -inf
+#pragma unroll
+                    for (int u = 0; u < kSelUnroll; ++u)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) x[u][e] = fmaxf(x[u][e], -INFINITY);
+                }
+            }
+            sum += (double)part[0];
+        }
+    }
+
+    // the bar: first from the lanes' maxima; where that leaves many places, from theirs
+    const bool kept = batches <= kStages;
+    Key *cand = scan.cand(kept);
+    unsigned short *hit = scan.hit(kept);
+    float bar = warp_kth(m, beams - 1, lane);
+    int hits = list_hits(scan, hit, spans, bar, lane), count = 0;
+    Key best = 0;
+    if (hits > 32) {
+#pragma unroll 1
+        for (int h0 = 0; h0 < hits; h0 += 32) {
+            Key c = 0;
+            if (h0 + lane < hits) {
+                const int h = hit[h0 + lane];
+                c = make_key(scan.most[h >> 5][h & 31], h0 + lane);
+            }
+            if (__any_sync(kFull, c > __shfl_sync(kFull, best, beams - 1)))
+                best = merge_keys(best, sort_keys(c, 32, lane), lane);
+        }
+        bar = key_value(__shfl_sync(kFull, best, beams - 1));
+        hits = list_hits(scan, hit, spans, bar, lane);
+        best = 0;
+    }
+    Key last = bar > -INFINITY ? (Key)ordered(bar + 0.0f) << 32 : 0;  // candidates are larger
+    const int total = hits * per * kSelUnroll;  // groups of N to look at, two in flight a lane
+    const float inv_per = 1.0f / (float)per;
+#pragma unroll 1
+    for (int j0 = 0; j0 < total; j0 += 64) {
+        float x[2][N];
+        int at[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int j = j0 + u * 32 + lane, pb = j / kSelUnroll;
+            at[u] = c1;
+            if (j < total) {
+                const int q = (int)(((float)pb + 0.5f) * inv_per);  // pb / per
+                const int h = hit[q], batch = (h >> 5) * per + pb - q * per;
+                const int in = (j % kSelUnroll * 32 + (h & 31)) * N, c = c0 + batch * kBatch + in;
+                at[u] = c;
+                const T *src = kept ? reinterpret_cast<const T *>(scan.ring[batch % kStages] + skew) + in : row + c;
+                if (skew == 0 && c + N <= c1) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(src);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[u][e] = element<T>(ws[e * (int)sizeof(T) / 4], e & 1);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[u][e] = c + e < c1 ? to_f32(src[e]) : -INFINITY;
+                }
+            }
+        }
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float v = u ? x[1][e] : x[0][e];
+                const int i = (u ? at[1] : at[0]) + e;
+                const bool in = i < c1 && v >= bar;  // (NaN is not)
+                if (!__any_sync(kFull, in)) continue;
+                const Key c = in ? make_key(v, i) : 0;
+                append(cand, c, c > last, count, lane);
+                if (count >= 32) {
+                    best = take_32(cand, best, count, lane);
+                    const Key kth = __shfl_sync(kFull, best, beams - 1);
+                    last = kth > last ? kth : last;
+                }
+            }
+        }
+    }
+    if (count > 0) best = take_32(cand, best, count, lane);
+    __syncwarp();  // the next scan of this warp writes here again
+    const float top = warp_max(m);
+    // an infinite top: lanes that saw it have counted it, the others add nothing
+    if (m != top) sum = m > -INFINITY ? sum * (double)exp2_approx((m - top) * kLog2e) : 0.0;
+    sum = warp_sum(sum);
+    if (lane < beams) out.best[lane] = best;
+    if (lane == 0) {
+        out.top = top;
+        out.sum = sum;
+    }
+}
+
+// What a line's merge works on in shared memory.
+struct Merge {
+    double score[TRBA_MAX_BEAMS][TRBA_MAX_BEAMS];
+    int tok[TRBA_MAX_BEAMS][TRBA_MAX_BEAMS];
+    Key cand[16][kBuffer];  // a warp's each
+};
+
+// Joins what was found in the rows' segments and picks the line's best: a warp
+// a beam joins the segments of its row, then the first warp merges the beams'
+// lists, its lane b at the head of beam b's.  find(b, s): segment s of beam b.
+template <class F>
+__device__ __forceinline__ void merge_line(F find, int segs, float my_score, unsigned alive, unsigned over, int beams,
+                                           int eos, i64 slot0, Merge &mg, float *out_scores, int32_t *out_tokens,
+                                           int32_t *out_parents, uint8_t *out_finished) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll 1
+    for (int b = warp; b < beams; b += warps) {
+        const float sc = __shfl_sync(kFull, my_score, b);
         double out = -INFINITY;
         int tok = kNone;
-        if (fin && !dead) {
+        if ((alive >> b & 1) && (over >> b & 1)) {
             if (lane == 0) {
                 out = (double)sc;
                 tok = eos;
             }
-        } else if (!dead) {
-            const T *row = logits + (slot0 + b) * ld;
-            WarpList best;
-            float thr = -INFINITY, m = -INFINITY;
+        } else if (alive >> b & 1) {
+            // the row's sum; and a bar: the row's beams-th best is at least any segment's
+            float top = -INFINITY;
             double sum = 0.0;
-            for (int c0 = 0; c0 < vocab; c0 += 32) {
-                const int c = c0 + lane;
-                const float x = fmaxf(c < vocab ? to_f32(row[c]) : -INFINITY, -INFINITY);  // NaN counts as -inf
-                if (x > -INFINITY) {
-                    if (x > m) {
-                        sum = sum * (double)__expf(m - x) + 1.0;
-                        m = x;
-                    } else {
-                        sum += x == m ? 1.0 : (double)__expf(x - m);
+            unsigned bar = 0;
+#pragma unroll 1
+            for (int s = lane; s < segs; s += 32) {
+                const Found *f = find(b, s);
+                const float m = f->top;
+                const double part = f->sum;
+                bar = max(bar, (unsigned)(f->best[beams - 1] >> 32));
+                if (m > top) {
+                    sum *= (double)exp2_approx((top - m) * kLog2e);
+                    top = m;
+                }
+                if (m > -INFINITY) sum += m == top ? part : part * (double)exp2_approx((m - top) * kLog2e);
+            }
+            bar = __reduce_max_sync(kFull, bar);
+            const float all = warp_max(top);
+            if (top != all) sum = top > -INFINITY ? sum * (double)exp2_approx((top - all) * kLog2e) : 0.0;
+            const double lse = log(warp_sum(sum));
+            Key best = segs == 1 && lane < beams ? find(b, 0)->best[lane] : 0;
+            if (segs > 1) {
+                Key *cand = mg.cand[warp];
+                int count = 0;
+                const float inv = 1.0f / (float)beams;
+#pragma unroll 1
+                for (int e0 = 0; e0 < segs * beams; e0 += 128) {
+                    Key key[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int e = e0 + u * 32 + lane, s = (int)(((float)e + 0.5f) * inv);  // e / beams
+                        key[u] = e < segs * beams ? find(b, s)->best[e - s * beams] : 0;
+                    }
+#pragma unroll 1
+                    for (int u = 0; u < 4; ++u) {
+                        const Key c = u == 0 ? key[0] : u == 1 ? key[1] : u == 2 ? key[2] : key[3];
+                        append(cand, c, c != 0 && (unsigned)(c >> 32) >= bar, count, lane);
+                        if (count >= 32) best = take_32(cand, best, count, lane);
                     }
                 }
-                // candidates in index order: a later one that ties with the last of the list loses
-                unsigned some = __ballot_sync(kFull, x > thr);
-                while (some) {
-                    const int src = __ffs(some) - 1;
-                    best.insert(__shfl_sync(kFull, x, src), c0 + src, lane);
-                    thr = __shfl_sync(kFull, best.v, beams - 1);
-                    some &= some - 1;
-                    some &= __ballot_sync(kFull, x > thr);
-                }
+                if (count > 0) best = take_32(cand, best, count, lane);
+                __syncwarp();
             }
-            const float top = warp_max(m);
-            const double lse = log(warp_sum(m > -INFINITY ? (m == top ? sum : sum * exp((double)m - (double)top)) : 0.0));
-            if (lane < beams && best.i != kNone) {
-                out = (double)sc + ((best.v == top ? 0.0 : (double)best.v - (double)top) - lse);
-                tok = best.i;
+            if (lane < beams && best) {
+                const float x = key_value(best);
+                out = (double)sc + ((x == all ? 0.0 : (double)x - (double)all) - lse);
+                tok = key_index(best);
             }
         }
         if (!((float)out > -INFINITY)) out = -INFINITY;
         if (lane < beams) {
-            s_score[b][lane] = out;
-            s_tok[b][lane] = tok;
+            mg.score[b][lane] = out + 0.0;  // no -0: scores are compared by their bits below
+            mg.tok[b][lane] = tok;
         }
-        if (lane == 0) s_fin[b] = fin;
     }
     __syncthreads();
     if (warp != 0) return;
-    int head = 0;
+    int head = 1;
+    double v = lane < beams ? mg.score[lane][0] : -INFINITY;
+    double v1 = lane < beams && beams > 1 ? mg.score[lane][1] : -INFINITY;  // the next, ahead of its use
+    unsigned key = ordered((float)v);
+#pragma unroll 1
     for (int k = 0; k < beams; ++k) {
-        double v = lane < beams && head < beams ? s_score[lane][head] : -INFINITY;
-        int who = lane;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {  // ties between beams go to the lower beam
-            const double ov = __shfl_xor_sync(kFull, v, o);
-            const int ow = __shfl_xor_sync(kFull, who, o);
-            if (ov > v || (ov == v && ow < who)) {
-                v = ov;
-                who = ow;
+        // the largest in f32 (rounding keeps the order); only lanes that tie there compare in f64
+        const unsigned most = __reduce_max_sync(kFull, key);
+        unsigned tied = __ballot_sync(kFull, key == most);
+        int who = __ffs(tied) - 1;
+        const bool none = most == ordered(-INFINITY);
+        if ((tied & (tied - 1)) && !none) {
+            double top = __shfl_sync(kFull, v, who);
+#pragma unroll 1
+            while (tied &= tied - 1) {  // ties between beams go to the lower beam
+                const int w = __ffs(tied) - 1;
+                const double o = __shfl_sync(kFull, v, w);
+                if (o > top) {
+                    top = o;
+                    who = w;
+                }
             }
         }
-        const bool none = !(v > -INFINITY);
         if (lane == who) {
-            const int tok = none ? (eos < 0 ? 0 : eos) : s_tok[who][head];
-            const int parent = none ? k : who;
+            const int tok = none ? max(eos, 0) : mg.tok[lane][head - 1];
             out_scores[slot0 + k] = (float)v;
             out_tokens[slot0 + k] = tok;
-            out_parents[slot0 + k] = parent;
-            out_finished[slot0 + k] = eos >= 0 && (none || tok == eos || s_fin[who]);
+            out_parents[slot0 + k] = none ? k : lane;
+            out_finished[slot0 + k] = eos >= 0 && (none || tok == eos || (over >> lane & 1));
             ++head;
+            v = v1;
+            key = ordered((float)v);
+            v1 = head < beams && lane < beams ? mg.score[lane][head] : -INFINITY;
         }
     }
+}
+
+// A line's beams: bit b of `alive` when beam b has a score above -inf (a NaN
+// has not), of `over` when it is finished.
+struct Line {
+    float score;  // lane b: beam b's
+    unsigned alive, over;
+    __device__ __forceinline__ void load(const float *scores, const uint8_t *finished, i64 slot0, int beams) {
+        const int lane = threadIdx.x & 31;
+        score = lane < beams ? scores[slot0 + lane] : -INFINITY;
+        const bool fin = lane < beams && finished && finished[slot0 + lane];
+        alive = __ballot_sync(kFull, score > -INFINITY);
+        over = __ballot_sync(kFull, fin);
+    }
+};
+
+// Short rows: a CTA a line, a warp a row.
+template <class T>
+__global__ void __launch_bounds__(512) select_line_kernel(const T *__restrict__ logits, i64 ld, const float *scores,
+                                                          const uint8_t *finished, int beams, int vocab, int eos,
+                                                          float *out_scores, int32_t *__restrict__ out_tokens,
+                                                          int32_t *__restrict__ out_parents, uint8_t *out_finished) {
+    extern __shared__ __align__(16) uint8_t sel_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const i64 slot0 = (i64)blockIdx.x * beams;
+    Merge &mg = *reinterpret_cast<Merge *>(sel_smem);
+    Scan *scan = reinterpret_cast<Scan *>(&mg + 1);
+    Found *found = reinterpret_cast<Found *>(scan + warps);
+    Line line;
+    line.load(scores, finished, slot0, beams);
+#pragma unroll 1
+    for (int b = warp; b < beams; b += warps)
+        if ((line.alive & ~line.over) >> b & 1)
+            scan_segment<T>(logits + (slot0 + b) * ld, 0, vocab, beams, lane, scan[warp], found[b]);
+    __syncwarp();  // (the warp that scanned a row joins it too)
+    merge_line([&](int b, int) -> const Found * { return found + b; }, 1, line.score, line.alive, line.over, beams, eos,
+               slot0, mg, out_scores, out_tokens, out_parents, out_finished);
+}
+
+// Long rows, first part: a warp a segment of a row, to the workspace.  Warps
+// of dead and finished beams end at once; the others come and go, so that
+// some read while others pick their best.
+constexpr int kScanWarps = 4;
+template <class T>
+__global__ void __launch_bounds__(kScanWarps * 32, 6) select_scan_kernel(
+    const T *__restrict__ logits, i64 ld, const float *__restrict__ scores, const uint8_t *__restrict__ finished,
+    int beams, int vocab, int segs, int seg_len, i64 units, Found *__restrict__ found) {
+    __shared__ Scan scan[kScanWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const i64 u = (i64)blockIdx.x * kScanWarps + warp;
+    if (u >= units) return;
+    const i64 row = u / segs;
+    if (!(scores[row] > -INFINITY) || (finished && finished[row])) return;
+    const int c0 = (int)(u - row * segs) * seg_len;
+    scan_segment<T>(logits + row * ld, c0, min(vocab, c0 + seg_len), beams, lane, scan[warp], found[u]);
+}
+
+// Second part: a CTA a line.
+__global__ void __launch_bounds__(512) select_merge_kernel(const Found *__restrict__ found, int segs,
+                                                           const float *scores, const uint8_t *finished, int beams,
+                                                           int eos, float *out_scores, int32_t *__restrict__ out_tokens,
+                                                           int32_t *__restrict__ out_parents, uint8_t *out_finished) {
+    extern __shared__ __align__(16) uint8_t sel_smem[];
+    const i64 slot0 = (i64)blockIdx.x * beams;
+    Line line;
+    line.load(scores, finished, slot0, beams);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first part ends
+    merge_line([&](int b, int s) -> const Found * { return found + (slot0 + b) * segs + s; }, segs, line.score,
+               line.alive, line.over, beams, eos, slot0, *reinterpret_cast<Merge *>(sel_smem), out_scores, out_tokens,
+               out_parents, out_finished);
 }
 
 // -------------------------------------------------------------- reordering --
@@ -226,13 +665,82 @@ int launched() {
     return (int)e;
 }
 
+// How a selection runs: rows of up to two batches whole (segs = 0), longer
+// ones in segments of whole batches: one round of warps on the device, but no
+// segment so short that picking its best (and joining them, with many beams)
+// costs more than reading it, and none much longer than the spans that are
+// remembered.  64 lines of 10 beams, 65536 f32: 72 us at 2 batches a segment,
+// 43 at 8, 38 at 24; 8 lines of 4 beams, 32000 f32: 12 us at 2, 19 at 24.
+struct Plan {
+    int segs, len;
+    Plan(int lines, int beams, int vocab, int size) {
+        const int batch = kSelUnroll * 32 * 16 / size, batches = (vocab - 1) / batch + 1;
+        segs = len = 0;
+        if (batches <= 2) return;
+        const i64 all = (i64)lines * beams * batches, slots = (i64)sm_count() * 6 * kScanWarps;
+        const int least = beams > 8 ? beams / 4 : 2, most = 24;
+        int per = all >= slots * most ? most : (int)(all / slots) + 1;
+        if (per < least) per = least;
+        if (per < (batches + 127) / 128) per = (batches + 127) / 128;
+        segs = (batches + per - 1) / per;
+        len = (batches + segs - 1) / segs * batch;
+        segs = (vocab - 1) / len + 1;
+    }
+};
+
+int size_of(int dtype) { return dtype == TRBA_F32 ? 4 : 2; }
+
+// Raises a kernel's shared-memory limit, once a device.
+template <class K>
+int allow_smem(K kernel, std::atomic<unsigned long long> &done) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) {
+        report_error(__FILE__, __LINE__, cudaGetErrorString(e), (int)e);
+        return (int)e;
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
+
 template <class T>
 int select(const void *logits, i64 ld, const float *scores, const uint8_t *finished, int lines, int beams, int vocab,
            int eos, float *out_scores, int32_t *out_tokens, int32_t *out_parents, uint8_t *out_finished,
-           cudaStream_t st) {
-    beam_select_kernel<T><<<lines, kSelThreads, 0, st>>>(static_cast<const T *>(logits), ld, scores, finished, beams,
-                                                         vocab, eos, out_scores, out_tokens, out_parents,
-                                                         out_finished);
+           void *workspace, cudaStream_t st) {
+    const Plan plan(lines, beams, vocab, (int)sizeof(T));
+    const int warps = beams < 16 ? beams : 16;
+    if (plan.segs == 0) {
+        static std::atomic<unsigned long long> sized{0};
+        if (const int e = allow_smem(select_line_kernel<T>, sized)) return e;
+        const size_t smem = sizeof(Merge) + sizeof(Scan) * warps + sizeof(Found) * beams;
+        select_line_kernel<T><<<lines, warps * 32, smem, st>>>(static_cast<const T *>(logits), ld, scores, finished,
+                                                               beams, vocab, eos, out_scores, out_tokens, out_parents,
+                                                               out_finished);
+        return launched();
+    }
+    static std::atomic<unsigned long long> sized{0};
+    Found *found = static_cast<Found *>(workspace);
+    const i64 units = (i64)lines * beams * plan.segs;
+    select_scan_kernel<T><<<(unsigned)((units + kScanWarps - 1) / kScanWarps), kScanWarps * 32, 0, st>>>(
+        static_cast<const T *>(logits), ld, scores, finished, beams, vocab, plan.segs, plan.len, units, found);
+    if (const int e = launched()) return e;
+    if (const int e = allow_smem(select_merge_kernel, sized)) return e;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(lines);
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = sizeof(Merge);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, select_merge_kernel, static_cast<const Found *>(found), plan.segs, scores, finished, beams,
+                       eos, out_scores, out_tokens, out_parents, out_finished);
     return launched();
 }
 
@@ -243,11 +751,19 @@ using namespace trba;
 
 extern "C" {
 
+long long trba_beam_select_workspace(int dtype, int lines, int beams, int vocab) {
+    if (lines <= 0 || beams <= 0 || beams > TRBA_MAX_BEAMS || vocab <= 0 || vocab > (1 << 30) ||
+        (dtype != TRBA_F32 && dtype != TRBA_BF16 && dtype != TRBA_F16))
+        return 0;
+    return (long long)sizeof(Found) * lines * beams * Plan(lines, beams, vocab, size_of(dtype)).segs;
+}
+
 int trba_beam_select(const void *logits, int dtype, long long ld, const float *scores, const uint8_t *finished,
                      int lines, int beams, int vocab, int eos, float *out_scores, int32_t *out_tokens,
-                     int32_t *out_parents, uint8_t *out_finished, void *stream) {
-    TRBA_REQUIRE_RET(lines >= 0 && beams > 0 && beams <= TRBA_MAX_BEAMS && vocab > 0 && ld >= vocab &&
-                         (i64)beams * vocab < (1ll << 31),
+                     int32_t *out_parents, uint8_t *out_finished, void *workspace, long long workspace_bytes,
+                     void *stream) {
+    TRBA_REQUIRE_RET(lines >= 0 && beams > 0 && beams <= TRBA_MAX_BEAMS && vocab > 0 && vocab <= (1 << 30) &&
+                         ld >= vocab && (i64)beams * vocab < (1ll << 31) && (i64)lines * beams < (1ll << 24),
                      "trba_beam_select: bad sizes", -1);
     TRBA_REQUIRE_RET(eos >= -1 && eos < vocab && (eos >= 0 || !finished),
                      "trba_beam_select: eos outside the vocabulary, or finished beams without an end token", -1);
@@ -256,17 +772,20 @@ int trba_beam_select(const void *logits, int dtype, long long ld, const float *s
     if (lines == 0) return 0;
     TRBA_REQUIRE_RET(logits && scores && out_scores && out_tokens && out_parents && out_finished,
                      "trba_beam_select: null pointer", -1);
-    TRBA_REQUIRE_RET(reinterpret_cast<uintptr_t>(logits) % (dtype == TRBA_F32 ? 4 : 2) == 0,
+    TRBA_REQUIRE_RET(reinterpret_cast<uintptr_t>(logits) % size_of(dtype) == 0,
                      "trba_beam_select: logits are not aligned to their elements", -1);
+    const long long need = trba_beam_select_workspace(dtype, lines, beams, vocab);
+    TRBA_REQUIRE_RET(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                     "trba_beam_select: workspace missing, too small or not aligned to 16 bytes", -1);
     cudaStream_t st = as_stream(stream);
     if (dtype == TRBA_F32)
         return select<float>(logits, ld, scores, finished, lines, beams, vocab, eos, out_scores, out_tokens,
-                             out_parents, out_finished, st);
+                             out_parents, out_finished, workspace, st);
     if (dtype == TRBA_BF16)
         return select<__nv_bfloat16>(logits, ld, scores, finished, lines, beams, vocab, eos, out_scores, out_tokens,
-                                     out_parents, out_finished, st);
+                                     out_parents, out_finished, workspace, st);
     return select<__half>(logits, ld, scores, finished, lines, beams, vocab, eos, out_scores, out_tokens, out_parents,
-                          out_finished, st);
+                          out_finished, workspace, st);
 }
 
 int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t *parents, int lines, int beams,

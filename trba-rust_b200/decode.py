@@ -127,8 +127,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         ld = logits.stride(0)
     else:
         raise ValueError("logits must be [lines * beams, vocab] or [lines, beams, vocab]")
-    if vocab < 1 or beams * vocab >= 1 << 31:
-        raise ValueError("vocab must be positive and beams * vocab below 2**31")
+    if not 1 <= vocab <= 1 << 30 or beams * vocab >= 1 << 31:
+        raise ValueError("vocab must be 1 to 2**30 and beams * vocab below 2**31")
+    if lines * beams >= 1 << 24:
+        raise ValueError("lines * beams must be below 2**24")
     if vocab > 1 and logits.stride(-1) != 1:
         raise ValueError("the logits of a row must be contiguous")
     if lines * beams > 1:
@@ -161,9 +163,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
                 _check_out(f"out.{name}", t, (lines, beams), dtype, device)
         if lines:
             L = lib()
+            need = L.trba_beam_select_workspace(code, lines, beams, vocab)
+            work = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
             rc = L.trba_beam_select(logits.data_ptr(), code, ld, scores.data_ptr(), fin, lines, beams, vocab, eos,
                                     out.scores.data_ptr(), out.tokens.data_ptr(), out.parents.data_ptr(),
-                                    out.finished.data_ptr(), s.ptr)
+                                    out.finished.data_ptr(), work, need, s.ptr)
             if rc:
                 _fail(L, "beam_select", rc)
     return out
