@@ -595,67 +595,194 @@ __global__ void __launch_bounds__(512) select_merge_kernel(const Found *__restri
 }
 
 // -------------------------------------------------------------- reordering --
+// A copy, bound by memory.  A warp moves a piece of a row at a time, 4 units of
+// 16 bytes or 8 smaller ones a lane in flight.  Rows whose addresses are all multiples of
+// 4, 8 or 16 bytes go in such units; others in 4-byte words of the
+// destination, each put together from the two source words it lies in.
 constexpr int kMaxStates = 16;
+__host__ __device__ constexpr int moves_of(int vec) { return vec == 16 ? 4 : 8; }
 struct StateView {
     const char *src;
     char *dst;
-    i64 units, src_row, dst_row, mid, src_mid, dst_mid, src_outer, dst_outer, total;
-    int vec;
+    i64 bytes, src_row, dst_row, src_mid, dst_mid, src_outer, dst_outer;
+    int mid, per_row;  // parts of a row; pieces of a part
+    int vec;           // unit in bytes, 0: words that are put together
+    int first;         // the state's first piece in the launch
 };
 struct StateViews {
     StateView s[kMaxStates];
+    int n, pieces;
 };
 
-// Grid y is the state; its units of `vec` bytes in the order [outer][row][mid][unit].
 template <class V>
-__device__ __forceinline__ void reorder_units(const StateView &s, const int32_t *__restrict__ parents, i64 rows,
-                                              int beams) {
-    GRID_LOOP(e, s.total) {
-        const i64 u = e % s.units, q = e / s.units, mid = q % s.mid, q2 = q / s.mid, row = q2 % rows, o = q2 / rows;
-        const int p = parents[row];
-        if ((unsigned)p >= (unsigned)beams) continue;
-        const i64 from = row - row % beams + p;
-        *reinterpret_cast<V *>(s.dst + o * s.dst_outer + row * s.dst_row + mid * s.dst_mid + u * sizeof(V)) =
-            *reinterpret_cast<const V *>(s.src + o * s.src_outer + from * s.src_row + mid * s.src_mid + u * sizeof(V));
+__device__ __forceinline__ void move_units(const char *src, char *dst, i64 units, int lane) {
+    constexpr int kMoves = moves_of(sizeof(V));
+    V v[kMoves];
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u)
+        if (u * 32 + lane < units) v[u] = __ldcs(reinterpret_cast<const V *>(src) + u * 32 + lane);
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u)
+        if (u * 32 + lane < units) __stcs(reinterpret_cast<V *>(dst) + u * 32 + lane, v[u]);
+}
+
+// `bytes` from any src to any dst, at most moves_of(0) * 128.
+__device__ __forceinline__ void move_bytes(const char *src, char *dst, int bytes, int lane) {
+    const int head = min(bytes, (int)(-reinterpret_cast<uintptr_t>(dst) & 3)), words = (bytes - head) >> 2;
+    if (lane < head) dst[lane] = src[lane];
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src + head);
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3);
+    const int shift = (int)(at & 3) * 8;
+    constexpr int kMoves = moves_of(0);
+    uint32_t lo[kMoves], hi[kMoves];
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u) {
+        const int i = u * 32 + lane;
+        if (i < words) {
+            lo[u] = w[i];
+            hi[u] = shift ? w[i + 1] : 0;  // holds bytes of this word
+        }
     }
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u) {
+        const int i = u * 32 + lane;
+        if (i < words) reinterpret_cast<uint32_t *>(dst + head)[i] = __funnelshift_r(lo[u], hi[u], shift);
+    }
+    const int done = head + words * 4;
+    if (lane < bytes - done) dst[done + lane] = src[done + lane];
 }
 
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant__ StateViews st,
-                                                           const int32_t *__restrict__ parents, i64 rows, int beams) {
-    const StateView &s = st.s[blockIdx.y];
-    if (s.vec == 16) reorder_units<uint4>(s, parents, rows, beams);
-    else if (s.vec == 8) reorder_units<uint2>(s, parents, rows, beams);
-    else if (s.vec == 4) reorder_units<uint32_t>(s, parents, rows, beams);
-    else if (s.vec == 2) reorder_units<uint16_t>(s, parents, rows, beams);
-    else reorder_units<uint8_t>(s, parents, rows, beams);
+                                                           const int32_t *__restrict__ parents, int rows, int beams) {
+    const int lane = threadIdx.x & 31, warps = gridDim.x * 8;
+    int k = 0;
+    for (int piece = blockIdx.x * 8 + (threadIdx.x >> 5); piece < st.pieces; piece += warps) {
+        while (k + 1 < st.n && piece >= st.s[k + 1].first) ++k;
+        const StateView &s = st.s[k];
+        const int local = piece - s.first, part = local / s.per_row, q = local - part * s.per_row;
+        const int row_o = part / s.mid, mid = part - row_o * s.mid, outer = row_o / rows, row = row_o - outer * rows;
+        const int p = parents[row];
+        if ((unsigned)p >= (unsigned)beams) continue;
+        const int from = row - row % beams + p;
+        const int unit = s.vec ? s.vec : 4;
+        const i64 at = (i64)q * (moves_of(s.vec) * 32) * unit, left = s.bytes - at;
+        const char *src = s.src + outer * s.src_outer + (i64)from * s.src_row + mid * s.src_mid + at;
+        char *dst = s.dst + outer * s.dst_outer + (i64)row * s.dst_row + mid * s.dst_mid + at;
+        if (s.vec == 16) move_units<uint4>(src, dst, left / 16, lane);
+        else if (s.vec == 8) move_units<uint2>(src, dst, left / 8, lane);
+        else if (s.vec == 4) move_units<uint32_t>(src, dst, left / 4, lane);
+        else move_bytes(src, dst, (int)min(left, (i64)moves_of(0) * 128), lane);
+    }
 }
 
 // --------------------------------------------------------------- sequences --
-// One thread a slot walks from the last step to the first.
-__global__ void __launch_bounds__(128) beam_sequences_kernel(const int32_t *__restrict__ tokens,
-                                                             const int32_t *__restrict__ parents, int steps, int lines,
-                                                             int beams, int eos, int pad, int32_t *__restrict__ seq,
-                                                             int32_t *__restrict__ lengths) {
-    const i64 n = (i64)lines * beams, e = (i64)blockIdx.x * blockDim.x + threadIdx.x;
-    if (e >= n) return;
-    const i64 line0 = e - e % beams;
-    int slot = (int)(e % beams), len = steps;
-    bool bad = false;
-    for (int t = steps - 1; t >= 0; --t) {
-        const i64 at = t * n + line0 + slot;
-        const int tok = tokens[at];
-        seq[e * steps + t] = tok;
-        if (tok == eos) len = t;
-        if (t > 0) {
-            slot = parents[at];
-            if ((unsigned)slot >= (unsigned)beams) {
-                bad = true;
-                break;
+// A path is a chain of dependent reads, so the walk goes over shared memory
+// and in parallel: the steps are cut into segments, one thread a segment and
+// slot finds where the slot leads to at the segment's start, the segments'
+// maps are composed, and a second walk from the right slots notes the path.
+// A CTA takes `group` lines, or a part of one line's beams (all CTAs of a line
+// read its parents).  Steps that do not fit go in chunks, last first.
+constexpr uint8_t kLost = 255;  // behind a parent out of range
+
+constexpr int kTraceSmem = 96 * 1024;
+
+struct Trace {
+    const int32_t *tokens, *parents;
+    int32_t *seq, *lengths;
+    int steps, lines, beams, eos, pad;
+    int group, segs, chunk, splits;
+};
+
+constexpr int kTraceThreads = 512, kTraceLoads = 4;  // loads in flight a thread
+
+__global__ void __launch_bounds__(kTraceThreads) beam_sequences_kernel(const Trace a) {
+    extern __shared__ uint8_t tr_smem[];
+    const int gk = a.group * a.beams;  // slots of the CTA's lines
+    uint8_t *par = tr_smem;            // [chunk][gk]
+    uint8_t *path = par + a.chunk * gk;
+    uint8_t *map = path + a.chunk * gk;  // [segs][gk], then the segments' entry slots
+    uint8_t *end = map + a.segs * gk;    // [gk]: where the paths stand
+    int *len = reinterpret_cast<int *>(tr_smem + ((2 * a.chunk * gk + (a.segs + 1) * gk + 3) & ~3));
+    const int line0 = blockIdx.x * a.group, slots = min(a.group, a.lines - line0) * a.beams;
+    // the slots whose sequences this CTA writes
+    const int k0 = slots * blockIdx.y / a.splits, own = slots * (blockIdx.y + 1) / a.splits - k0;
+    const i64 n = (i64)a.lines * a.beams, base = (i64)line0 * a.beams;
+    const int32_t *__restrict__ parents = a.parents + base, *__restrict__ tokens = a.tokens + base;
+    for (int e = threadIdx.x; e < slots; e += kTraceThreads) {
+        end[e] = (uint8_t)(e % a.beams);
+        len[e] = a.steps;
+    }
+    for (int hi = a.steps; hi > 0; hi -= a.chunk) {  // the steps [lo, hi)
+        const int lo = max(0, hi - a.chunk), c = hi - lo;
+        __syncthreads();
+        for (int e0 = threadIdx.x; e0 < c * slots; e0 += kTraceThreads * kTraceLoads) {
+            int p[kTraceLoads], at[kTraceLoads];
+#pragma unroll
+            for (int u = 0; u < kTraceLoads; ++u) {
+                const int e = e0 + u * kTraceThreads, t = e / slots, k = e - t * slots;
+                at[u] = t * gk + k;
+                p[u] = e < c * slots && lo + t ? parents[(lo + t) * n + k] : 0;  // step 0 has no parents
+            }
+#pragma unroll
+            for (int u = 0; u < kTraceLoads; ++u)
+                if (e0 + u * kTraceThreads < c * slots)
+                    par[at[u]] = (unsigned)p[u] < (unsigned)a.beams ? (uint8_t)p[u] : kLost;
+        }
+        __syncthreads();
+        const int per = (c + a.segs - 1) / a.segs;
+        for (int w = threadIdx.x; w < a.segs * slots; w += kTraceThreads) {
+            const int s = w / slots, e = w - s * slots, l = e - e % a.beams;
+            uint8_t x = (uint8_t)(e % a.beams);
+            for (int t = min(c, (s + 1) * per) - 1; t >= s * per && x != kLost; --t) x = par[t * gk + l + x];
+            map[s * gk + e] = x;
+        }
+        __syncthreads();
+        // maps become entry slots; a segment's map is read by all slots of its
+        // line, so the entries wait in the path's first rows
+        for (int e = threadIdx.x; e < slots; e += kTraceThreads) {
+            const int l = e - e % a.beams;
+            uint8_t x = end[e];
+            for (int s = a.segs - 1; s >= 0; --s) {
+                path[s * gk + e] = x;
+                if (x != kLost) x = map[s * gk + l + x];
+            }
+            end[e] = x;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < a.segs * gk; e += kTraceThreads) map[e] = path[e];
+        __syncthreads();
+        for (int w = threadIdx.x; w < a.segs * own; w += kTraceThreads) {
+            const int s = w / own, e = k0 + w - s * own, l = e - e % a.beams;
+            uint8_t x = map[s * gk + e];
+            for (int t = min(c, (s + 1) * per) - 1; t >= s * per; --t) {
+                path[t * gk + e] = x;
+                if (x != kLost) x = par[t * gk + l + x];
+            }
+        }
+        __syncthreads();
+        for (int e0 = threadIdx.x; e0 < c * own; e0 += kTraceThreads * kTraceLoads) {
+            int tok[kTraceLoads], k[kTraceLoads], t[kTraceLoads], x[kTraceLoads];
+#pragma unroll
+            for (int u = 0; u < kTraceLoads; ++u) {
+                const int e = min(e0 + u * kTraceThreads, c * own - 1), q = e / c;
+                t[u] = e - q * c, k[u] = k0 + q;
+                x[u] = path[t[u] * gk + k[u]];
+                tok[u] = x[u] == kLost ? a.pad : tokens[(lo + t[u]) * n + k[u] - k[u] % a.beams + x[u]];
+            }
+#pragma unroll
+            for (int u = 0; u < kTraceLoads; ++u) {
+                if (e0 + u * kTraceThreads >= c * own) break;
+                if (x[u] == kLost) atomicMin(&len[k[u]], -1);
+                else if (tok[u] == a.eos) atomicMin(&len[k[u]], lo + t[u]);
+                a.seq[(base + k[u]) * a.steps + lo + t[u]] = tok[u];
             }
         }
     }
-    for (int t = bad ? 0 : len; t < steps; ++t) seq[e * steps + t] = pad;
-    lengths[e] = bad ? -1 : len;
+    __syncthreads();
+    for (int e = threadIdx.x; e < own; e += kTraceThreads) a.lengths[base + k0 + e] = len[k0 + e];
+    for (int e = threadIdx.x >> 5; e < own; e += kTraceThreads / 32)  // what follows the end
+        for (int t = max(0, len[k0 + e]) + (threadIdx.x & 31); t < a.steps; t += 32)
+            a.seq[(base + k0 + e) * a.steps + t] = a.pad;
 }
 
 int launched() {
@@ -795,17 +922,19 @@ int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t
     if (n_states == 0 || lines == 0) return 0;
     TRBA_REQUIRE_RET(states && parents, "trba_beam_reorder: null pointer", -1);
     const i64 rows = (i64)lines * beams;
+    TRBA_REQUIRE_RET(rows < (1ll << 24), "trba_beam_reorder: bad sizes", -1);
     for (int i = 0; i < n_states; ++i) {
         const trba_beam_state &s = states[i];
         TRBA_REQUIRE_RET(s.bytes >= 0 && s.mid >= 0 && s.outer >= 0, "trba_beam_reorder: negative size", -1);
         TRBA_REQUIRE_RET((s.src && s.dst) || s.bytes == 0 || s.mid == 0 || s.outer == 0,
                          "trba_beam_reorder: null state", -1);
+        TRBA_REQUIRE_RET(s.mid < (1ll << 31) && s.outer < (1ll << 31), "trba_beam_reorder: bad sizes", -1);
     }
-    for (int i0 = 0; i0 < n_states; i0 += kMaxStates) {
+    int i = 0;
+    while (i < n_states) {
         StateViews v{};
-        int n = 0;
-        i64 most = 0;
-        for (int i = i0; i < n_states && i < i0 + kMaxStates; ++i) {
+        i64 pieces = 0;
+        for (; i < n_states && v.n < kMaxStates; ++i) {
             const trba_beam_state &s = states[i];
             if (s.bytes == 0 || s.mid == 0 || s.outer == 0) continue;
             // the widest unit that every address of the view is a multiple of
@@ -813,21 +942,30 @@ int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t
                        s.src_row | s.dst_row;
             if (s.mid > 1) bits |= s.src_mid | s.dst_mid;
             if (s.outer > 1) bits |= s.src_outer | s.dst_outer;
-            int vec = 16;
-            while (bits & (vec - 1)) vec >>= 1;
-            StateView &d = v.s[n++];
+            StateView &d = v.s[v.n];
+            d.vec = !(bits & 15) ? 16 : !(bits & 7) ? 8 : !(bits & 3) ? 4 : 0;
+            const i64 piece = moves_of(d.vec) * 32 * (d.vec ? d.vec : 4), per_row = (s.bytes - 1) / piece + 1;
+            const double all = (double)per_row * (double)s.mid * (double)s.outer * (double)rows;
+            TRBA_REQUIRE_RET(all < 2147483647.0, "trba_beam_reorder: a state is too large for one launch", -1);
+            const i64 mine = per_row * s.mid * s.outer * rows;
+            if (pieces + mine > 2147483647ll - (1 << 20)) break;  // the next launch takes it
+            d.first = (int)pieces;
+            pieces += mine;
             d.src = static_cast<const char *>(s.src);
             d.dst = static_cast<char *>(s.dst);
-            d.vec = vec;
-            d.units = s.bytes / vec;
+            d.bytes = s.bytes, d.per_row = (int)per_row, d.mid = (int)s.mid;
             d.src_row = s.src_row, d.dst_row = s.dst_row;
-            d.mid = s.mid, d.src_mid = s.src_mid, d.dst_mid = s.dst_mid;
+            d.src_mid = s.src_mid, d.dst_mid = s.dst_mid;
             d.src_outer = s.src_outer, d.dst_outer = s.dst_outer;
-            d.total = d.units * s.mid * s.outer * rows;
-            if (d.total > most) most = d.total;
+            ++v.n;
         }
-        if (n == 0) continue;
-        beam_reorder_kernel<<<dim3(grid_for(most), n), 256, 0, as_stream(stream)>>>(v, parents, rows, beams);
+        if (v.n == 0) {
+            TRBA_REQUIRE_RET(i >= n_states, "trba_beam_reorder: a state is too large for one launch", -1);
+            break;
+        }
+        v.pieces = (int)pieces;
+        const i64 want = (pieces + 7) / 8, cap = (i64)sm_count() * 8;
+        beam_reorder_kernel<<<(int)(want < cap ? want : cap), 256, 0, as_stream(stream)>>>(v, parents, (int)rows, beams);
         if (const int e = launched()) return e;
     }
     return 0;
@@ -836,14 +974,34 @@ int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t
 int trba_beam_sequences(const int32_t *tokens, const int32_t *parents, int steps, int lines, int beams, int eos,
                         int pad, int32_t *sequences, int32_t *lengths, void *stream) {
     TRBA_REQUIRE_RET(steps >= 0 && lines >= 0 && beams > 0 && beams <= TRBA_MAX_BEAMS &&
-                         (i64)lines * beams < (1ll << 31),
+                         (i64)lines * beams < (1ll << 24) && steps < (1 << 24),
                      "trba_beam_sequences: bad sizes", -1);
     if (lines == 0) return 0;
     TRBA_REQUIRE_RET(lengths && (steps == 0 || (tokens && parents && sequences)), "trba_beam_sequences: null pointer",
                      -1);
-    const i64 n = (i64)lines * beams;
-    beam_sequences_kernel<<<(int)((n + 127) / 128), 128, 0, as_stream(stream)>>>(tokens, parents, steps, lines, beams,
-                                                                                 eos, pad, sequences, lengths);
+    Trace a{};
+    a.tokens = tokens, a.parents = parents, a.seq = sequences, a.lengths = lengths;
+    a.steps = steps, a.lines = lines, a.beams = beams, a.eos = eos, a.pad = pad;
+    // About as many segments as steps in a segment, and lines until a CTA's
+    // threads have a walk each, as long as that leaves a CTA for every SM;
+    // few lines of many steps are split by their beams instead.
+    a.segs = 1;
+    while (a.segs < 64 && a.segs * a.segs * 2 < steps) a.segs *= 2;
+    a.group = kTraceThreads / (beams * a.segs);
+    const int even = (lines + sm_count() - 1) / sm_count();
+    if (a.group > even) a.group = even;
+    if (a.group < 1) a.group = 1;
+    a.splits = 1;
+    while (steps >= 128 && a.group == 1 && a.splits < 8 && 2 * a.splits <= beams && 2 * a.splits * lines <= sm_count())
+        a.splits *= 2;
+    const int gk = a.group * beams;
+    a.chunk = kTraceSmem / (2 * gk);
+    if (a.chunk > steps) a.chunk = steps;
+    if (a.chunk < a.segs) a.chunk = a.segs;  // (the entry slots pass through the path's rows)
+    const size_t smem = (((size_t)2 * a.chunk * gk + (size_t)(a.segs + 1) * gk + 3) & ~(size_t)3) + (size_t)gk * 4;
+    static std::atomic<unsigned long long> sized{0};
+    if (const int e = allow_smem(beam_sequences_kernel, sized)) return e;
+    beam_sequences_kernel<<<dim3((lines + a.group - 1) / a.group, a.splits), kTraceThreads, smem, as_stream(stream)>>>(a);
     return launched();
 }
 

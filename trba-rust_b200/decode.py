@@ -10,6 +10,7 @@ are checked here: a ValueError or TypeError means that nothing ran.
 """
 from __future__ import annotations
 
+import math
 import struct
 from typing import NamedTuple, Sequence
 
@@ -32,35 +33,25 @@ def _fail(L, what, rc):
     raise RuntimeError(f"{what} failed ({rc}): " + L.trba_last_error_string().decode())
 
 
-class on_stream:
-    """Makes `stream` (None: the current one) and the tensors' device current
-    for one call; `.ptr` is the stream handle."""
-    __slots__ = ("device", "stream", "ptr", "ctx")
+Tensor = torch.Tensor
+# the raw handle of torch's current stream of a device, without the object around it where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = torch.cuda.current_device
 
-    def __init__(self, device: torch.device, stream):
-        self.device, self.stream, self.ctx = device, stream, None
 
-    def __enter__(self):
-        index = self.device.index
-        if self.stream is not None:
-            if self.stream.device != self.device:
-                raise ValueError(f"stream is on {self.stream.device}, the tensors are on {self.device}")
-            self.ctx = torch.cuda.stream(self.stream)
-            self.ctx.__enter__()
-        elif index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(index)
-            self.ctx.__enter__()
-        self.ptr = torch.cuda.current_stream(index).cuda_stream
-        return self
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _on(device: torch.device, stream):
+    """Context in which `stream` (None: the device's current one) and `device` are current."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
+    return torch.cuda.stream(stream)
 
 
 def _check_tensors(**tensors):
     for name, t in tensors.items():
-        if t is not None and not isinstance(t, torch.Tensor):
+        if t is not None and not isinstance(t, Tensor):
             raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
 
 
@@ -69,16 +60,6 @@ def _check_cuda(name, t, device=None):
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-
-
-def _check_device(**tensors) -> torch.device:
-    """The one CUDA device that all tensors are on."""
-    device = None
-    for name, t in tensors.items():
-        if t is not None:
-            _check_cuda(name, t, device)
-            device = t.device
-    return device
 
 
 def _check_beams(beams):
@@ -106,7 +87,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     continuations above -inf fills up with score -inf, token eos, parent = the
     slot.  A NaN logit counts as -inf.  `out`: buffers to write into; its
     scores and finished may be the inputs'."""
-    _check_tensors(scores=scores, logits=logits, finished=finished)
+    if not (isinstance(scores, Tensor) and isinstance(logits, Tensor)
+            and (finished is None or isinstance(finished, Tensor))):
+        _check_tensors(scores=scores, logits=logits, finished=finished)
     code = DTYPE_CODES.get(logits.dtype)
     if code is None:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
@@ -114,62 +97,65 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         raise ValueError("scores must be a float32 tensor [lines, beams]")
     lines, beams = scores.shape
     _check_beams(beams)
-    vocab = logits.shape[-1]
-    if logits.dim() == 3:
-        if logits.shape[0] != lines or logits.shape[1] != beams:
-            raise ValueError(f"logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
-        if lines > 1 and logits.stride(0) != beams * logits.stride(1):
+    shape, strides = logits.shape, logits.stride()
+    vocab = shape[-1] if shape else 0
+    if len(shape) == 2 and shape[0] == lines * beams:
+        ld = strides[0]
+    elif len(shape) == 3 and shape[0] == lines and shape[1] == beams:
+        if lines > 1 and strides[0] != beams * strides[1]:
             raise ValueError("logits must have one stride over all (line, beam) rows")
-        ld = logits.stride(1) if beams > 1 else logits.stride(0)
-    elif logits.dim() == 2:
-        if logits.shape[0] != lines * beams:
-            raise ValueError(f"logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
-        ld = logits.stride(0)
+        ld = strides[1] if beams > 1 else strides[0]
     else:
-        raise ValueError("logits must be [lines * beams, vocab] or [lines, beams, vocab]")
+        raise ValueError(f"logits {tuple(shape)} do not fit scores {tuple(scores.shape)}: [lines * beams, vocab] or "
+                         "[lines, beams, vocab] is expected")
     if not 1 <= vocab <= 1 << 30 or beams * vocab >= 1 << 31:
         raise ValueError("vocab must be 1 to 2**30 and beams * vocab below 2**31")
     if lines * beams >= 1 << 24:
         raise ValueError("lines * beams must be below 2**24")
-    if vocab > 1 and logits.stride(-1) != 1:
+    if vocab > 1 and strides[-1] != 1:
         raise ValueError("the logits of a row must be contiguous")
-    if lines * beams > 1:
-        if ld < vocab:
-            raise ValueError("logits rows overlap")
-    else:
+    if lines * beams <= 1:
         ld = vocab
+    elif ld < vocab:
+        raise ValueError("logits rows overlap")
     if not -1 <= eos < vocab:
         raise ValueError(f"eos must be -1 or in [0, {vocab}), got {eos}")
+    device = scores.device
     if finished is not None:
         if eos < 0:
             raise ValueError("finished beams need an end token (eos)")
         if finished.shape != scores.shape or finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError("finished must be a bool or uint8 tensor [lines, beams]")
-    device = _check_device(scores=scores, logits=logits, finished=finished)
-    with on_stream(device, stream) as s:
-        scores, fin = scores.contiguous(), None
-        if finished is not None:
-            finished = finished.contiguous()
-            fin = finished.data_ptr()
-        if out is None:
-            shape = (lines, beams)
-            out = BeamStep(torch.empty(shape, dtype=torch.float32, device=device),
-                           torch.empty(shape, dtype=torch.int32, device=device),
-                           torch.empty(shape, dtype=torch.int32, device=device),
-                           torch.empty(shape, dtype=torch.bool, device=device))
-        else:
-            out = BeamStep(*out)
-            for name, t, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32, torch.bool)):
-                _check_out(f"out.{name}", t, (lines, beams), dtype, device)
-        if lines:
-            L = lib()
-            need = L.trba_beam_select_workspace(code, lines, beams, vocab)
-            work = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
-            rc = L.trba_beam_select(logits.data_ptr(), code, ld, scores.data_ptr(), fin, lines, beams, vocab, eos,
-                                    out.scores.data_ptr(), out.tokens.data_ptr(), out.parents.data_ptr(),
-                                    out.finished.data_ptr(), work, need, s.ptr)
-            if rc:
-                _fail(L, "beam_select", rc)
+        if finished.device != device:
+            _check_cuda("finished", finished, device)
+    if not scores.is_cuda or logits.device != device:
+        _check_cuda("scores", scores)
+        _check_cuda("logits", logits, device)
+    if stream is not None or device.index != _current_device():
+        with _on(device, stream):
+            return beam_select(logits, scores, finished, eos=eos, out=out)
+    if not scores.is_contiguous():
+        scores = scores.contiguous()
+    if finished is not None and not finished.is_contiguous():
+        finished = finished.contiguous()
+    if out is None:
+        empty = torch.empty_like
+        out = BeamStep(empty(scores), empty(scores, dtype=torch.int32), empty(scores, dtype=torch.int32),
+                       empty(scores, dtype=torch.bool))
+    else:
+        out = BeamStep(*out)
+        for name, t, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32, torch.bool)):
+            _check_out(f"out.{name}", t, (lines, beams), dtype, device)
+    if lines:
+        L = lib()
+        need = L.trba_beam_select_workspace(code, lines, beams, vocab)
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = L.trba_beam_select(logits.data_ptr(), code, ld, scores.data_ptr(),
+                                None if finished is None else finished.data_ptr(), lines, beams, vocab, eos,
+                                out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
+                                work.data_ptr() if need else None, need, _raw_stream(device.index))
+        if rc:
+            _fail(L, "beam_select", rc)
     return out
 
 
@@ -189,8 +175,12 @@ def _collapse(shape, src, dst, size):
 
 
 def _state(src, dst, dim):
-    """The ten fields of a trba_beam_state for one tensor and its output."""
+    """The fields of a trba_beam_state for one tensor and its output."""
     size, shape = src.element_size(), src.shape
+    if src.is_contiguous() and dst.is_contiguous():
+        row, outer = math.prod(shape[dim + 1:]) * size, math.prod(shape[:dim])
+        across = shape[dim] * row if outer > 1 else 0
+        return src.data_ptr(), dst.data_ptr(), row, row, row, 1, 0, 0, outer, across, across
     outer = _collapse(shape[:dim], src.stride()[:dim], dst.stride()[:dim], size)
     inner = _collapse(shape[dim + 1:], src.stride()[dim + 1:], dst.stride()[dim + 1:], size)
     nbytes = size
@@ -214,16 +204,21 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
     tensors, or writes into `out` (the same shapes and types, not overlapping
     any state: keep two sets and use them in turn)."""
     states = list(states)
-    _check_tensors(parents=parents, **{f"states[{i}]": t for i, t in enumerate(states)})
+    if not (isinstance(parents, Tensor) and all(isinstance(t, Tensor) for t in states)):
+        _check_tensors(parents=parents, **{f"states[{i}]": t for i, t in enumerate(states)})
     if parents.dim() != 2 or parents.dtype != torch.int32:
         raise ValueError("parents must be an int32 tensor [lines, beams]")
     lines, beams = parents.shape
     _check_beams(beams)
+    rows = lines * beams
+    if rows >= 1 << 24:
+        raise ValueError("lines * beams must be below 2**24")
+    device = parents.device
     for i, t in enumerate(states):
         if not -t.dim() <= dim < t.dim():
             raise ValueError(f"states[{i}] has no dimension {dim}")
-        if t.shape[dim] != lines * beams:
-            raise ValueError(f"states[{i}]: dimension {dim} is {t.shape[dim]}, expected lines * beams = {lines * beams}")
+        if t.shape[dim] != rows:
+            raise ValueError(f"states[{i}]: dimension {dim} is {t.shape[dim]}, expected lines * beams = {rows}")
     if out is not None:
         out = list(out)
         if len(out) != len(states):
@@ -233,27 +228,30 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
             if o.shape != t.shape or o.dtype != t.dtype:
                 raise ValueError(f"out[{i}] must have the shape and type of states[{i}]")
         _check_apart(states, out)
-    device = _check_device(parents=parents)
+    _check_cuda("parents", parents)
     for i, t in enumerate(states):
-        _check_cuda(f"states[{i}]", t, device)
+        if t.device != device:
+            _check_cuda(f"states[{i}]", t, device)
     for i, t in enumerate(out or ()):
         _check_cuda(f"out[{i}]", t, device)
-    with on_stream(device, stream) as s:
+    if stream is not None or device.index != _current_device():
+        with _on(device, stream):
+            return beam_reorder(states, parents, dim=dim, out=out)
+    if not parents.is_contiguous():
         parents = parents.contiguous()
-        if out is None:
-            out = [torch.empty(t.shape, dtype=t.dtype, device=device) for t in states]
-        fields = []
-        n = 0
-        for t, o in zip(states, out):
-            if t.numel():
-                fields += _state(t, o, dim % t.dim())
-                n += 1
-        if n:
-            L = lib()
-            rc = L.trba_beam_reorder(struct.pack(f"={len(fields)}q", *fields), n, parents.data_ptr(), lines, beams,
-                                     s.ptr)
-            if rc:
-                _fail(L, "beam_reorder", rc)
+    if out is None:
+        out = [torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device)
+               for t in states]
+    fields = []
+    for t, o in zip(states, out):
+        if t.numel():
+            fields += _state(t, o, dim if dim >= 0 else dim + t.dim())
+    if fields:
+        L = lib()
+        rc = L.trba_beam_reorder(struct.pack(f"={len(fields)}q", *fields), len(fields) // 11, parents.data_ptr(),
+                                 lines, beams, _raw_stream(device.index))
+        if rc:
+            _fail(L, "beam_reorder", rc)
     return out
 
 
@@ -287,24 +285,30 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1
         raise ValueError("tokens and parents must be int32 tensors [steps, lines, beams]")
     steps, lines, beams = tokens.shape
     _check_beams(beams)
+    if lines * beams >= 1 << 24 or steps >= 1 << 24:
+        raise ValueError("lines * beams and steps must be below 2**24")
     for name, v in (("eos", eos), ("pad", pad)):
         if not -2 ** 31 <= v < 2 ** 31:
             raise ValueError(f"{name} must fit in 32 bits, got {v}")
-    device = _check_device(tokens=tokens, parents=parents)
-    with on_stream(device, stream) as s:
-        tokens, parents = tokens.contiguous(), parents.contiguous()
-        if out is None:
-            out = (torch.empty((lines, beams, steps), dtype=torch.int32, device=device),
-                   torch.empty((lines, beams), dtype=torch.int32, device=device))
-        else:
-            seq, lengths = out
-            _check_out("out[0]", seq, (lines, beams, steps), torch.int32, device)
-            _check_out("out[1]", lengths, (lines, beams), torch.int32, device)
-            out = (seq, lengths)
-        if lines:
-            L = lib()
-            rc = L.trba_beam_sequences(tokens.data_ptr(), parents.data_ptr(), steps, lines, beams, eos, pad,
-                                       out[0].data_ptr(), out[1].data_ptr(), s.ptr)
-            if rc:
-                _fail(L, "beam_sequences", rc)
+    device = tokens.device
+    _check_cuda("tokens", tokens)
+    _check_cuda("parents", parents, device)
+    if stream is not None or device.index != _current_device():
+        with _on(device, stream):
+            return beam_sequences(tokens, parents, eos=eos, pad=pad, out=out)
+    tokens, parents = tokens.contiguous(), parents.contiguous()
+    if out is None:
+        out = (torch.empty((lines, beams, steps), dtype=torch.int32, device=device),
+               torch.empty((lines, beams), dtype=torch.int32, device=device))
+    else:
+        seq, lengths = out
+        _check_out("out[0]", seq, (lines, beams, steps), torch.int32, device)
+        _check_out("out[1]", lengths, (lines, beams), torch.int32, device)
+        out = (seq, lengths)
+    if lines:
+        L = lib()
+        rc = L.trba_beam_sequences(tokens.data_ptr(), parents.data_ptr(), steps, lines, beams, eos, pad,
+                                   out[0].data_ptr(), out[1].data_ptr(), _raw_stream(device.index))
+        if rc:
+            _fail(L, "beam_sequences", rc)
     return out

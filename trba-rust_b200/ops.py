@@ -149,7 +149,7 @@ class LinearInt4:
         float32 or float16; bias [out] float32 or None.  W = (code - 8) *
         scale.  The tensors are copied."""
         import torch
-        from .decode import DTYPE_CODES, _check_device, _check_tensors, on_stream
+        from .decode import DTYPE_CODES, _check_cuda, _check_tensors, _on, _raw_stream
         _check_tensors(codes=codes, scales=scales, bias=bias)
         if in_features < 1 or codes.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[1] != -(-in_features // 2):
             raise ValueError(f"codes must be a uint8 tensor [out, {-(-in_features // 2)}]")
@@ -160,14 +160,18 @@ class LinearInt4:
             raise ValueError(f"scales must be float32 or float16 [{out_features}, {-(-in_features // group)}]")
         if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (out_features,)):
             raise ValueError(f"bias must be float32 [{out_features}]")
-        device = _check_device(codes=codes, scales=scales, bias=bias)
+        device = codes.device
+        for name, t in (("codes", codes), ("scales", scales), ("bias", bias)):
+            if t is not None:
+                _check_cuda(name, t, device)
         self = cls.__new__(cls)
-        with on_stream(device, None) as s:
+        with _on(device, None):
             codes, scales = codes.contiguous(), scales.contiguous()
             bias = None if bias is None else bias.contiguous()
             self._own(in_features, out_features, group, lib().trba_linear_int4_create_codes(
                 in_features, out_features, group, codes.data_ptr(), codes.shape[1], scales.data_ptr(),
-                DTYPE_CODES[scales.dtype], scales.shape[1], None if bias is None else bias.data_ptr(), s.ptr))
+                DTYPE_CODES[scales.dtype], scales.shape[1], None if bias is None else bias.data_ptr(),
+                _raw_stream(device.index)))
         return self
 
     def close(self):
@@ -186,38 +190,45 @@ class LinearInt4:
         float16); leading dimensions of x are rows.  Runs on torch's current
         stream, or on `stream` (a torch.cuda.Stream)."""
         import torch
-        from .decode import DTYPE_CODES, _check_cuda, _check_tensors, on_stream
-        _check_tensors(x=x, out=out)
-        code = DTYPE_CODES.get(x.dtype)
+        from . import decode
+        if not isinstance(x, torch.Tensor) or out is not None:
+            decode._check_tensors(x=x, out=out)
+        code = decode.DTYPE_CODES.get(x.dtype)
         if code is None:
             raise TypeError(f"LinearInt4::forward: x must be float32, bfloat16 or float16, got {x.dtype}")
-        if x.dim() < 1 or x.shape[-1] != self.in_features:
-            raise ValueError(f"LinearInt4::forward: x {tuple(x.shape)} does not end in in_features {self.in_features}")
-        shape = x.shape[:-1] + (self.out_features,)
-        _check_cuda("x", x, self.device)
-        with on_stream(self.device, stream) as s:
-            if x.dim() != 2:
-                x = x.reshape(-1, self.in_features)
-            rows = x.shape[0]
-            if (self.in_features > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < self.in_features):
-                x = x.contiguous()
-            if out is None:
-                out = torch.empty(shape, dtype=x.dtype, device=self.device)
-                ldy = self.out_features
-            else:
-                _check_cuda("out", out, self.device)
-                if out.shape != shape or out.dtype != x.dtype:
-                    raise ValueError(f"LinearInt4::forward: out must be {x.dtype} {tuple(shape)}")
-                if out.dim() != 2 and not out.is_contiguous():
-                    raise ValueError("LinearInt4::forward: out must be contiguous")
-                ldy = out.stride(0) if out.dim() == 2 and rows > 1 else self.out_features
-                if ldy < self.out_features or (self.out_features > 1 and out.stride(-1) != 1):
-                    raise ValueError("LinearInt4::forward: the rows of out must be contiguous and apart")
-            if rows:
-                ldx = x.stride(0) if rows > 1 else self.in_features
-                rc = self.L.trba_linear_int4_forward(self.h, x.data_ptr(), code, ldx, rows, out.data_ptr(), ldy, s.ptr)
-                if rc:
-                    raise _err(self.L, "LinearInt4::forward")
+        ins, outs, device = self.in_features, self.out_features, self.device
+        if x.dim() < 1 or x.shape[-1] != ins:
+            raise ValueError(f"LinearInt4::forward: x {tuple(x.shape)} does not end in in_features {ins}")
+        shape = x.shape[:-1] + (outs,)
+        if x.device != device:
+            decode._check_cuda("x", x, device)
+        if stream is not None or device.index != decode._current_device():
+            with decode._on(device, stream):
+                return self.forward(x, out)
+        if x.dim() != 2:
+            x = x.reshape(-1, ins)
+        rows = x.shape[0]
+        if not x.is_contiguous() and ((ins > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < ins)):
+            x = x.contiguous()
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=device)
+            ldy = outs
+        else:
+            decode._check_cuda("out", out, device)
+            if out.shape != shape or out.dtype != x.dtype:
+                raise ValueError(f"LinearInt4::forward: out must be {x.dtype} {tuple(shape)}")
+            if out.dim() != 2 and not out.is_contiguous():
+                raise ValueError("LinearInt4::forward: out must be contiguous")
+            ldy = out.stride(0) if out.dim() == 2 and rows > 1 else outs
+            if ldy < outs or (outs > 1 and out.stride(-1) != 1):
+                raise ValueError("LinearInt4::forward: the rows of out must be contiguous and apart")
+        if rows > 1 << 20:
+            raise ValueError("LinearInt4::forward: at most 2**20 rows")
+        if rows:
+            rc = self.L.trba_linear_int4_forward(self.h, x.data_ptr(), code, x.stride(0) if rows > 1 else ins, rows,
+                                                 out.data_ptr(), ldy, decode._raw_stream(device.index))
+            if rc:
+                raise _err(self.L, "LinearInt4::forward")
         return out
 
     def state(self) -> dict:
