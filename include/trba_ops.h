@@ -69,7 +69,8 @@ long long trba_linear_int8_param_count(const trba_linear_int8 *l);
  *
  * A layer keeps its weights on the device that was current when it was
  * created; forward is refused on another one.  forward only launches kernels:
- * it may run on several streams at once and be captured into CUDA graphs. */
+ * it may be captured into CUDA graphs and, each call with a workspace of its
+ * own, run on several streams at once. */
 typedef struct trba_linear_int4 trba_linear_int4;
 /* From f32 weights [out, in] row-major and bias [out] (NULL = zeros), both on
  * the host.  scale = max |w| of the group / 7 (1 when all are zero), code - 8
@@ -88,9 +89,13 @@ trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_feature
 void trba_linear_int4_destroy(trba_linear_int4 *l);
 /* x [rows, in] and y [rows, out] on the device, both of `dtype` (TRBA_F32,
  * TRBA_BF16, TRBA_F16), row strides ldx >= in and ldy >= out in elements; y
- * must not overlap x.  0 (an empty call) to 2^20 rows. */
+ * must not overlap x.  0 (an empty call) to 2^20 rows.  More than a few rows
+ * need a workspace of trba_linear_int4_workspace(...) bytes, aligned to 16 (0
+ * bytes: none, NULL will do), which calls that may overlap must not share;
+ * what it holds before and after does not matter. */
+long long trba_linear_int4_workspace(const trba_linear_int4 *l, int dtype, int rows);
 int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype, long long ldx, int rows, void *y,
-                             long long ldy, void *stream);
+                             long long ldy, void *workspace, long long workspace_bytes, void *stream);
 /* Host copies of the state (any pointer may be NULL): codes [out, (in + 1) /
  * 2] in the order above, scales [out, ceil(in / group)] as f32, bias [out]. */
 int trba_linear_int4_get(const trba_linear_int4 *l, uint8_t *codes, float *scales, float *bias);

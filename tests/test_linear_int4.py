@@ -49,7 +49,8 @@ def test_c_refusals(lib):
     refused(lib.trba_linear_int4_create(4, 4, 32, None, None), b"bad arguments")
     for bad in ((None, 2, p, 0, 1), (p, 1, p, 0, 1), (p, 2, None, 0, 1), (p, 2, p, 1, 1), (p, 2, p, 0, 0)):
         refused(lib.trba_linear_int4_create_codes(4, 4, 32, *bad, None, None), b"bad arguments")
-    refused(lib.trba_linear_int4_forward(None, p, 0, 4, 1, p, 4, None), b"bad arguments")
+    refused(lib.trba_linear_int4_forward(None, p, 0, 4, 1, p, 4, None, 0, None), b"bad arguments")
+    assert lib.trba_linear_int4_workspace(None, 0, 9) == 0
     assert lib.trba_linear_int4_get(None, None, None, None) == -1 and lib.trba_linear_int4_param_count(None) == -1
     lib.trba_linear_int4_destroy(None)
     assert lib.trba_last_error() == 0
@@ -165,7 +166,9 @@ def test_strides_and_leading_dimensions(off, ldx, ldy, dtype, cuda):
     assert torch.equal(lin.forward(x.contiguous()), want)
     assert torch.equal(lin.forward(x.contiguous().view(1, rows, ins))[0], want)
     assert torch.equal(lin.forward(x.T.contiguous().T), want)
-    assert torch.equal(lin.forward(x[4]), want[4]) and lin.forward(x[:0]).shape == (0, outs)
+    one = lin.forward(x[4])  # (the order of a row's sum may depend on the number of rows)
+    assert one.shape == (outs,) and lin.forward(x[:0]).shape == (0, outs)
+    check(one, x[4], q, s, b, ins, 64)
 
 
 @pytest.mark.gpu
@@ -204,10 +207,11 @@ def test_forward_refusals(lib, cuda):
     p = C.c_void_p(x.data_ptr())
     for args, word in (((None, 0, 40, 1, p, 8), b"bad arguments"), ((p, 0, 39, 1, p, 8), b"bad arguments"), ((p, 0, 40, -1, p, 8), b"bad arguments"),
                        ((p, 0, 40, 1, p, 7), b"bad arguments"), ((p, 3, 40, 1, p, 8), b"element type"),
-                       ((C.c_void_p(x.data_ptr() + 2), 0, 40, 1, p, 8), b"not aligned")):
-        assert lib.trba_linear_int4_forward(lin.h, *args, None) == -1 and word in lib.trba_last_error_string()
+                       ((C.c_void_p(x.data_ptr() + 2), 0, 40, 1, p, 8), b"not aligned"), ((p, 0, 40, 9, p, 8), b"workspace")):
+        assert lib.trba_linear_int4_forward(lin.h, *args, None, 0, None) == -1 and word in lib.trba_last_error_string()
         lib.trba_clear_error()
-    assert lib.trba_linear_int4_forward(lin.h, None, 0, 40, 0, None, 8, None) == 0
+    assert lib.trba_linear_int4_forward(lin.h, None, 0, 40, 0, None, 8, None, 0, None) == 0
+    assert lib.trba_linear_int4_workspace(lin.h, 0, 1) == 0 < lib.trba_linear_int4_workspace(lin.h, 0, 9)
     lin.close()
     lin.close()
 

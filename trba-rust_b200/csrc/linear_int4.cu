@@ -6,7 +6,6 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
-#include <cstdlib>
 #include <new>
 
 #include "common.cuh"
@@ -117,44 +116,39 @@ __global__ void __launch_bounds__(256) int4_natural_kernel(const uint8_t *__rest
 }
 
 // ----------------------------------------------------------------- forward --
-constexpr int kPair = 2;  // blocks of a stage
-// One column tile needs few registers: 32 warps hide more latency.  Stages of
-// a warp's ring: 64 KB are in flight a SM either way.
-constexpr int warps_of(int nt) { return nt == 1 ? 32 : 16; }
-constexpr int depth_of(int warps) { return warps == 32 ? 2 : 3; }
+constexpr int kPair = 2;  // blocks of a stage of the few-columns kernel
+// Few columns need few registers: 32 warps hide more latency; two stages of
+// two blocks each keep 64 KB in flight a SM.
+constexpr int kFewWarps = 32, kManyWarps = 16;
+constexpr int many_depth(int nt) { return nt <= 5 ? 4 : 3; }
 
 // y^T = W x^T on the tensor cores: A is a 16-output tile of the weights, the
 // codes turned into exact bf16 or f16 integers in registers, B the
-// activations from shared memory, eight columns at a time.  An f32
-// activation enters as three bf16 columns whose sum it is exactly, so its
-// products with the codes are exact in all types, and a group's sum is
-// accumulated in f32 before its scale multiplies it.
+// activations, eight columns at a time.  An f32 activation enters as three
+// bf16 columns whose sum it is exactly, so its products with the codes are
+// exact in all types, and a group's sum is accumulated in f32 before its
+// scale multiplies it.
 //
 // What bounds it: at few rows, reading the codes (half a byte a weight).  The
 // warp-level mma is enough for that: a 1 KB block of codes costs 8 mma per
-// eight columns and about 90 integer and conversion instructions.
+// eight columns and about 75 integer and conversion instructions.
 //
-// One CTA a SM for the whole product: its tiles are a contiguous share of all
-// of them, its warps are `wn` tiles by `wk` parts of
-// the inputs.  Every warp streams its blocks, over all its tiles, through a
-// ring of cp.async stages of its own, so that loads stay in flight while
-// activations are staged, sums are joined and outputs written.  Activations
-// are staged in slabs of inputs, each once a CTA, all tiles running over one
-// slab before the next; sums wait in shared memory in between.  The order of
-// every sum is fixed.
+// One CTA a SM for the whole product, its tiles a contiguous share of all of
+// them, its warps `wn` tiles side by side by `wk` parts of the inputs.  The
+// order of every sum is fixed.
 struct Args {
     const uint8_t *blocks;
     const float *bias;
     const void *x;
     void *y;
+    uint4 *frags;  // [row block][chunk][word][column tile][lane]
     i64 ldx, ldy;
     int in, out, rows, dtype;
     int tiles, chunks, gpc;
-    int wn;              // wk = W / wn
-    int slab;            // chunks whose activations are staged at once
-    int block_rows;      // rows a CTA takes
-    int packed;          // f32: columns 3 r + p of a single column tile (else p * rows + r)
-    int xs_at, red_at, sums_at;  // shared memory: ring, activations, partial sums, sums between slabs
+    int wn;              // wk = warps / wn
+    int slab;            // few columns: chunks whose activations are staged at once
+    int block_rows;      // many columns: rows a CTA takes
+    int xs_at, red_at, sums_at;  // in shared memory: activations, partial sums, sums between slabs
 };
 
 __device__ __forceinline__ float scale_f32(float v) { return v; }
@@ -295,20 +289,115 @@ __device__ __forceinline__ void store8(const Args &a, const Eight &v, uint8_t *d
         *reinterpret_cast<uint4 *>(dst + p * apart) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
 }
 
-// S: type of the scales; WG: words (32 inputs) a group has in a chunk; NT:
-// tiles of eight columns; W: warps.
-template <bool F16, class S, int WG, int NT, int W>
-__global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_constant__ Args a) {
+// The activations as B fragments: a thread a fragment's 16 bytes (three for f32).
+__global__ void __launch_bounds__(256) int4_fragments_kernel(const __grid_constant__ Args a, int nt) {
+    const int split = a.dtype == TRBA_F32 ? 3 : 1, per = nt / split;  // column tiles of a part
+    const i64 total = (i64)a.chunks * 4 * per * 32;
+    const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
+    uint4 *frags = a.frags + (i64)blockIdx.y * a.chunks * 4 * nt * 32;
+    GRID_LOOP(e, total) {
+        const int lane = (int)(e & 31);
+        const i64 q = e >> 5, cw = q / per;
+        const int n = (int)(q - cw * per), r = n * 8 + (lane >> 2);
+        Eight v;
+        v.lo = v.hi = make_uint4(0, 0, 0, 0);
+        if (r < rows) v = load8(a, row0 + r, (int)cw * 32 + (lane & 3) * 8);
+        store8(a, v, reinterpret_cast<uint8_t *>(frags + (cw * nt + n) * 32 + lane), per * 512);
+    }
+}
+
+// One block: tot += scales * (codes - 8) . activations.  x(w, n): the B
+// fragment of word w and column tile n.  S: type of the scales; WG: words (32
+// inputs) a group has in a chunk; NT: tiles of eight columns.
+template <bool F16, class S, int WG, int NT, class X>
+__device__ __forceinline__ void block_product(const uint8_t *blk, X x, float (&tot)[NT][4], int lane) {
+    const uint4 lo = *reinterpret_cast<const uint4 *>(blk + lane * 16);
+    const uint4 hi = *reinterpret_cast<const uint4 *>(blk + 512 + lane * 16);
+    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+    const S *sp = reinterpret_cast<const S *>(blk + 1024) + (lane >> 2);
+    float c[NT][4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t a0[4], a1[4];
+        code_pairs<F16>(wl[w], a0[0], a0[2], a1[0], a1[2]);
+        code_pairs<F16>(wh[w], a0[1], a0[3], a1[1], a1[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint4 b = x(w, n);
+            mma<F16>(c[n], a0, b.x, b.y, w % WG == 0);
+            mma<F16>(c[n], a1, b.z, b.w, false);
+        }
+        if (w % WG == WG - 1) {
+            const float s0 = scale_f32(sp[(w / WG) * 16]), s1 = scale_f32(sp[(w / WG) * 16 + 8]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                tot[n][0] = fmaf(s0, c[n][0], tot[n][0]);
+                tot[n][1] = fmaf(s0, c[n][1], tot[n][1]);
+                tot[n][2] = fmaf(s1, c[n][2], tot[n][2]);
+                tot[n][3] = fmaf(s1, c[n][3], tot[n][3]);
+            }
+        }
+    }
+}
+
+// Writes a tile's sums: outputs 16 tile + g and + 8 of the rows in this lane's columns.
+template <bool F16, int NT>
+__device__ __forceinline__ void write_tile(const Args &a, int tile, int row0, int rows, const float (&tot)[NT][4],
+                                           int lane) {
+    constexpr float kUnit = F16 ? 1.0f : 4.0f;  // of the code pairs
+    const int g = lane >> 2, t = lane & 3, n0 = tile * 16 + g;
+    auto put = [&](int r, int n, float v) {
+        if (r >= rows || n >= a.out) return;
+        v = fmaf(v, kUnit, a.bias[n]);
+        const i64 at = (row0 + r) * a.ldy + n;
+        if (a.dtype == TRBA_F32) static_cast<float *>(a.y)[at] = v;
+        else if (a.dtype == TRBA_BF16) static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(v);
+        else static_cast<__half *>(a.y)[at] = __float2half_rn(v);
+    };
+    if (a.dtype != TRBA_F32) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8, tot[n][q]);
+    } else if (NT == 1) {  // columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float v[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    v[p] = __shfl_sync(kFull, tot[0][2 * h + ((3 * r + p) & 1)], 4 * g + (3 * r + p) / 2);
+                if (t == r) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
+            }
+    } else if (NT % 3 == 0) {  // the three parts are a third of the column tiles each
+        constexpr int kPer = NT / 3 > 0 ? NT / 3 : 1;
+#pragma unroll
+        for (int n = 0; n < kPer; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8,
+                    tot[n][q] + (tot[(n + kPer) % NT][q] + tot[(n + 2 * kPer) % NT][q]));
+    }
+}
+
+// Up to eight columns: every warp streams its blocks, over all its tiles,
+// through a ring of cp.async stages of its own, so that loads stay in flight
+// while activations are staged, sums are joined and outputs written.
+// Activations are staged in slabs of inputs, each once a CTA, all tiles
+// running over one slab before the next; sums wait in shared memory in between.
+template <bool F16, class S, int WG>
+__global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int W = kFewWarps, NT = 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wk_n = W / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
     const int t0 = (int)((i64)a.tiles * blockIdx.x / gridDim.x) + wn;
     const int t1 = (int)((i64)a.tiles * (blockIdx.x + 1) / gridDim.x);
-    const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
-    const int split = a.dtype == TRBA_F32 ? 3 : 1;
-    constexpr int kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S), kSlot = kPair * kBlock, kDepth = depth_of(W);
+    const int rows = a.rows, split = a.dtype == TRBA_F32 ? 3 : 1;
+    constexpr int kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S), kSlot = kPair * kBlock;
     const int pitch = a.slab * 256 + 64;  // 64 mod 128: eight lanes' 16-byte reads meet 32 different banks
-    const int ring = warp * kDepth * kSlot;  // offsets in shared memory
+    const int ring = warp * 2 * kSlot;    // offsets in shared memory
 
     // the stream of this warp's stages: for each slab, for each of its tiles, its part of the chunks
     int ptile = t0 - a.wn, pslab = t0 < t1 ? 0 : a.chunks, left = 0;
@@ -316,63 +405,38 @@ __global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_co
     const uint32_t ring_s = smem_addr(smem) + ring + lane * 16;
     uint32_t dst = ring_s;
     auto issue = [&]() {
-        if (left <= 0) {
-            while (pslab < a.chunks && left <= 0) {  // the next tile, or the next slab's first
-                ptile += a.wn;
-                if (ptile >= t1) {
-                    ptile = t0;
-                    pslab += a.slab;
-                    if (pslab >= a.chunks) break;
-                }
-                const int sc = min(a.slab, a.chunks - pslab), c = pslab + sc * wk / wk_n;
-                left = pslab + sc * (wk + 1) / wk_n - c;
-                psrc = a.blocks + ((i64)ptile * a.chunks + c) * kBlock + lane * 16;
+        while (left <= 0 && pslab < a.chunks) {  // the next tile, or the next slab's first
+            ptile += a.wn;
+            if (ptile >= t1) {
+                ptile = t0;
+                pslab += a.slab;
+                if (pslab >= a.chunks) break;
             }
+            const int sc = min(a.slab, a.chunks - pslab), c = pslab + sc * wk / wk_n;
+            left = pslab + sc * (wk + 1) / wk_n - c;
+            psrc = a.blocks + ((i64)ptile * a.chunks + c) * kBlock + lane * 16;
         }
         if (left > 0) {
-            if (left > 1) {
+            const int bytes = left > 1 ? kSlot : kBlock;
 #pragma unroll
-                for (int j = 0; j < (kSlot + 511) / 512; ++j)
-                    if (512 * (j + 1) <= kSlot || lane * 16 < kSlot - 512 * j) cp16(dst + 512 * j, psrc + 512 * j);
-            } else {
-#pragma unroll
-                for (int j = 0; j < (kBlock + 511) / 512; ++j)
-                    if (512 * (j + 1) <= kBlock || lane * 16 < kBlock - 512 * j) cp16(dst + 512 * j, psrc + 512 * j);
-            }
+            for (int j = 0; j < (kSlot + 511) / 512; ++j)
+                if (lane * 16 < bytes - 512 * j) cp16(dst + 512 * j, psrc + 512 * j);
             psrc += kSlot;
             left -= kPair;
-            if (kDepth == 2) {
-                dst = 2 * ring_s + kSlot - dst;
-            } else {
-                dst += kSlot;
-                if (dst == ring_s + kDepth * kSlot) dst = ring_s;
-            }
+            dst = 2 * ring_s + kSlot - dst;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int i = 0; i < kDepth - 1; ++i) issue();
+    issue();
 
-    const int g = lane >> 2, t = lane & 3;
     // a column of mma depends on its own activations alone: lanes behind the
     // last column read it again
-    int xcol[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        int col = n * 8 + g;
-        if (split == 1 || a.packed) {
-            col = min(col, rows * split - 1);
-        } else {
-            constexpr int kPer = (NT + 2) / 3;
-            col = (n / kPer) * rows + min((n % kPer) * 8 + g, rows - 1);
-        }
-        xcol[n] = a.xs_at + col * pitch + t * 16;
-    }
-    int blk = ring;
-    int turn = 0;  // partial-sum buffers are used in turn
+    const int xcol = a.xs_at + min(lane >> 2, rows * split - 1) * pitch + (lane & 3) * 16;
+    int blk = ring, turn = 0;  // partial-sum buffers are used in turn
     for (int s0 = 0; s0 < a.chunks; s0 += a.slab) {
         const int sc = min(a.slab, a.chunks - s0), n8 = sc * 16;
         if (s0) __syncthreads();
-        constexpr int kLoads = W == 32 ? 2 : 4;  // in flight a thread
+        constexpr int kLoads = 2;  // in flight a thread
         for (int e0 = threadIdx.x; e0 < rows * n8; e0 += kLoads * W * 32) {
             Eight v[kLoads];
             int r[kLoads], k[kLoads];
@@ -380,130 +444,151 @@ __global__ void __launch_bounds__(W * 32, 1) int4_forward_kernel(const __grid_co
             for (int u = 0; u < kLoads; ++u) {
                 const int e = e0 + u * W * 32;
                 r[u] = e / n8, k[u] = e - r[u] * n8;
-                if (r[u] < rows) v[u] = load8(a, row0 + r[u], s0 * 128 + k[u] * 8);
+                if (r[u] < rows) v[u] = load8(a, r[u], s0 * 128 + k[u] * 8);
             }
 #pragma unroll
             for (int u = 0; u < kLoads; ++u)
-                if (r[u] < rows)
-                    store8(a, v[u], smem + a.xs_at + (a.packed ? 3 * r[u] : r[u]) * pitch + k[u] * 16,
-                           a.packed ? pitch : rows * pitch);
+                if (r[u] < rows) store8(a, v[u], smem + a.xs_at + split * r[u] * pitch + k[u] * 16, pitch);
         }
         __syncthreads();
         const int cb = sc * wk / wk_n, ce = sc * (wk + 1) / wk_n;
         for (int u = t0; u < t1; u += a.wn, turn ^= 1) {
-            float tot[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
+            float tot[NT][4] = {};
             for (int xo = cb * 256; xo < ce * 256; xo += kPair * 256) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
                 __syncwarp();
                 issue();
 #pragma unroll
                 for (int p = 0; p < kPair; ++p) {
                     if (p && xo + 256 * p >= ce * 256) break;
-                    const uint8_t *bp = smem + blk + p * kBlock;
-                    const uint4 lo = *reinterpret_cast<const uint4 *>(bp + lane * 16);
-                    const uint4 hi = *reinterpret_cast<const uint4 *>(bp + 512 + lane * 16);
-                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-                    const S *sp = reinterpret_cast<const S *>(bp + 1024) + g;
-                    float c[NT][4];
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t a0[4], a1[4];
-                        code_pairs<F16>(wl[w], a0[0], a0[2], a1[0], a1[2]);
-                        code_pairs<F16>(wh[w], a0[1], a0[3], a1[1], a1[3]);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint4 b = *reinterpret_cast<const uint4 *>(smem + xcol[n] + xo + p * 256 + w * 64);
-                            mma<F16>(c[n], a0, b.x, b.y, w % WG == 0);
-                            mma<F16>(c[n], a1, b.z, b.w, false);
-                        }
-                        if (w % WG == WG - 1) {
-                            const float s0f = scale_f32(sp[(w / WG) * 16]), s1f = scale_f32(sp[(w / WG) * 16 + 8]);
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                tot[n][0] = fmaf(s0f, c[n][0], tot[n][0]);
-                                tot[n][1] = fmaf(s0f, c[n][1], tot[n][1]);
-                                tot[n][2] = fmaf(s1f, c[n][2], tot[n][2]);
-                                tot[n][3] = fmaf(s1f, c[n][3], tot[n][3]);
-                            }
-                        }
-                    }
+                    block_product<F16, S, WG, NT>(
+                        smem + blk + p * kBlock,
+                        [&](int w, int) { return *reinterpret_cast<const uint4 *>(smem + xcol + xo + p * 256 + w * 64); },
+                        tot, lane);
                 }
-                if (kDepth == 2) {
-                    blk = 2 * ring + kSlot - blk;
-                } else {
-                    blk += kSlot;
-                    if (blk == ring + kDepth * kSlot) blk = ring;
-                }
+                blk = 2 * ring + kSlot - blk;
             }
             // join the wk_n warps of the tile; two buffers in turn, so that a
             // buffer is written again only after the next tile's barrier
             if (wk_n > 1) {
-                float4 *red = reinterpret_cast<float4 *>(smem + a.red_at) +
-                              ((turn * a.wn + wn) * (wk_n - 1)) * NT * 32 + lane;
-                if (wk > 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        red[((wk - 1) * NT + n) * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
-                }
+                float4 *red = reinterpret_cast<float4 *>(smem + a.red_at) + ((turn * a.wn + wn) * (wk_n - 1)) * 32 + lane;
+                if (wk > 0) red[(wk - 1) * 32] = make_float4(tot[0][0], tot[0][1], tot[0][2], tot[0][3]);
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + wn), "r"(wk_n * 32) : "memory");
                 if (wk > 0) continue;
-                for (int k = 0; k < wk_n - 1; ++k)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float4 v = red[(k * NT + n) * 32];
-                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
-                    }
+                for (int k = 0; k < wk_n - 1; ++k) {
+                    const float4 v = red[k * 32];
+                    tot[0][0] += v.x, tot[0][1] += v.y, tot[0][2] += v.z, tot[0][3] += v.w;
+                }
             }
             if (a.slab < a.chunks) {
-                float4 *sums = reinterpret_cast<float4 *>(smem + a.sums_at) + (u - (t0 - wn)) * NT * 32 + lane;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (s0) {
-                        const float4 v = sums[n * 32];
-                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
-                    }
-                    if (s0 + sc < a.chunks) sums[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
+                float4 *sums = reinterpret_cast<float4 *>(smem + a.sums_at) + (u - (t0 - wn)) * 32 + lane;
+                if (s0) {
+                    const float4 v = *sums;
+                    tot[0][0] += v.x, tot[0][1] += v.y, tot[0][2] += v.z, tot[0][3] += v.w;
                 }
-                if (s0 + sc < a.chunks) continue;
+                if (s0 + sc < a.chunks) {
+                    *sums = make_float4(tot[0][0], tot[0][1], tot[0][2], tot[0][3]);
+                    continue;
+                }
             }
-            // outputs 16 u + g and + 8 of the rows in this lane's columns
-            const int n0 = u * 16 + g;
-            constexpr float kUnit = F16 ? 1.0f : 4.0f;
-            auto put = [&](int r, int n, float v) {
-                if (r >= rows || n >= a.out) return;
-                v = fmaf(v, kUnit, a.bias[n]);
-                const i64 at = (row0 + r) * a.ldy + n;
-                if (a.dtype == TRBA_F32) static_cast<float *>(a.y)[at] = v;
-                else if (a.dtype == TRBA_BF16) static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(v);
-                else static_cast<__half *>(a.y)[at] = __float2half_rn(v);
-            };
-            if (split == 1) {
+            write_tile<F16, NT>(a, u, 0, rows, tot, lane);
+        }
+    }
+}
+
+// More columns: the CTA moves in steps of a block a warp, `wn` tiles side by
+// side and wk chunks deep, through stages that hold the step's B fragments
+// (read by all warps) and each warp's block.  Staging the activations as
+// fragments in memory first makes their copies plain and aligned; per SM and
+// step they are read once for wn tiles.  From about 24 columns on the tensor
+// pipe bounds it (a 16 x 8 x 16 mma takes 2.4 cycles a SM).
+template <bool F16, class S, int WG, int NT>
+__global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __grid_constant__ Args a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int D = many_depth(NT), kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wk_n = kManyWarps / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
+    const int groups = (a.tiles + a.wn - 1) / a.wn;
+    const int g0 = (int)((i64)groups * blockIdx.x / gridDim.x), g1 = (int)((i64)groups * (blockIdx.x + 1) / gridDim.x);
+    const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
+    const int xbytes = wk_n * NT * 2048, stage = xbytes + kManyWarps * kBlock;
+    const uint8_t *frags = reinterpret_cast<const uint8_t *>(a.frags) + (i64)blockIdx.y * a.chunks * NT * 2048;
+    const uint32_t smem_s = smem_addr(smem);
+    float4 *red = reinterpret_cast<float4 *>(smem + a.red_at);
+
+    int pg = g0, pc = 0, ps = 0;  // the next stage to fill: its group, first chunk, place
+    auto weights = [&](uint32_t to) {
+        const int tile = pg * a.wn + wn, c = pc + wk;
+        if (pg < g1 && tile < a.tiles && c < a.chunks) {
+            const uint8_t *src = a.blocks + ((i64)tile * a.chunks + c) * kBlock + lane * 16;
+            const uint32_t dst = to + xbytes + warp * kBlock + lane * 16;
+            cp16(dst, src);
+            cp16(dst + 512, src + 512);
+            if (lane * 16 < kBlock - 1024) cp16(dst + 1024, src + 1024);
+        }
+    };
+    auto activations = [&](uint32_t to) {
+        if (pg < g1) {
+            const int bytes = min(wk_n, a.chunks - pc) * NT * 2048;
+            const uint8_t *src = frags + (i64)pc * NT * 2048;
+            for (int o = threadIdx.x * 16; o < bytes; o += kManyWarps * 32 * 16) cp16(to + o, src + o);
+        }
+    };
+    auto next = [&]() {
+        pc += wk_n;
+        if (pc >= a.chunks) {
+            pc = 0;
+            ++pg;
+        }
+        ps = ps + 1 == D ? 0 : ps + 1;
+    };
+    // the first weights are on their way while the fragments are made
+    weights(smem_s);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = 0; i < D - 1; ++i) {
+        if (i) weights(smem_s + ps * stage);
+        activations(smem_s + ps * stage);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next();
+    }
+    int cs = 0;
+    for (int g = g0; g < g1; ++g) {
+        const int tile = g * a.wn + wn;
+        float tot[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
+        for (int c0 = 0; c0 < a.chunks; c0 += wk_n) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+            __syncthreads();  // the stage is there for all, and the last one is free
+            weights(smem_s + ps * stage);
+            activations(smem_s + ps * stage);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            next();
+            if (tile < a.tiles && c0 + wk < a.chunks) {
+                const uint8_t *st = smem + cs * stage, *xs = st + wk * NT * 2048 + lane * 16;
+                block_product<F16, S, WG, NT>(
+                    st + xbytes + warp * kBlock,
+                    [&](int w, int n) { return *reinterpret_cast<const uint4 *>(xs + (w * NT + n) * 512); }, tot, lane);
+            }
+            cs = cs + 1 == D ? 0 : cs + 1;
+        }
+        if (wk_n > 1) {  // join the warps of a tile; the next group's first barrier keeps `red` until it was read
+            if (wk > 0) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8, tot[n][q]);
-            } else if (NT == 1) {  // packed: columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float v[3];
-#pragma unroll
-                        for (int p = 0; p < 3; ++p)
-                            v[p] = __shfl_sync(kFull, tot[0][2 * h + ((3 * r + p) & 1)], 4 * g + (3 * r + p) / 2);
-                        if (t == r) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
-                    }
-            } else if (NT % 3 == 0) {
-#pragma unroll
-                for (int n = 0; n < NT / 3; ++n)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8,
-                            tot[n][q] + (tot[n + NT / 3][q] + tot[n + 2 * (NT / 3)][q]));
+                    red[((wn * (wk_n - 1) + wk - 1) * NT + n) * 32 + lane] =
+                        make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
             }
+            __syncthreads();
+            if (wk > 0) continue;
+            for (int k = 0; k < wk_n - 1; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float4 v = red[((wn * (wk_n - 1) + k) * NT + n) * 32 + lane];
+                    tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
+                }
         }
+        if (tile < a.tiles) write_tile<F16, NT>(a, tile, row0, rows, tot, lane);
     }
 }
 
@@ -515,12 +600,12 @@ int launched() {
 }
 
 constexpr int kMaxSmem = 227 * 1024;
-constexpr int kMaxJoin = 48 * 1024;  // shared memory of the warps' partial sums
 
-template <bool F16, class S, int WG, int NT>
-int launch(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
-    auto fn = int4_forward_kernel<F16, S, WG, NT, warps_of(NT)>;
-    static std::atomic<unsigned long long> sized{0};  // one bit a device: its limit has been raised
+// Raises the kernel's shared-memory limit (once a device) and launches it;
+// `overlap`: as soon as the kernel before it ends, its own wait taking care
+// of the rest.
+int launch(void (*fn)(const Args), std::atomic<unsigned long long> &sized, const Args &a, dim3 grid, int warps,
+           size_t smem, bool overlap, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     const unsigned long long bit = 1ull << (dev & 63);
@@ -533,20 +618,41 @@ int launch(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
         }
         sized.fetch_or(bit, std::memory_order_relaxed);
     }
-    fn<<<grid, warps_of(NT) * 32, smem, st>>>(a);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, fn, a);
     return launched();
+}
+
+template <bool F16, class S, int WG>
+int launch_few(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
+    static std::atomic<unsigned long long> sized{0};
+    return launch(int4_few_kernel<F16, S, WG>, sized, a, grid, kFewWarps, smem, false, st);
+}
+template <bool F16, class S, int WG, int NT>
+int launch_many(const Args &a, dim3 grid, size_t smem, cudaStream_t st) {
+    static std::atomic<unsigned long long> sized{0};
+    return launch(int4_many_kernel<F16, S, WG, NT>, sized, a, grid, kManyWarps, smem, true, st);
 }
 
 template <bool F16, class S, int WG>
 int launch_nt(const Args &a, int nt, dim3 grid, size_t smem, cudaStream_t st) {
     switch (nt) {
-        case 1: return launch<F16, S, WG, 1>(a, grid, smem, st);
-        case 2: return launch<F16, S, WG, 2>(a, grid, smem, st);
-        case 3: return launch<F16, S, WG, 3>(a, grid, smem, st);
-        case 4: return launch<F16, S, WG, 4>(a, grid, smem, st);
-        case 5: return launch<F16, S, WG, 5>(a, grid, smem, st);
-        case 6: return launch<F16, S, WG, 6>(a, grid, smem, st);
-        default: return launch<F16, S, WG, 8>(a, grid, smem, st);
+        case 1: return launch_few<F16, S, WG>(a, grid, smem, st);
+        case 2: return launch_many<F16, S, WG, 2>(a, grid, smem, st);
+        case 3: return launch_many<F16, S, WG, 3>(a, grid, smem, st);
+        case 4: return launch_many<F16, S, WG, 4>(a, grid, smem, st);
+        case 5: return launch_many<F16, S, WG, 5>(a, grid, smem, st);
+        case 6: return launch_many<F16, S, WG, 6>(a, grid, smem, st);
+        default: return launch_many<F16, S, WG, 8>(a, grid, smem, st);
     }
 }
 
@@ -562,58 +668,84 @@ int launch_type(const Args &a, bool scale_f16, int wg, int nt, dim3 grid, size_t
     return launch_nt<F16, float, 4>(a, nt, grid, smem, st);
 }
 
-int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int rows, void *y, i64 ldy, cudaStream_t st) {
+// How the rows are shared out: up to 64 columns a row block, an f32 row being
+// three (one or two rows pack them into one column tile, 16 rows make six).
+struct Shape {
+    int blocks, block_rows, nt;
+    Shape(int rows, int dtype) {
+        const bool f32 = dtype == TRBA_F32;
+        const int most = f32 ? 16 : 64;
+        blocks = (rows + most - 1) / most;
+        block_rows = (rows + blocks - 1) / blocks;
+        nt = f32 ? (block_rows <= 2 ? 1 : block_rows <= 8 ? 3 : 6) : (block_rows + 7) / 8;
+        if (nt == 7) nt = 8;
+    }
+    i64 workspace(int chunks) const { return nt > 1 ? (i64)blocks * chunks * 4 * nt * 512 : 0; }
+};
+
+int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int rows, void *y, i64 ldy, void *workspace,
+            cudaStream_t st) {
+    const Shape shape(rows, dtype);
     Args a{};
     a.blocks = l->base, a.bias = l->bias;
     a.x = x, a.y = y, a.ldx = ldx, a.ldy = ldy;
+    a.frags = static_cast<uint4 *>(workspace);
     a.in = l->in, a.out = l->out, a.rows = rows, a.dtype = dtype;
     a.tiles = l->tiles, a.chunks = l->chunks, a.gpc = l->gpc;
     const bool scale_f16 = l->scale_dtype == TRBA_F16;
-    // rows of a CTA: up to 64 columns, an f32 row being three (16 rows make six tiles of them)
-    const bool f32 = dtype == TRBA_F32;
-    const int most = f32 ? 16 : 64, blocks_y = (rows + most - 1) / most;
-    a.block_rows = (rows + blocks_y - 1) / blocks_y;
-    a.packed = f32 && a.block_rows <= 2;
-    int nt = f32 ? (a.packed ? 1 : a.block_rows <= 8 ? 3 : 6) : (a.block_rows + 7) / 8;
-    if (nt == 7) nt = 8;
-    const int cols = a.block_rows * (f32 ? 3 : 1);
+    const int nt = shape.nt, blocks_y = shape.blocks;
+    a.block_rows = shape.block_rows;
     i64 smem = 0;
-    const int frag = nt * 512;  // bytes of one tile's sums
-    const int warps = warps_of(nt), ring = warps * depth_of(warps) * kPair * l->block;
-    const auto x_bytes = [&](int chunks) { return ((i64)cols * (chunks * 256 + 64) + 127) & ~127ll; };
-    int ctas = a.tiles < sm_count() ? a.tiles : sm_count();
-    for (;; ctas = ctas * 2 < a.tiles ? ctas * 2 : a.tiles) {
-        const int share = (a.tiles + ctas - 1) / ctas;  // tiles of a CTA, at most
-        // Tiles of a CTA that run side by side: the fewest steps of (chunks a
-        // warp streams + the join of the warps that share a tile).
-        long long best = -1;
-        int red = 0;
-        for (int wn = warps; wn >= 1; wn >>= 1) {
-            if (wn == 16 && warps > 16) continue;  // named barriers 1 + wn go up to 15
-            const int wk = warps / wn, bytes = 2 * wn * (wk - 1) * frag;
-            const long long steps = (share + wn - 1) / wn;
-            const long long cost = steps * (4 * ((a.chunks + wk - 1) / wk) + (wk > 1 ? 4 + wk : 0));
-            if (bytes <= kMaxJoin && (best < 0 || cost < best)) best = cost, a.wn = wn, red = bytes;
+    int ctas = 0;
+    if (nt > 1) {
+        int4_fragments_kernel<<<dim3(grid_for((i64)l->chunks * 4 * nt * 32), blocks_y), 256, 0, st>>>(a, nt);
+        if (const int e = launched()) return e;
+        // Tiles side by side: the fewest steps of the CTA with the most.
+        i64 best = -1;
+        for (int wn = kManyWarps; wn >= 1; wn >>= 1) {
+            const int wk = kManyWarps / wn, red = wn * (wk - 1) * nt * 512;
+            const i64 stages = (i64)many_depth(nt) * (wk * nt * 2048 + kManyWarps * l->block);
+            if (stages + red > kMaxSmem) break;
+            const int groups = (a.tiles + wn - 1) / wn, grid = groups < sm_count() ? groups : sm_count();
+            const i64 cost = (i64)((groups + grid - 1) / grid) * ((a.chunks + wk - 1) / wk + 1);
+            if (best < 0 || cost < best) best = cost, a.wn = wn, ctas = grid, a.red_at = (int)stages, smem = stages + red;
         }
-        if (const char *e = getenv("TUNE_WN")) a.wn = atoi(e), red = 2 * a.wn * (warps / a.wn - 1) * frag;
-        // All activations at once where they fit; else as many chunks as fit
-        // beside the sums that wait between slabs.  Sums that leave no room
-        // for a slab of a few chunks go to more CTAs.
-        const i64 room = kMaxSmem - ring - red;
-        i64 sums = 0;
-        a.slab = a.chunks;
-        if (x_bytes(a.chunks) > room) {
-            sums = (i64)share * frag;
-            a.slab = (int)(((room - sums - 128) / cols - 64) / 256);
-            if (a.slab < 4 && ctas < a.tiles) continue;
+    } else {
+        const int cols = rows * (dtype == TRBA_F32 ? 3 : 1);
+        const int ring = kFewWarps * 2 * kPair * l->block;
+        const auto x_bytes = [&](int chunks) { return ((i64)cols * (chunks * 256 + 64) + 127) & ~127ll; };
+        for (ctas = a.tiles < sm_count() ? a.tiles : sm_count();; ctas = ctas * 2 < a.tiles ? ctas * 2 : a.tiles) {
+            const int share = (a.tiles + ctas - 1) / ctas;  // tiles of a CTA, at most
+            // Tiles of a CTA that run side by side: the fewest steps of (chunks a
+            // warp streams + the join of the warps that share a tile).
+            i64 best = -1;
+            int red = 0;
+            for (int wn = kFewWarps; wn >= 1; wn >>= 1) {
+                if (wn == 16) continue;  // named barriers 1 + wn go up to 15
+                const int wk = kFewWarps / wn, bytes = 2 * wn * (wk - 1) * 512;
+                const i64 steps = (share + wn - 1) / wn;
+                const i64 cost = steps * (4 * ((a.chunks + wk - 1) / wk) + (wk > 1 ? 4 + wk : 0));
+                if (best < 0 || cost < best) best = cost, a.wn = wn, red = bytes;
+            }
+            // All activations at once where they fit; else as many chunks as fit
+            // beside the sums that wait between slabs.  Sums that leave no room
+            // for a slab of a few chunks go to more CTAs.
+            const i64 room = kMaxSmem - ring - red;
+            i64 sums = 0;
+            a.slab = a.chunks;
+            if (x_bytes(a.chunks) > room) {
+                sums = (i64)share * 512;
+                a.slab = (int)(((room - sums - 128) / cols - 64) / 256);
+                if (a.slab < 4 && ctas < a.tiles) continue;
+            }
+            a.xs_at = ring;
+            a.red_at = a.xs_at + (int)x_bytes(a.slab);
+            a.sums_at = a.red_at + red;
+            smem = a.sums_at + sums;
+            break;
         }
-        if (const char *e = getenv("TUNE_SLAB")) a.slab = atoi(e), sums = (i64)share * frag;
-        a.xs_at = ring;
-        a.red_at = a.xs_at + (int)x_bytes(a.slab);
-        a.sums_at = a.red_at + red;
-        smem = a.sums_at + sums;
-        break;
     }
+    TRBA_REQUIRE_RET(smem > 0 && smem <= kMaxSmem, "trba_linear_int4_forward: shared memory", -1);
     const int wg = l->group >= 128 ? 4 : l->group / 32;
     const dim3 grid(ctas, blocks_y);
     return dtype == TRBA_F16 ? launch_type<true>(a, scale_f16, wg, nt, grid, smem, st)
@@ -719,8 +851,12 @@ void trba_linear_int4_destroy(trba_linear_int4 *l) {
     delete l;
 }
 
+long long trba_linear_int4_workspace(const trba_linear_int4 *l, int dtype, int rows) {
+    return l && rows > 0 ? Shape(rows, dtype).workspace(l->chunks) : 0;
+}
+
 int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype, long long ldx, int rows, void *y,
-                             long long ldy, void *stream) {
+                             long long ldy, void *workspace, long long workspace_bytes, void *stream) {
     TRBA_REQUIRE_RET(l && rows >= 0 && rows <= (1 << 20), "trba_linear_int4_forward: bad arguments", -1);
     if (rows == 0) return 0;
     TRBA_REQUIRE_RET(x && y && ldx >= l->in && ldy >= l->out, "trba_linear_int4_forward: bad arguments", -1);
@@ -732,7 +868,10 @@ int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype
     int dev = -1;
     cudaGetDevice(&dev);
     TRBA_REQUIRE_RET(dev == l->device, "trba_linear_int4_forward: the layer is on another device", -1);
-    return forward(l, x, dtype, ldx, rows, y, ldy, as_stream(stream));
+    const long long need = trba_linear_int4_workspace(l, dtype, rows);
+    TRBA_REQUIRE_RET(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                     "trba_linear_int4_forward: workspace missing, too small or not aligned to 16 bytes", -1);
+    return forward(l, x, dtype, ldx, rows, y, ldy, workspace, as_stream(stream));
 }
 
 int trba_linear_int4_get(const trba_linear_int4 *l, uint8_t *codes, float *scales, float *bias) {

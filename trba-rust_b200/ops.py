@@ -225,8 +225,11 @@ class LinearInt4:
         if rows > 1 << 20:
             raise ValueError("LinearInt4::forward: at most 2**20 rows")
         if rows:
+            need = self.L.trba_linear_int4_workspace(self.h, code, rows) if rows > 2 else 0
+            work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             rc = self.L.trba_linear_int4_forward(self.h, x.data_ptr(), code, x.stride(0) if rows > 1 else ins, rows,
-                                                 out.data_ptr(), ldy, decode._raw_stream(device.index))
+                                                 out.data_ptr(), ldy, work.data_ptr() if need else None, need,
+                                                 decode._raw_stream(device.index))
             if rc:
                 raise _err(self.L, "LinearInt4::forward")
         return out
