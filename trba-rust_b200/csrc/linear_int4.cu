@@ -2,6 +2,7 @@
 // decoding step (include/trba_ops.h, LinearInt4).  No counterpart in the
 // reference; the quantisation rule is LinearInt8's (src/linear.rs:53-59) for
 // 4 bits and groups.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -35,6 +36,8 @@ struct trba_linear_int4 {
 
 namespace trba {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -146,6 +149,7 @@ struct Args {
     int in, out, rows, dtype;
     int tiles, chunks, gpc;
     int wn;              // wk = warps / wn
+    int cs;              // many columns: CTAs that share a tile's chunks
     int slab;            // few columns: chunks whose activations are staged at once
     int block_rows;      // many columns: rows a CTA takes
     int xs_at, red_at, sums_at;  // in shared memory: activations, partial sums, sums between slabs
@@ -509,17 +513,19 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wk_n = kManyWarps / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
     const int groups = (a.tiles + a.wn - 1) / a.wn;
-    const int g0 = (int)((i64)groups * blockIdx.x / gridDim.x), g1 = (int)((i64)groups * (blockIdx.x + 1) / gridDim.x);
+    const int rank = blockIdx.x % a.cs, bx = blockIdx.x / a.cs, gx = gridDim.x / a.cs;
+    const int g0 = (int)((i64)groups * bx / gx), g1 = (int)((i64)groups * (bx + 1) / gx);
+    const int cb = a.chunks * rank / a.cs, ce = a.chunks * (rank + 1) / a.cs;  // this CTA's chunks
     const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
     const int xbytes = wk_n * NT * 2048, stage = xbytes + kManyWarps * kBlock;
     const uint8_t *frags = reinterpret_cast<const uint8_t *>(a.frags) + (i64)blockIdx.y * a.chunks * NT * 2048;
     const uint32_t smem_s = smem_addr(smem);
     float4 *red = reinterpret_cast<float4 *>(smem + a.red_at);
 
-    int pg = g0, pc = 0, ps = 0;  // the next stage to fill: its group, first chunk, place
+    int pg = g0, pc = cb, ps = 0;  // the next stage to fill: its group, first chunk, place
     auto weights = [&](uint32_t to) {
         const int tile = pg * a.wn + wn, c = pc + wk;
-        if (pg < g1 && tile < a.tiles && c < a.chunks) {
+        if (pg < g1 && tile < a.tiles && c < ce) {
             const uint8_t *src = a.blocks + ((i64)tile * a.chunks + c) * kBlock + lane * 16;
             const uint32_t dst = to + xbytes + warp * kBlock + lane * 16;
             cp16(dst, src);
@@ -529,15 +535,15 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
     };
     auto activations = [&](uint32_t to) {
         if (pg < g1) {
-            const int bytes = min(wk_n, a.chunks - pc) * NT * 2048;
+            const int bytes = min(wk_n, ce - pc) * NT * 2048;
             const uint8_t *src = frags + (i64)pc * NT * 2048;
             for (int o = threadIdx.x * 16; o < bytes; o += kManyWarps * 32 * 16) cp16(to + o, src + o);
         }
     };
     auto next = [&]() {
         pc += wk_n;
-        if (pc >= a.chunks) {
-            pc = 0;
+        if (pc >= ce) {
+            pc = cb;
             ++pg;
         }
         ps = ps + 1 == D ? 0 : ps + 1;
@@ -557,14 +563,14 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
         float tot[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
-        for (int c0 = 0; c0 < a.chunks; c0 += wk_n) {
+        for (int c0 = cb; c0 < ce; c0 += wk_n) {
             asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
             __syncthreads();  // the stage is there for all, and the last one is free
             weights(smem_s + ps * stage);
             activations(smem_s + ps * stage);
             asm volatile("cp.async.commit_group;" ::: "memory");
             next();
-            if (tile < a.tiles && c0 + wk < a.chunks) {
+            if (tile < a.tiles && c0 + wk < ce) {
                 const uint8_t *st = smem + cs * stage, *xs = st + wk * NT * 2048 + lane * 16;
                 block_product<F16, S, WG, NT>(
                     st + xbytes + warp * kBlock,
@@ -572,7 +578,8 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
             }
             cs = cs + 1 == D ? 0 : cs + 1;
         }
-        if (wk_n > 1) {  // join the warps of a tile; the next group's first barrier keeps `red` until it was read
+        // join the warps of a tile; the next group's first barrier keeps `red` until it was read
+        if (wk_n > 1) {
             if (wk > 0) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -580,14 +587,37 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
                         make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
             }
             __syncthreads();
-            if (wk > 0) continue;
-            for (int k = 0; k < wk_n - 1; ++k)
+            if (wk == 0) {
+                for (int k = 0; k < wk_n - 1; ++k)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float4 v = red[((wn * (wk_n - 1) + k) * NT + n) * 32 + lane];
-                    tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
-                }
+                    for (int n = 0; n < NT; ++n) {
+                        const float4 v = red[((wn * (wk_n - 1) + k) * NT + n) * 32 + lane];
+                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
+                    }
+            }
         }
+        if (a.cs > 1) {  // one group a CTA: the stages are done with and hold the sums
+            __syncthreads();
+            float4 *part = reinterpret_cast<float4 *>(smem) + wn * NT * 32 + lane;
+            if (rank > 0 && wk == 0) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) part[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
+            }
+            cg::this_cluster().sync();
+            if (rank == 0 && wk == 0) {
+                for (int k = 1; k < a.cs; ++k) {
+                    const float4 *other = cg::this_cluster().map_shared_rank(part, k);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float4 v = other[n * 32];
+                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
+                    }
+                }
+            }
+            cg::this_cluster().sync();  // no CTA leaves while its sums are read
+            if (rank > 0) return;
+        }
+        if (wk > 0) continue;
         if (tile < a.tiles) write_tile<F16, NT>(a, tile, row0, rows, tot, lane);
     }
 }
@@ -618,16 +648,18 @@ int launch(void (*fn)(const Args), std::atomic<unsigned long long> &sized, const
         }
         sized.fetch_or(bit, std::memory_order_relaxed);
     }
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cs, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = overlap ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = !overlap ? 0 : a.cs > 1 ? 2 : 1;
     cudaLaunchKernelEx(&cfg, fn, a);
     return launched();
 }
@@ -687,6 +719,7 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
             cudaStream_t st) {
     const Shape shape(rows, dtype);
     Args a{};
+    a.cs = 1;
     a.blocks = l->base, a.bias = l->bias;
     a.x = x, a.y = y, a.ldx = ldx, a.ldy = ldy;
     a.frags = static_cast<uint4 *>(workspace);
@@ -707,8 +740,12 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
             const i64 stages = (i64)many_depth(nt) * (wk * nt * 2048 + kManyWarps * l->block);
             if (stages + red > kMaxSmem) break;
             const int groups = (a.tiles + wn - 1) / wn, grid = groups < sm_count() ? groups : sm_count();
-            const i64 cost = (i64)((groups + grid - 1) / grid) * ((a.chunks + wk - 1) / wk + 1);
-            if (best < 0 || cost < best) best = cost, a.wn = wn, ctas = grid, a.red_at = (int)stages, smem = stages + red;
+            int cs = 1;  // (then every CTA has one group)
+            while (cs < 8 && 2 * cs * groups <= sm_count() && 2 * cs * wk <= a.chunks) cs *= 2;
+            const i64 each = (a.chunks + cs - 1) / cs;
+            const i64 cost = (i64)((groups + grid - 1) / grid) * ((each + wk - 1) / wk + 1) + (cs > 1 ? 2 : 0);
+            if (best < 0 || cost < best)
+                best = cost, a.wn = wn, a.cs = cs, ctas = grid * cs, a.red_at = (int)stages, smem = stages + red;
         }
     } else {
         const int cols = rows * (dtype == TRBA_F32 ? 3 : 1);
