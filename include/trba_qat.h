@@ -95,6 +95,21 @@ int trba_model_infer(trba_model *m, const int8_t *img, int batch, int32_t *step_
  * followed by -1, lengths (host, [batch]) their counts.  Synchronises. */
 int trba_model_infer_host(trba_model *m, const int8_t *img, int batch, int32_t *tokens, int32_t *lengths,
                           void *stream);
+/* Beam search instead of the greedy decoder (no counterpart in the
+ * reference): the same encoder and decoder step, the `beams` (1 .. 32) best
+ * continuations of a line kept at every step by trba_beam_select
+ * (trba_decode.h).  Unlike the greedy path, a line's beam that produced eos is
+ * finished on its own.  sequences (device, [batch, beams, max_len+1] int32):
+ * tokens before eos, then pad, best beam first; lengths (device, [batch,
+ * beams]); scores (device, [batch, beams] f32 log probabilities, or NULL); a
+ * slot that holds no sequence has score -inf.  The model keeps the search's
+ * buffers; the first call that needs more than any before allocates (and
+ * waits), so make it before a capture. */
+int trba_model_infer_beam(trba_model *m, const int8_t *img, int batch, int beams, int32_t *sequences,
+                          int32_t *lengths, float *scores, void *stream);
+/* The same with host buffers.  Synchronises. */
+int trba_model_infer_beam_host(trba_model *m, const int8_t *img, int batch, int beams, int32_t *sequences,
+                               int32_t *lengths, float *scores, void *stream);
 /* Clip (first clip_warmup steps), Muon/Adam, re-quantise. */
 int trba_model_optimizer_step(trba_model *m, void *stream);
 /* forward_backward, gradient all-reduce (when data-parallel), optimizer_step. */

@@ -861,6 +861,42 @@ class OracleTrba:
                 break
         return out, step_tok
 
+    def decode_logits(self, enc, b, t, prefixes):
+        """Generator logits [len(prefixes), V] after each (line, token list):
+        the decoder of greedy_decode fed with sos and those tokens."""
+        cfg = self.cfg
+        H, P = cfg.hidden, self.p
+        bh = enc.reshape(b, t, H)
+        proj_h = dot64(bh.reshape(b * t, H), P["attn.i2h.w"].T).reshape(b, t, H)
+        line = np.array([p[0] for p in prefixes])
+        bh, proj_h, n = bh[line], proj_h[line], len(prefixes)
+        h, cc = np.zeros((n, H), F32), np.zeros((n, H), F32)
+        scw = P["attn.score.w"].reshape(H)
+        wc, wtok = P["attn.w_ih"][:, :H], P["attn.w_ih"][:, H:]
+        bsum = (P["attn.b_ih"] + P["attn.b_hh"]).astype(F32)
+        toks = np.array([[cfg.sos] + list(p[1]) for p in prefixes], np.int64)
+        for st in range(toks.shape[1]):
+            phh = linear_fwd(h, P["attn.h2h.w"], P["attn.h2h.b"])
+            e = dot64(tanh32(proj_h + phh[:, None, :]), scw)
+            ex = exp32(e - e.max(axis=1, keepdims=True))
+            alpha = (ex / sum64(ex, axis=1)[:, None]).astype(F32)
+            ctx = np.einsum("bt,btk->bk", alpha.astype(F64), bh.astype(F64)).astype(F32)
+            pre = (((bsum + dot64(ctx, wc.T)) + wtok[:, toks[:, st]].T) + dot64(h, P["attn.w_hh"].T)).astype(F32)
+            ig, fg = sigmoid(pre[:, :H]), sigmoid(pre[:, H:2 * H])
+            cg, og = tanh32(pre[:, 2 * H:3 * H]), sigmoid(pre[:, 3 * H:])
+            cc = (fg * cc + ig * cg).astype(F32)
+            h = (og * tanh32(cc)).astype(F32)
+        return linear_fwd(h, P["attn.gen.w"], P["attn.gen.b"])
+
+    def encode(self, img):
+        """The BiLSTM stack's output [b * t, hidden] of run_inference, and t."""
+        b = img.shape[0]
+        feat, ctr = self.cnn_fwd(np.ascontiguousarray(img.reshape(-1)), b, train=False)
+        x = feat
+        for li in range(self.cfg.rnn_layers):
+            x, _ = self.bilstm_layer_fwd(li, x, b, ctr["wf"])
+        return x, ctr["wf"]
+
     def infer(self, img):
         """run_inference (later snapshot src/main.rs:2690): the CNN with BN
         running statistics, the BiLSTM stack, greedy attention decoding."""

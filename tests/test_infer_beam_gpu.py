@@ -1,0 +1,107 @@
+"""Beam search over the recogniser's own decoder (trba_model_infer_beam):
+against a search by the oracle that carries every beam's token list along and
+recomputes its logits from the start at every step; and, with one beam, against
+greedy decoding."""
+import sys
+
+import numpy as np
+import pytest
+
+from conftest import REPO
+from test_infer_gpu import _pair
+
+sys.path.insert(0, str(REPO / "oracle"))
+import decode_oracle as do  # noqa: E402
+import step_oracle as so  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def search(orc, cfg, img, K):
+    """[line][beam] = (tokens before eos, f64 score), best first."""
+    b = img.shape[0]
+    enc, t = orc.encode(img)
+    paths = [[[] for _ in range(K)] for _ in range(b)]
+    scores = np.full((b, K), -np.inf)
+    scores[:, 0] = 0
+    fin = np.zeros((b, K), bool)
+    for _ in range(cfg.steps):
+        logits = orc.decode_logits(enc, b, t, [(i, p) for i in range(b) for p in paths[i]])
+        # the device rounds the running score to f32 at every step
+        s, tok, par, fin = do.beam_select(logits, scores.astype(np.float32), fin, cfg.eos)
+        scores = s.astype(np.float32).astype(np.float64)
+        paths = [[paths[i][par[i, k]] + [int(tok[i, k])] for k in range(K)] for i in range(b)]
+    cut = [[p[:p.index(cfg.eos)] if cfg.eos in p else p for p in line] for line in paths]
+    return cut, scores
+
+
+@pytest.mark.parametrize("K", [1, 3, 8])
+@pytest.mark.parametrize("geom,B,steps", [(dict(img_w=64, max_len=4), 8, 3), (dict(img_w=96, max_len=9), 3, 2)],
+                         ids=["32x64_b8", "32x96_b3"])
+def test_beam_search_matches_oracle(geom, B, steps, K, lib, cuda):
+    import torch
+    ocfg, orc, gm = _pair(geom, B, seed=78, train_steps=steps)
+    img, *_ = so.make_batch(ocfg, B, seed=1235)
+    want, want_s = search(orc, ocfg, img, K)
+    dev = torch.from_numpy(np.ascontiguousarray(img)).cuda()
+    seq, lengths, scores = (x.cpu().numpy() for x in gm.infer_beam(dev, K))
+    # a step's score is off by at most 2^-19 and half an f32 step (see the
+    # selection's tests), so a path's by that times its steps; a beam whose
+    # oracle score is nearer than that to another's may change places with it
+    tol = ocfg.steps * (2.0 ** -19 + 2.0 ** -24 * np.abs(want_s).max())
+    assert np.abs(scores - want_s).max() <= tol
+    for i in range(B):
+        apart = np.diff(want_s[i]) < -2 * tol
+        clear = np.concatenate([[True], apart]) & np.concatenate([apart, [False]])
+        for k in range(K):
+            n = lengths[i, k]
+            assert (seq[i, k, n:] == ocfg.pad).all()
+            got = seq[i, k, :n].tolist()
+            if clear[k]:
+                assert got == want[i][k]
+            elif k + 1 < K:
+                assert got in want[i]
+    host = gm.infer_beam_host(img, K)
+    assert [[t for t, _ in line] for line in host] == [[seq[i, k, :lengths[i, k]].tolist() for k in range(K)] for i in range(B)]
+    assert np.array_equal(np.array([[s for _, s in line] for line in host], np.float32), scores)
+    other, *_ = so.make_batch(ocfg, B, seed=4)
+    gm.infer_beam_host(other[:2], K + 1)  # an unrelated call in between, smaller and larger, leaves no trace
+    again = gm.infer_beam(dev, K)
+    assert np.array_equal(again[0].cpu().numpy(), seq) and np.array_equal(again[2].cpu().numpy(), scores)
+    assert lib.trba_last_error() == 0, lib.trba_last_error_string()
+
+
+def test_one_beam_is_greedy_until_eos(lib, cuda):
+    import torch
+    ocfg, _, gm = _pair(dict(img_w=160, max_len=20), 4, seed=77, train_steps=2)
+    img, *_ = so.make_batch(ocfg, 4, seed=1234)
+    dev = torch.from_numpy(np.ascontiguousarray(img)).cuda()
+    greedy = gm.infer(dev)
+    seq, lengths, _ = (x.cpu().numpy() for x in gm.infer_beam(dev, 1))
+    for i in range(4):
+        g = greedy[:, i].tolist()
+        g = g[:g.index(ocfg.eos)] if ocfg.eos in g else g
+        assert seq[i, 0, :lengths[i, 0]].tolist() == g
+    assert np.array_equal(gm.infer(dev), greedy)  # the greedy path is as it was
+
+
+def test_expert_runner_decodes_with_beams(lib, cuda):
+    """Serving: the best beam of every line, whatever the decoding batch."""
+    import torch
+    import trba_b200.mope as mp
+    run = mp.ExpertRunner(mp.default_experts()[1], batch=5, seed=11)
+    ocfg = so.Config(img_w=96, max_len=5)
+    img, *_ = so.make_batch(ocfg, 12, seed=31)
+    dev = torch.from_numpy(np.ascontiguousarray(img)).cuda()
+    lists = run.decode_beam(dev, 4)
+    assert len(lists) == 12
+    whole = [run.model.infer_beam(dev[s:s + 5], 4) for s in range(0, 12, 5)]
+    for s, (seq, lengths, scores) in zip(range(0, 12, 5), whole):
+        assert (scores[:, :-1] >= scores[:, 1:]).all()
+        for i in range(seq.shape[0]):
+            assert lists[s + i] == seq[i, 0, :lengths[i, 0]].tolist()
+    with pytest.raises(ValueError, match="beams"):
+        run.model.infer_beam(dev[:1], 33)
+    with pytest.raises(RuntimeError, match="infer_beam"):
+        run.model.infer_beam(dev, 2)  # more lines than the model was made for
+    run.close()

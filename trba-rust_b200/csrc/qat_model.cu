@@ -25,6 +25,7 @@
 #include "qat_kernels.cuh"
 #include "seq_kernels.cuh"
 #include "trba_backend.h"
+#include "trba_decode.h"
 #include "trba_qat.h"
 
 using namespace trba;
@@ -267,6 +268,8 @@ struct trba_model {
     int gkey_batch = 0, gkey_probe = -1;
     long long graph_kernels = 0;  // kernel launches recorded in the step graph
     Probe probe;
+    uint8_t *beam_mem = nullptr;  // buffers of the beam search, grown when a call needs more
+    size_t beam_bytes = 0;
 };
 
 namespace {
@@ -1265,8 +1268,8 @@ void head_forward(Ctx &c, const int32_t *text_in, const int32_t *target, const i
 }
 
 // Inference head (run_inference, later snapshot src/main.rs:2690): the
-// BiLSTM stack as in training, then greedy attention decoding.
-void head_infer(Ctx &c, int32_t *step_tokens) {
+// BiLSTM stack as in training; gives what the attention decoder works on.
+seq::AttnFwd head_encode(Ctx &c) {
     trba_model *m = c.m;
     const auto &cf = m->cfg;
     const int B = c.B, T = m->T, H = cf.hidden, V = cf.classes, S = m->steps;
@@ -1293,8 +1296,83 @@ void head_infer(Ctx &c, int32_t *step_tokens) {
     a.gen_b = c.P + entry_off(m, "attn.gen.b");
     a.sos = cf.sos;
     a.B = B, a.T = T, a.H = H, a.V = V, a.steps = S;
+    return a;
+}
+
+// Greedy attention decoding.
+void head_infer(Ctx &c, int32_t *step_tokens) {
+    seq::AttnFwd a = head_encode(c);
     a.step_tokens = step_tokens;
     seq::attn_decode(a, c.st);
+}
+
+// Beam search starts with one live beam a line.
+__global__ void beam_start_kernel(float *scores, uint8_t *finished, int n, int beams) {
+    GRID_LOOP(i, n) {
+        scores[i] = i % beams == 0 ? 0.0f : -INFINITY;
+        finished[i] = 0;
+    }
+}
+
+// What a beam search of `rows` beams keeps on the device, in one allocation.
+struct BeamBuffers {
+    size_t used = 0;
+    float *h[2], *c[2], *logits, *scores;
+    int32_t *tokens, *parents, *sequences, *lengths;
+    uint8_t *finished;
+    void *work;
+    long long work_bytes;
+    BeamBuffers(uint8_t *base, const trba_model *m, int lines, int beams) {
+        const i64 rows = (i64)lines * beams, H = m->cfg.hidden, V = m->cfg.classes, S = m->steps;
+        const auto take = [&](i64 bytes) {
+            uint8_t *p = base + used;
+            used += (size_t)((bytes + 255) & ~255ll);
+            return p;
+        };
+        const auto f = [&](i64 n) { return reinterpret_cast<float *>(take(n * 4)); };
+        const auto i = [&](i64 n) { return reinterpret_cast<int32_t *>(take(n * 4)); };
+        for (int k = 0; k < 2; ++k) h[k] = f(rows * H), c[k] = f(rows * H);
+        logits = f(rows * V), scores = f(rows);
+        tokens = i(S * rows), parents = i(S * rows), sequences = i(S * rows), lengths = i(rows);
+        finished = take(rows);
+        work_bytes = trba_beam_select_workspace(TRBA_F32, lines, beams, (int)V);
+        work = take(work_bytes);
+    }
+};
+
+// Beam search over the attention decoder.
+int head_infer_beam(Ctx &c, const BeamBuffers &bb, int beams, int32_t *sequences, int32_t *lengths, float *scores) {
+    trba_model *m = c.m;
+    const auto &cf = m->cfg;
+    const int B = c.B, H = cf.hidden, V = cf.classes, S = m->steps, rows = B * beams;
+    seq::AttnFwd a = head_encode(c);
+    a.B = rows, a.beams = beams, a.steps = 1;
+    a.logits = bb.logits;
+    a.h_out = bb.h[1], a.c_out = bb.c[1];
+    beam_start_kernel<<<grid_for(rows), 256, 0, c.st>>>(bb.scores, bb.finished, rows, beams);
+    TRBA_LAUNCH_CHECK();
+    for (int s = 0; s < S; ++s) {
+        seq::attn_step(a, c.st);
+        int32_t *tok = bb.tokens + (i64)s * rows, *par = bb.parents + (i64)s * rows;
+        int rc = trba_beam_select(bb.logits, TRBA_F32, V, bb.scores, bb.finished, B, beams, V, cf.eos, bb.scores, tok, par,
+                                  bb.finished, bb.work, bb.work_bytes, c.st);
+        if (rc) return rc;
+        if (s + 1 == S) break;
+        trba_beam_state st[2]{};
+        for (int k = 0; k < 2; ++k) {
+            st[k].src = k ? bb.c[1] : bb.h[1];
+            st[k].dst = k ? bb.c[0] : bb.h[0];
+            st[k].bytes = st[k].src_row = st[k].dst_row = (long long)H * 4;
+            st[k].mid = st[k].outer = 1;
+        }
+        rc = trba_beam_reorder(st, 2, par, B, beams, c.st);
+        if (rc) return rc;
+        a.h_in = bb.h[0], a.c_in = bb.c[0];
+        a.tok_in = tok;
+    }
+    if (scores)
+        TRBA_CHECK(cudaMemcpyAsync(scores, bb.scores, (size_t)rows * 4, cudaMemcpyDeviceToDevice, c.st));
+    return trba_beam_sequences(bb.tokens, bb.parents, S, B, beams, cf.eos, cf.pad, sequences, lengths, c.st);
 }
 
 void head_backward(Ctx &c) {
@@ -1554,6 +1632,7 @@ void trba_model_destroy(trba_model *m) {
     if (m->gstream) cudaStreamDestroy(m->gstream);
     for (cudaEvent_t e : m->probe.ev) cudaEventDestroy(e);
     if (m->probe.stamps) cudaFree(m->probe.stamps);
+    cudaFree(m->beam_mem);
     delete m;
 }
 
@@ -1672,6 +1751,61 @@ int trba_model_infer(trba_model *m, const int8_t *img, int batch, int32_t *step_
     cnn_forward(c, img);
     head_infer(c, step_tokens ? step_tokens : m->step_tokens.get());
     return cuda_status();
+}
+
+int trba_model_infer_beam(trba_model *m, const int8_t *img, int batch, int beams, int32_t *sequences,
+                          int32_t *lengths, float *scores, void *stream) {
+    if (!m || !img || !sequences || !lengths || batch <= 0 || batch > m->B || beams <= 0 || beams > TRBA_MAX_BEAMS)
+        return -1;
+    if (m->cfg.eos < 0 || m->cfg.eos >= m->cfg.classes) return -1;
+    cudaStream_t st = as_stream(stream);
+    const size_t need = BeamBuffers(nullptr, m, batch, beams).used;
+    if (need > m->beam_bytes) {
+        cudaFree(m->beam_mem);  // waits for what still uses it
+        m->beam_mem = nullptr;
+        m->beam_bytes = 0;
+        const cudaError_t e = cudaMalloc(&m->beam_mem, need);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            report_error(__FILE__, __LINE__, "trba_model_infer_beam: device allocation failed", (int)e);
+            return (int)e;
+        }
+        m->beam_bytes = need;
+    }
+    Ctx c{m, st, batch, m->P.get(), m->G.get()};
+    c.eval = true;
+    m->last_B = batch;
+    TRBA_CHECK(cudaMemsetAsync(m->zarena.base, 0, m->zarena.used, st));
+    cnn_forward(c, img);
+    const int rc = head_infer_beam(c, BeamBuffers(m->beam_mem, m, batch, beams), beams, sequences, lengths, scores);
+    return rc ? rc : cuda_status();
+}
+
+int trba_model_infer_beam_host(trba_model *m, const int8_t *img, int batch, int beams, int32_t *sequences,
+                               int32_t *lengths, float *scores, void *stream) {
+    if (!m || !img || !sequences || !lengths || batch <= 0 || batch > m->B || beams <= 0 || beams > TRBA_MAX_BEAMS)
+        return -1;
+    cudaStream_t st = as_stream(stream);
+    const size_t rows = (size_t)batch * beams, n = rows * m->steps;
+    int32_t *dev = nullptr;  // sequences, lengths, scores
+    TRBA_CHECK(cudaMemcpyAsync(m->in_img.get(), img, (size_t)batch * 3 * m->cfg.img_h * m->cfg.img_w,
+                               cudaMemcpyHostToDevice, st));
+    const cudaError_t e = cudaMallocAsync(reinterpret_cast<void **>(&dev), (n + 2 * rows) * 4, st);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        report_error(__FILE__, __LINE__, "trba_model_infer_beam_host: device allocation failed", (int)e);
+        return (int)e;
+    }
+    int rc = trba_model_infer_beam(m, m->in_img.get(), batch, beams, dev, dev + n,
+                                   reinterpret_cast<float *>(dev + n + rows), stream);
+    if (rc == 0) {
+        TRBA_CHECK(cudaMemcpyAsync(sequences, dev, n * 4, cudaMemcpyDeviceToHost, st));
+        TRBA_CHECK(cudaMemcpyAsync(lengths, dev + n, rows * 4, cudaMemcpyDeviceToHost, st));
+        if (scores) TRBA_CHECK(cudaMemcpyAsync(scores, dev + n + rows, rows * 4, cudaMemcpyDeviceToHost, st));
+    }
+    TRBA_CHECK(cudaFreeAsync(dev, st));
+    TRBA_CHECK(cudaStreamSynchronize(st));
+    return rc ? rc : cuda_status();
 }
 
 int trba_model_infer_host(trba_model *m, const int8_t *img, int batch, int32_t *tokens, int32_t *lengths,

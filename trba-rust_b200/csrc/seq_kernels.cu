@@ -402,11 +402,12 @@ __device__ __forceinline__ double dot2_d(const float *x, const float *w, int str
 // f32 -> f64 conversion runs on the SM's narrow conversion pipe, which bounds
 // these kernels), and a thread that owns one weight column serves every
 // sample of the CTA with one conversion per weight.
-// DECODE = false: teacher-forced forward of the training step (tokens from
-// text_in, every trace stored).  DECODE = true: greedy decoding
-// (src/attn.rs:368-447): the token fed at step s is the argmax (first
-// maximum) of the generator logits of step s-1, sos at step 0; only the
-// per-step argmax tokens are stored.
+// kTrain: teacher-forced forward of the training step (tokens from text_in,
+// every trace stored).  kGreedy: greedy decoding (src/attn.rs:368-447): the
+// token fed at step s is the argmax (first maximum) of the generator logits
+// of step s-1, sos at step 0; only the per-step argmax tokens are stored.
+// kStep: one decoding step of every (line, beam), the same arithmetic as a
+// greedy step: states and tokens in, states and generator logits out.
 // stage bit 0: the CTA's encoder projections [S][T][H] are copied into
 // shared memory once (read at every step); bit 1: the encoder features too.
 constexpr int kAttnRows = 4;  // (sample, t) rows whose warp reductions overlap
@@ -417,8 +418,13 @@ __host__ __device__ inline size_t attn_fwd_smem_base(int H, int T, int V, bool d
            sizeof(float) * ((size_t)9 * H * H + 16 + 4 * S * H + S * G4 + 2 * S * T + S + (decode ? S * V : 0));
 }
 
-template <bool DECODE>
+enum AttnMode { kTrain, kGreedy, kStep };
+
+template <AttnMode MODE>
 __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int stage) {
+    constexpr bool TRAIN = MODE == kTrain, DECODE = MODE == kGreedy, STEP = MODE == kStep;
+    // row of the encoder that sample b looks at
+    const auto enc = [&](int b) { return STEP ? min(b, a.B - 1) / a.beams : min(b, a.B - 1); };
     extern __shared__ __align__(16) double attn_smd[];
     const int H = a.H, T = a.T, V = a.V, G4 = 4 * H, CV = H + V;
     constexpr int S = kAttnS;
@@ -451,16 +457,27 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
     }
     for (int i = threadIdx.x; i < S * T * H; i += blockDim.x) {
         const int sl = i / (T * H), r = i - sl * T * H;
-        const i64 g = (i64)min(b0 + sl, a.B - 1) * T * H + r;
+        const i64 g = (i64)enc(b0 + sl) * T * H + r;
         if (stage & 1) sph[i] = a.proj_h[g];
         if (stage & 2) sbh[i] = a.bh[g];
     }
     for (int i = threadIdx.x; i < S * H; i += blockDim.x) {
         h[i] = c[i] = 0.0f;
         hd[i] = 0.0;
+        if (STEP && a.h_in) {
+            const int sl = i / H, k = i - sl * H;
+            const i64 at = (i64)min(b0 + sl, a.B - 1) * H + k;
+            h[i] = a.h_in[at];
+            c[i] = a.c_in[at];
+        }
+    }
+    if (STEP && a.h_in) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < S * H; i += blockDim.x) hd[i % H * S + i / H] = (double)h[i];
     }
     for (int k = threadIdx.x; k < H; k += blockDim.x) swd[k] = (double)a.score_w[k];
-    if (DECODE && threadIdx.x < S) tok[threadIdx.x] = a.sos;
+    if (!TRAIN && threadIdx.x < S)
+        tok[threadIdx.x] = STEP && a.tok_in ? a.tok_in[min(b0 + (int)threadIdx.x, a.B - 1)] : a.sos;
     __syncthreads();
     for (int st = 0; st < a.steps; ++st) {
         // proj_hh = h2h(h) + bias
@@ -475,7 +492,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
             if (j < H) a0 = fma(hd[j * S + sl], (double)h2hT[j * H + k], a0);
             phh[i] = fadd((float)(a0 + a1), a.h2h_b[k]);
         }
-        if (!DECODE && threadIdx.x < S) {
+        if (TRAIN && threadIdx.x < S) {
             const int b = min(b0 + (int)threadIdx.x, a.B - 1);
             tok[threadIdx.x] = a.text_in[(i64)b * a.steps + st];
         }
@@ -490,10 +507,10 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
                 const int p = p0 + u * nwarps;
                 if (p < S * T) {
                     const int sl = p / T, t = p - sl * T, b = b0 + sl;
-                    const float *php = (stage & 1) ? sph + p * H : a.proj_h + ((i64)min(b, a.B - 1) * T + t) * H;
+                    const float *php = (stage & 1) ? sph + p * H : a.proj_h + ((i64)enc(b) * T + t) * H;
                     for (int k = lane; k < H; k += 32) {
                         const float v = cr_tanhf(fadd(php[k], phh[sl * H + k]));
-                        if (!DECODE && b < a.B) a.tanh_tr[(((i64)st * a.B + b) * T + t) * H + k] = v;
+                        if (TRAIN && b < a.B) a.tanh_tr[(((i64)st * a.B + b) * T + t) * H + k] = v;
                         acc[u] = fma((double)v, swd[k], acc[u]);
                     }
                 }
@@ -526,14 +543,14 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
                 const float v = fdiv(al[sl * T + t], sf);
                 al[sl * T + t] = v;
                 ald[sl * T + t] = (double)v;
-                if (!DECODE && b < a.B) a.alpha[((i64)st * a.B + b) * T + t] = v;
+                if (TRAIN && b < a.B) a.alpha[((i64)st * a.B + b) * T + t] = v;
             }
         }
         __syncthreads();
         // context and the decoder cell input [ctx, one-hot token]
         for (int i = threadIdx.x; i < S * H; i += blockDim.x) {
             const int sl = i / H, k = i - sl * H;
-            const int b = min(b0 + sl, a.B - 1);
+            const int b = enc(b0 + sl);
             const float *bp = (stage & 2) ? sbh + sl * T * H + k : a.bh + (i64)b * T * H + k;
             double acc = 0.0;
             for (int t = 0; t < T; ++t) acc = fma(ald[sl * T + t], (double)bp[t * H], acc);
@@ -542,7 +559,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
             ctxd[k * S + sl] = (double)cv;
         }
         __syncthreads();
-        if (!DECODE) {
+        if (TRAIN) {
             for (int i = threadIdx.x; i < S * CV; i += blockDim.x) {
                 const int sl = i / CV, j = i - sl * CV, b = b0 + sl;
                 if (b < a.B)
@@ -599,7 +616,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
             const float ig = sigm(pg[k]), fg = sigm(pg[H + k]), cg = cr_tanhf(pg[2 * H + k]), og = sigm(pg[3 * H + k]);
             const float cn = fadd(fmul(fg, c[i]), fmul(ig, cg));
             const float hn = fmul(og, cr_tanhf(cn));
-            if (!DECODE && b < a.B) {
+            if (TRAIN && b < a.B) {
                 const i64 sb = (i64)st * a.B + b;
                 a.gates[sb * G4 + k] = ig;
                 a.gates[sb * G4 + H + k] = fg;
@@ -611,8 +628,20 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_kernel(AttnFwd a, int s
             c[i] = cn;
             h[i] = hn;
             hd[k * S + sl] = (double)hn;
+            if (STEP && b < a.B) {
+                a.h_out[(i64)b * H + k] = hn;
+                a.c_out[(i64)b * H + k] = cn;
+            }
         }
         __syncthreads();
+        if (STEP) {
+            for (int i = threadIdx.x; i < S * V; i += blockDim.x) {
+                const int sl = i / V, v = i - sl * V;
+                if (b0 + sl < a.B)
+                    a.logits[(i64)(b0 + sl) * V + v] =
+                        fadd((float)dot2_d(h + sl * H, a.gen_w + (i64)v * H, 1, H), a.gen_b[v]);
+            }
+        }
         if (DECODE) {
             // generator logits = gen_w h + gen_b (the training path's GEMM
             // expression: f64 dot rounded once, then the bias)
@@ -1098,8 +1127,8 @@ void attn_fwd(const AttnFwd &a, cudaStream_t st) {
     size_t total = 0;
     const int stage = attn_fwd_stage(attn_fwd_smem_base(H, T, a.V, false), sizeof(float) * (size_t)S * T * H, &total);
     TRBA_REQUIRE(total <= kAttnMaxSmem, "attn_fwd: hidden / encoder length too large for shared memory");
-    set_smem((const void *)attn_fwd_kernel<false>, total);
-    attn_fwd_kernel<false><<<(a.B + S - 1) / S, kAttnThreads, total, st>>>(a, stage);
+    set_smem((const void *)attn_fwd_kernel<kTrain>, total);
+    attn_fwd_kernel<kTrain><<<(a.B + S - 1) / S, kAttnThreads, total, st>>>(a, stage);
     TRBA_LAUNCH_CHECK();
 }
 
@@ -1109,8 +1138,19 @@ void attn_decode(const AttnFwd &a, cudaStream_t st) {
     size_t total = 0;
     const int stage = attn_fwd_stage(attn_fwd_smem_base(H, T, a.V, true), sizeof(float) * (size_t)S * T * H, &total);
     TRBA_REQUIRE(total <= kAttnMaxSmem, "attn_decode: hidden / encoder length too large for shared memory");
-    set_smem((const void *)attn_fwd_kernel<true>, total);
-    attn_fwd_kernel<true><<<(a.B + S - 1) / S, kAttnThreads, total, st>>>(a, stage);
+    set_smem((const void *)attn_fwd_kernel<kGreedy>, total);
+    attn_fwd_kernel<kGreedy><<<(a.B + S - 1) / S, kAttnThreads, total, st>>>(a, stage);
+    TRBA_LAUNCH_CHECK();
+}
+
+void attn_step(const AttnFwd &a, cudaStream_t st) {
+    const int H = a.H, T = a.T, S = kAttnS;
+    TRBA_REQUIRE(H % 4 == 0, "attn_step: hidden size must be a multiple of 4 (gate rows fill whole warps)");
+    size_t total = 0;
+    const int stage = attn_fwd_stage(attn_fwd_smem_base(H, T, a.V, false), sizeof(float) * (size_t)S * T * H, &total);
+    TRBA_REQUIRE(total <= kAttnMaxSmem, "attn_step: hidden / encoder length too large for shared memory");
+    set_smem((const void *)attn_fwd_kernel<kStep>, total);
+    attn_fwd_kernel<kStep><<<(a.B + S - 1) / S, kAttnThreads, total, st>>>(a, stage);
     TRBA_LAUNCH_CHECK();
 }
 

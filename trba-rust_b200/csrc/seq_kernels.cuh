@@ -66,11 +66,21 @@ struct AttnFwd {
     const float *gen_w = nullptr, *gen_b = nullptr;  // [V, H], [V]
     int sos = 1;
     int32_t *step_tokens = nullptr;  // [steps, B]: argmax token of every step
+    // a single step (attn_step): B = lines * beams rows, bh and proj_h of the
+    // lines; null h_in / c_in are zeros, null tok_in is sos
+    int beams = 1;
+    const float *h_in = nullptr, *c_in = nullptr;  // [B, H]
+    const int32_t *tok_in = nullptr;               // [B]
+    float *h_out = nullptr, *c_out = nullptr;      // [B, H]
+    float *logits = nullptr;                       // [B, V]
 };
 void attn_fwd(const AttnFwd &a, cudaStream_t st);
 // Greedy decoding (src/attn.rs:368-447) over every step; the caller applies
 // the reference's stop rule (all samples at eos) to step_tokens.
 void attn_decode(const AttnFwd &a, cudaStream_t st);
+// One step of every (line, beam), for beam search: states and tokens in,
+// states and generator logits out; the arithmetic of a greedy step.
+void attn_step(const AttnFwd &a, cudaStream_t st);
 
 // Backward (src/attn.rs:263-500): d_out_hid [steps, B, H]; writes dgates
 // [steps, B, 4H], de [steps, B, T], dprojhh [steps, B, H], d_proj_h [B, T, H]

@@ -194,6 +194,41 @@ class QatModel:
         self._check(self.L.trba_model_infer_host(self.h, _ptr(img), b, _ptr(tok), _ptr(lens), stream), "infer_host")
         return [tok[i, :lens[i]].tolist() for i in range(b)]
 
+    def _check_beams(self, beams):
+        if not 1 <= beams <= 32:
+            raise ValueError(f"1 to 32 beams are supported, got {beams}")
+
+    def infer_beam(self, img, beams: int, stream=None):
+        """Beam search over device images [B, 3, H, W] int8: (sequences [B,
+        beams, max_len+1] int32 with pad behind each one's end, lengths [B,
+        beams], scores [B, beams] float32) as device tensors, best beam first.
+        Runs on torch's current stream unless a stream handle is given; the
+        caller then orders its use of the results after that stream."""
+        import torch
+        self._check_beams(beams)
+        if stream is None:
+            stream = torch.cuda.current_stream(img.device).cuda_stream
+        b = int(img.shape[0])
+        seq = torch.empty((b, beams, self.cfg.steps), dtype=torch.int32, device=img.device)
+        lengths = torch.empty((b, beams), dtype=torch.int32, device=img.device)
+        scores = torch.empty((b, beams), dtype=torch.float32, device=img.device)
+        self._check(self.L.trba_model_infer_beam(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lengths), _ptr(scores),
+                                                 stream), "infer_beam")
+        return seq, lengths, scores
+
+    def infer_beam_host(self, img, beams: int, stream=None) -> list:
+        """Beam search over host images: for every line a list of (tokens,
+        score), best first, without the slots that hold no sequence."""
+        self._check_beams(beams)
+        img = np.ascontiguousarray(img, np.int8)
+        b = int(img.shape[0])
+        seq = np.empty((b, beams, self.cfg.steps), np.int32)
+        lens, scores = np.empty((b, beams), np.int32), np.empty((b, beams), np.float32)
+        self._check(self.L.trba_model_infer_beam_host(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lens), _ptr(scores),
+                                                      stream), "infer_beam_host")
+        return [[(seq[i, k, :lens[i, k]].tolist(), float(scores[i, k])) for k in range(beams)
+                 if scores[i, k] > -np.inf] for i in range(b)]
+
     def loss(self) -> np.ndarray:
         """[total, attention CE, CTC] of the last step (synchronises)."""
         out = np.zeros(3, np.float32)

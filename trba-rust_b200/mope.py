@@ -117,6 +117,18 @@ class ExpertRunner:
             out.extend(decode_rule(st, self.cfg.eos))
         return out
 
+    def decode_beam(self, imgs, beams: int, stream=None) -> list[list[int]]:
+        """Token lists of device images, the best of `beams` beams of each line
+        (which do not depend on the decoding batch, unlike the greedy rule's)."""
+        out = []
+        for s in range(0, imgs.shape[0], self.batch):
+            seq, lengths, _ = self.model.infer_beam(imgs[s:s + self.batch], beams, stream=stream)
+            if stream is not None:
+                self.model.L.cuda_sync(stream)
+            seq, lengths = seq[:, 0].cpu().numpy(), lengths[:, 0].cpu().numpy()
+            out.extend(seq[i, :n].tolist() for i, n in enumerate(lengths))
+        return out
+
     def close(self):
         self.model.close()
 
