@@ -72,7 +72,7 @@ long long trba_linear_int8_param_count(const trba_linear_int8 *l);
  * it may be captured into CUDA graphs and, each call with a workspace of its
  * own, run on several streams at once. */
 typedef struct trba_linear_int4 trba_linear_int4;
-/* From f32 weights [out, in] row-major and bias [out] (NULL = zeros), both on
+/* in and out are 1 .. 2^30.  From f32 weights [out, in] row-major and bias [out] (NULL = zeros), both on
  * the host.  scale = max |w| of the group / 7 (1 when all are zero), code - 8
  * = round(w / scale), halves away from zero (the rule of
  * LinearInt8::quantize, src/linear.rs:53-59, for 4 bits and groups). */
@@ -89,7 +89,7 @@ trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_feature
 void trba_linear_int4_destroy(trba_linear_int4 *l);
 /* x [rows, in] and y [rows, out] on the device, both of `dtype` (TRBA_F32,
  * TRBA_BF16, TRBA_F16), row strides ldx >= in and ldy >= out in elements; y
- * must not overlap x.  0 (an empty call) to 2^20 rows.  More than a few rows
+ * must not overlap x.  0 (an empty call) to 1000000 rows.  More than a few rows
  * need a workspace of trba_linear_int4_workspace(...) bytes, aligned to 16 (0
  * bytes: none, NULL will do), which calls that may overlap must not share;
  * what it holds before and after does not matter. */

@@ -225,11 +225,12 @@ def test_select_sorted_rows(order, dtype, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [515, 9001, 70000])
 @pytest.mark.parametrize("dtype", list(DTYPES))
-def test_select_special_values(dtype, cuda):
+def test_select_special_values(dtype, V, cuda):
     t = DTYPES[dtype]
     low = torch.finfo(t).min
-    V, K = 515, 4
+    K = 4
     g = torch.Generator().manual_seed(3)
     x = (torch.randn(8 * K, V, generator=g) * 2).to(t)
     v = x.view(8, K, V)
@@ -264,6 +265,21 @@ def test_select_strides_and_offsets(off, ld, dtype, cuda):
     view.copy_(x)
     check_step(decode.beam_select(view, s, f, eos=2), x, s, f, 2)
     check_step(decode.beam_select(view.unflatten(0, (L, K)), s.T.contiguous().T, f, eos=2), x, s, f, 2)
+    one = view[::K][:, None]  # one beam a line, every K-th row
+    check_step(decode.beam_select(one, s[:, :1], f[:, :1], eos=2), x[::K], s[:, :1], f[:, :1], 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_select_long_rows_at_odd_addresses(dtype, cuda):
+    """Rows of many segments whose starts miss 16-byte boundaries in every way."""
+    L, K, V = 2, 4, 20011
+    buf = torch.full((L * K * (V + 2) + 16,), 60000.0, device="cuda").to(DTYPES[dtype])
+    for off in range(8):
+        x, s, f = make(L, K, V, dtype, off)
+        view = buf[off:off + L * K * (V + 1)].view(L * K, V + 1)[:, :V]
+        view.copy_(x)
+        check_step(decode.beam_select(view, s, f, eos=2), x, s, f, 2)
 
 
 @pytest.mark.gpu

@@ -43,7 +43,7 @@ def test_c_refusals(lib):
         lib.trba_clear_error()
 
     p = C.c_void_p(64)
-    for ins, outs, group in ((0, 4, 32), (4, 0, 32), (4, 4, 0), (4, 4, 16), (4, 4, 48), (4, 4, 129), (4, 4, -32)):
+    for ins, outs, group in ((0, 4, 32), (4, 0, 32), (4, (1 << 30) + 1, 32), ((1 << 30) + 1, 4, 32), (4, 4, 0), (4, 4, 16), (4, 4, 48), (4, 4, 129), (4, 4, -32)):
         refused(lib.trba_linear_int4_create(ins, outs, group, p, None), b"bad arguments")
         refused(lib.trba_linear_int4_create_codes(ins, outs, group, p, 1 << 20, p, 0, 1 << 20, None, None), b"bad arguments")
     refused(lib.trba_linear_int4_create(4, 4, 32, None, None), b"bad arguments")
@@ -200,7 +200,8 @@ def test_forward_refusals(lib, cuda):
     for exc, word, args, kw in ((TypeError, "float32", (x.double(),), {}), (ValueError, "in_features", (x[:, :39],), {}),
                                 (ValueError, "CUDA", (x.cpu(),), {}), (ValueError, "out must be", (x,), dict(out=x)),
                                 (ValueError, "apart", (x,), dict(out=torch.zeros(1, 8, device="cuda").expand(2, 8))),
-                                (TypeError, "torch tensor", (x.cpu().numpy(),), {})):
+                                (TypeError, "torch tensor", (x.cpu().numpy(),), {}),
+                                (ValueError, "overlaps", (x,), dict(out=x.view(-1)[30:46].view(2, 8)))):
         with pytest.raises(exc, match=word):
             lin.forward(*args, **kw)
     lib.trba_clear_error()

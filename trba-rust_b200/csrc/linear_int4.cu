@@ -798,7 +798,7 @@ int layout(trba_linear_int4 *l, const uint8_t *codes, i64 pitch, const void *sca
 }
 
 bool sizes_ok(int in, int out, int group) {
-    return in > 0 && out > 0 && (group == 32 || group == 64 || (group >= 128 && group % 128 == 0));
+    return in > 0 && in <= (1 << 30) && out > 0 && out <= (1 << 30) && (group == 32 || group == 64 || (group >= 128 && group % 128 == 0));
 }
 
 trba_linear_int4 *allocate(int in, int out, int group, int scale_dtype) {
@@ -894,7 +894,7 @@ long long trba_linear_int4_workspace(const trba_linear_int4 *l, int dtype, int r
 
 int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype, long long ldx, int rows, void *y,
                              long long ldy, void *workspace, long long workspace_bytes, void *stream) {
-    TRBA_REQUIRE_RET(l && rows >= 0 && rows <= (1 << 20), "trba_linear_int4_forward: bad arguments", -1);
+    TRBA_REQUIRE_RET(l && rows >= 0 && rows <= 1000000, "trba_linear_int4_forward: bad arguments", -1);
     if (rows == 0) return 0;
     TRBA_REQUIRE_RET(x && y && ldx >= l->in && ldy >= l->out, "trba_linear_int4_forward: bad arguments", -1);
     TRBA_REQUIRE_RET(dtype == TRBA_F32 || dtype == TRBA_BF16 || dtype == TRBA_F16,

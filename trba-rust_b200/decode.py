@@ -5,11 +5,14 @@
     seqs, lengths = beam_sequences(tokens, parents, eos=2)
 
 Work is queued on torch's current stream of the tensors' device, or on
-``stream`` (a torch.cuda.Stream); outputs belong to that stream.  Arguments
-are checked here: a ValueError or TypeError means that nothing ran.
+``stream`` (a torch.cuda.Stream); outputs and workspaces belong to that
+stream.  As with torch's own operators, inputs that another stream writes have
+to be waited for, and kept, by the caller.  Arguments are checked here: a
+ValueError or TypeError means that nothing ran.
 """
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import NamedTuple, Sequence
@@ -62,6 +65,11 @@ def _check_cuda(name, t, device=None):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+@functools.lru_cache(maxsize=256)
+def _select_workspace(code, lines, beams, vocab, device_index):
+    return lib().trba_beam_select_workspace(code, lines, beams, vocab)
+
+
 def _check_beams(beams):
     if not 1 <= beams <= MAX_BEAMS:
         raise ValueError(f"1 to {MAX_BEAMS} beams are supported, got {beams}")
@@ -102,7 +110,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     if len(shape) == 2 and shape[0] == lines * beams:
         ld = strides[0]
     elif len(shape) == 3 and shape[0] == lines and shape[1] == beams:
-        if lines > 1 and strides[0] != beams * strides[1]:
+        if lines > 1 and beams > 1 and strides[0] != beams * strides[1]:
             raise ValueError("logits must have one stride over all (line, beam) rows")
         ld = strides[1] if beams > 1 else strides[0]
     else:
@@ -148,7 +156,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
             _check_out(f"out.{name}", t, (lines, beams), dtype, device)
     if lines:
         L = lib()
-        need = L.trba_beam_select_workspace(code, lines, beams, vocab)
+        need = _select_workspace(code, lines, beams, vocab, device.index)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         rc = L.trba_beam_select(logits.data_ptr(), code, ld, scores.data_ptr(),
                                 None if finished is None else finished.data_ptr(), lines, beams, vocab, eos,
@@ -280,7 +288,8 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1
     the paths that end in the last step's slots, from the [steps, lines,
     beams] int32 tokens and parents of all steps: each path's tokens before
     its first `eos`, then `pad`."""
-    _check_tensors(tokens=tokens, parents=parents)
+    if not (isinstance(tokens, Tensor) and isinstance(parents, Tensor)):
+        _check_tensors(tokens=tokens, parents=parents)
     if tokens.dim() != 3 or tokens.dtype != torch.int32 or parents.shape != tokens.shape or parents.dtype != torch.int32:
         raise ValueError("tokens and parents must be int32 tensors [steps, lines, beams]")
     steps, lines, beams = tokens.shape

@@ -129,14 +129,15 @@ class LinearInt4:
 
     @staticmethod
     def _check_sizes(in_features, out_features, group):
-        if in_features < 1 or out_features < 1:
-            raise ValueError(f"LinearInt4: sizes must be positive, got {in_features} -> {out_features}")
+        if not (1 <= in_features <= 1 << 30 and 1 <= out_features <= 1 << 30):
+            raise ValueError(f"LinearInt4: sizes must be 1 to 2**30, got {in_features} -> {out_features}")
         if group not in (32, 64) and (group < 128 or group % 128):
             raise ValueError(f"LinearInt4: group must be 32, 64 or a multiple of 128, got {group}")
 
     def _own(self, in_features, out_features, group, handle):
         import torch
-        self.L = lib()
+        from . import decode
+        self.L, self.torch, self.decode = lib(), torch, decode
         self.in_features, self.out_features, self.group, self.h = in_features, out_features, group, handle
         if not handle:
             raise _err(self.L, "LinearInt4")
@@ -189,8 +190,7 @@ class LinearInt4:
         """[rows, in] -> [rows, out] of the same type (float32, bfloat16 or
         float16); leading dimensions of x are rows.  Runs on torch's current
         stream, or on `stream` (a torch.cuda.Stream)."""
-        import torch
-        from . import decode
+        torch, decode = self.torch, self.decode
         if not isinstance(x, torch.Tensor) or out is not None:
             decode._check_tensors(x=x, out=out)
         code = decode.DTYPE_CODES.get(x.dtype)
@@ -222,8 +222,12 @@ class LinearInt4:
             ldy = out.stride(0) if out.dim() == 2 and rows > 1 else outs
             if ldy < outs or (outs > 1 and out.stride(-1) != 1):
                 raise ValueError("LinearInt4::forward: the rows of out must be contiguous and apart")
-        if rows > 1 << 20:
-            raise ValueError("LinearInt4::forward: at most 2**20 rows")
+            if rows:
+                (a, b), (c, d) = decode._span(x), decode._span(out)
+                if a < d and c < b:
+                    raise ValueError("LinearInt4::forward: out overlaps x")
+        if rows > 1000000:
+            raise ValueError("LinearInt4::forward: at most a million rows")
         if rows:
             need = self.L.trba_linear_int4_workspace(self.h, code, rows) if rows > 2 else 0
             work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
