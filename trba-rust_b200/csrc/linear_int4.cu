@@ -293,20 +293,25 @@ __device__ __forceinline__ void store8(const Args &a, const Eight &v, uint8_t *d
         *reinterpret_cast<uint4 *>(dst + p * apart) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
 }
 
-// The activations as B fragments: a thread a fragment's 16 bytes (three for f32).
+// The activations as B fragments: a thread eight of a row (three 16-byte
+// pieces for f32).  Columns go row by row, an f32 row's three next to each
+// other; what stands in the columns behind the last does not matter.
 __global__ void __launch_bounds__(256) int4_fragments_kernel(const __grid_constant__ Args a, int nt) {
-    const int split = a.dtype == TRBA_F32 ? 3 : 1, per = nt / split;  // column tiles of a part
-    const i64 total = (i64)a.chunks * 4 * per * 32;
+    const int split = a.dtype == TRBA_F32 ? 3 : 1;
     const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
     uint4 *frags = a.frags + (i64)blockIdx.y * a.chunks * 4 * nt * 32;
-    GRID_LOOP(e, total) {
-        const int lane = (int)(e & 31);
-        const i64 q = e >> 5, cw = q / per;
-        const int n = (int)(q - cw * per), r = n * 8 + (lane >> 2);
-        Eight v;
-        v.lo = v.hi = make_uint4(0, 0, 0, 0);
-        if (r < rows) v = load8(a, row0 + r, (int)cw * 32 + (lane & 3) * 8);
-        store8(a, v, reinterpret_cast<uint8_t *>(frags + (cw * nt + n) * 32 + lane), per * 512);
+    GRID_LOOP(e, (i64)a.chunks * 4 * rows * 4) {
+        const int t = (int)(e & 3);
+        const i64 q = e >> 2, cw = q / rows;
+        const int r = (int)(q - cw * rows);
+        const Eight v = load8(a, row0 + r, (int)cw * 32 + t * 8);
+        uint4 part[3];
+        store8(a, v, reinterpret_cast<uint8_t *>(part), 16);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const int c = split * r + p;
+            if (p < split) frags[(cw * nt + (c >> 3)) * 32 + (c & 7) * 4 + t] = part[p];
+        }
     }
 }
 
@@ -363,25 +368,21 @@ __device__ __forceinline__ void write_tile(const Args &a, int tile, int row0, in
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int q = 0; q < 4; ++q) put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8, tot[n][q]);
-    } else if (NT == 1) {  // columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
+    } else {  // columns 3 r, 3 r + 1, 3 r + 2 lie in up to two lanes
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int r = 0; r < NT * 8 / 3; ++r) {
+            if (r >= rows) break;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int h = 0; h < 2; ++h) {
                 float v[3];
 #pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    v[p] = __shfl_sync(kFull, tot[0][2 * h + ((3 * r + p) & 1)], 4 * g + (3 * r + p) / 2);
-                if (t == r) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
+                for (int p = 0; p < 3; ++p) {
+                    const int c = 3 * r + p;
+                    v[p] = __shfl_sync(kFull, tot[c / 8][2 * h + (c & 1)], 4 * g + (c & 7) / 2);
+                }
+                if (t == (r & 3)) put(r, n0 + 8 * h, v[0] + (v[1] + v[2]));
             }
-    } else if (NT % 3 == 0) {  // the three parts are a third of the column tiles each
-        constexpr int kPer = NT / 3 > 0 ? NT / 3 : 1;
-#pragma unroll
-        for (int n = 0; n < kPer; ++n)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                put(n * 8 + 2 * t + (q & 1), n0 + (q >> 1) * 8,
-                    tot[n][q] + (tot[(n + kPer) % NT][q] + tot[(n + 2 * kPer) % NT][q]));
+        }
     }
 }
 
@@ -700,16 +701,14 @@ int launch_type(const Args &a, bool scale_f16, int wg, int nt, dim3 grid, size_t
     return launch_nt<F16, float, 4>(a, nt, grid, smem, st);
 }
 
-// How the rows are shared out: up to 64 columns a row block, an f32 row being
-// three (one or two rows pack them into one column tile, 16 rows make six).
+// How the rows are shared out: up to 64 columns a row block, an f32 row being three.
 struct Shape {
     int blocks, block_rows, nt;
     Shape(int rows, int dtype) {
-        const bool f32 = dtype == TRBA_F32;
-        const int most = f32 ? 16 : 64;
+        const int split = dtype == TRBA_F32 ? 3 : 1, most = 64 / split;
         blocks = (rows + most - 1) / most;
         block_rows = (rows + blocks - 1) / blocks;
-        nt = f32 ? (block_rows <= 2 ? 1 : block_rows <= 8 ? 3 : 6) : (block_rows + 7) / 8;
+        nt = (block_rows * split + 7) / 8;
         if (nt == 7) nt = 8;
     }
     i64 workspace(int chunks) const { return nt > 1 ? (i64)blocks * chunks * 4 * nt * 512 : 0; }
@@ -731,7 +730,7 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
     i64 smem = 0;
     int ctas = 0;
     if (nt > 1) {
-        int4_fragments_kernel<<<dim3(grid_for((i64)l->chunks * 4 * nt * 32), blocks_y), 256, 0, st>>>(a, nt);
+        int4_fragments_kernel<<<dim3(grid_for((i64)l->chunks * 16 * a.block_rows), blocks_y), 256, 0, st>>>(a, nt);
         if (const int e = launched()) return e;
         // Tiles side by side: the fewest steps of the CTA with the most.
         i64 best = -1;
