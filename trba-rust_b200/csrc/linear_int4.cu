@@ -123,7 +123,8 @@ constexpr int kPair = 2;  // blocks of a stage of the few-columns kernel
 // Few columns need few registers: 32 warps hide more latency; two stages of
 // two blocks each keep 64 KB in flight a SM.
 constexpr int kFewWarps = 32, kManyWarps = 16;
-constexpr int many_depth(int nt) { return nt <= 5 ? 4 : 3; }
+constexpr int many_depth(int nt) { return nt > 3 && nt <= 5 ? 4 : 3; }
+constexpr int many_blocks(int nt) { return nt <= 3 ? 2 : 1; }  // of a warp in a step
 
 // y^T = W x^T on the tensor cores: A is a 16-output tile of the weights, the
 // codes turned into exact bf16 or f16 integers in registers, B the
@@ -501,8 +502,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
     }
 }
 
-// More columns: the CTA moves in steps of a block a warp, `wn` tiles side by
-// side and wk chunks deep, through stages that hold the step's B fragments
+// More columns: the CTA moves in steps of a block or two a warp, `wn` tiles
+// side by side and wk warps deep, through stages that hold the step's B fragments
 // (read by all warps) and each warp's block.  Staging the activations as
 // fragments in memory first makes their copies plain and aligned; per SM and
 // step they are read once for wn tiles.  From about 24 columns on the tensor
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
 template <bool F16, class S, int WG, int NT>
 __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int D = many_depth(NT), kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S);
+    constexpr int D = many_depth(NT), KS = many_blocks(NT), kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wk_n = kManyWarps / a.wn, wn = warp / wk_n, wk = warp - wn * wk_n;
     const int groups = (a.tiles + a.wn - 1) / a.wn;
@@ -518,31 +519,32 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
     const int g0 = (int)((i64)groups * bx / gx), g1 = (int)((i64)groups * (bx + 1) / gx);
     const int cb = a.chunks * rank / a.cs, ce = a.chunks * (rank + 1) / a.cs;  // this CTA's chunks
     const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
-    const int xbytes = wk_n * NT * 2048, stage = xbytes + kManyWarps * kBlock;
+    const int deep = wk_n * KS, xbytes = deep * NT * 2048, stage = xbytes + kManyWarps * KS * kBlock;
     const uint8_t *frags = reinterpret_cast<const uint8_t *>(a.frags) + (i64)blockIdx.y * a.chunks * NT * 2048;
     const uint32_t smem_s = smem_addr(smem);
     float4 *red = reinterpret_cast<float4 *>(smem + a.red_at);
 
     int pg = g0, pc = cb, ps = 0;  // the next stage to fill: its group, first chunk, place
     auto weights = [&](uint32_t to) {
-        const int tile = pg * a.wn + wn, c = pc + wk;
+        const int tile = pg * a.wn + wn, c = pc + wk * KS;
         if (pg < g1 && tile < a.tiles && c < ce) {
             const uint8_t *src = a.blocks + ((i64)tile * a.chunks + c) * kBlock + lane * 16;
-            const uint32_t dst = to + xbytes + warp * kBlock + lane * 16;
-            cp16(dst, src);
-            cp16(dst + 512, src + 512);
-            if (lane * 16 < kBlock - 1024) cp16(dst + 1024, src + 1024);
+            const uint32_t dst = to + xbytes + warp * KS * kBlock + lane * 16;
+            const int bytes = min(KS, ce - c) * kBlock - lane * 16;
+#pragma unroll
+            for (int o = 0; o < KS * kBlock; o += 512)
+                if (o < bytes) cp16(dst + o, src + o);
         }
     };
     auto activations = [&](uint32_t to) {
         if (pg < g1) {
-            const int bytes = min(wk_n, ce - pc) * NT * 2048;
+            const int bytes = min(deep, ce - pc) * NT * 2048;
             const uint8_t *src = frags + (i64)pc * NT * 2048;
             for (int o = threadIdx.x * 16; o < bytes; o += kManyWarps * 32 * 16) cp16(to + o, src + o);
         }
     };
     auto next = [&]() {
-        pc += wk_n;
+        pc += deep;
         if (pc >= ce) {
             pc = cb;
             ++pg;
@@ -564,17 +566,20 @@ __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __g
         float tot[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
-        for (int c0 = cb; c0 < ce; c0 += wk_n) {
+        for (int c0 = cb; c0 < ce; c0 += deep) {
             asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
             __syncthreads();  // the stage is there for all, and the last one is free
             weights(smem_s + ps * stage);
             activations(smem_s + ps * stage);
             asm volatile("cp.async.commit_group;" ::: "memory");
             next();
-            if (tile < a.tiles && c0 + wk < ce) {
-                const uint8_t *st = smem + cs * stage, *xs = st + wk * NT * 2048 + lane * 16;
+            const uint8_t *st = smem + cs * stage;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                if (tile >= a.tiles || c0 + wk * KS + j >= ce) break;
+                const uint8_t *xs = st + (wk * KS + j) * NT * 2048 + lane * 16;
                 block_product<F16, S, WG, NT>(
-                    st + xbytes + warp * kBlock,
+                    st + xbytes + (warp * KS + j) * kBlock,
                     [&](int w, int n) { return *reinterpret_cast<const uint4 *>(xs + (w * NT + n) * 512); }, tot, lane);
             }
             cs = cs + 1 == D ? 0 : cs + 1;
@@ -736,13 +741,14 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
         i64 best = -1;
         for (int wn = kManyWarps; wn >= 1; wn >>= 1) {
             const int wk = kManyWarps / wn, red = wn * (wk - 1) * nt * 512;
-            const i64 stages = (i64)many_depth(nt) * (wk * nt * 2048 + kManyWarps * l->block);
+            const int ks = many_blocks(nt);
+            const i64 stages = (i64)many_depth(nt) * ks * (wk * nt * 2048 + kManyWarps * l->block);
             if (stages + red > kMaxSmem) break;
             const int groups = (a.tiles + wn - 1) / wn, grid = groups < sm_count() ? groups : sm_count();
             int cs = 1;  // (then every CTA has one group)
-            while (cs < 8 && 2 * cs * groups <= sm_count() && 2 * cs * wk <= a.chunks) cs *= 2;
+            while (cs < 8 && 2 * cs * groups <= sm_count() && 2 * cs * wk * ks <= a.chunks) cs *= 2;
             const i64 each = (a.chunks + cs - 1) / cs;
-            const i64 cost = (i64)((groups + grid - 1) / grid) * ((each + wk - 1) / wk + 1) + (cs > 1 ? 2 : 0);
+            const i64 cost = (i64)((groups + grid - 1) / grid) * ((each + wk * ks - 1) / (wk * ks) * ks + 1) + (cs > 1 ? 2 : 0);
             if (best < 0 || cost < best)
                 best = cost, a.wn = wn, a.cs = cs, ctas = grid * cs, a.red_at = (int)stages, smem = stages + red;
         }
