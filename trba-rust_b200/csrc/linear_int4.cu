@@ -745,11 +745,15 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
             const i64 stages = (i64)many_depth(nt) * ks * (wk * nt * 2048 + kManyWarps * l->block);
             if (stages + red > kMaxSmem) break;
             const int groups = (a.tiles + wn - 1) / wn, grid = groups < sm_count() ? groups : sm_count();
-            int cs = 1;  // (then every CTA has one group)
-            while (cs < 8 && 2 * cs * groups <= sm_count() && 2 * cs * wk * ks <= a.chunks) cs *= 2;
+            // A split over clusters leaves every CTA one group.  Clusters of 8
+            // do not all find 8 free SMs next to each other on a full device:
+            // 16 of them ran 24.5 us where 32 of 4 ran 16.4.
+            int cs = 1;
+            const auto fits = [&](int c) { return c * groups <= (c == 8 ? 96 : c == 4 ? 128 : sm_count()); };
+            while (cs < 8 && fits(2 * cs) && 2 * cs * wk * ks <= a.chunks) cs *= 2;
             const i64 each = (a.chunks + cs - 1) / cs;
             const i64 cost = (i64)((groups + grid - 1) / grid) * ((each + wk * ks - 1) / (wk * ks) * ks + 1) + (cs > 1 ? 2 : 0);
-            if (best < 0 || cost < best)
+            if (best < 0 || cost <= best)
                 best = cost, a.wn = wn, a.cs = cs, ctas = grid * cs, a.red_at = (int)stages, smem = stages + red;
         }
     } else {
