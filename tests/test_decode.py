@@ -387,10 +387,11 @@ def test_sequences_match_oracle(T, L, K, lib, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K", [5, 8])
 @pytest.mark.parametrize("T", [3, 40, 700])
-def test_sequences_with_bad_parents(T, cuda):
+def test_sequences_with_bad_parents(T, K, cuda):
     rng = np.random.default_rng(T)
-    L, K = 4, 5
+    L = 4
     tok = rng.integers(3, 60, (T, L, K)).astype(np.int32)
     par = rng.integers(0, K, (T, L, K)).astype(np.int32)
     par[0] = -1

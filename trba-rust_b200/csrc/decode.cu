@@ -709,12 +709,31 @@ struct Trace {
     int32_t *seq, *lengths;
     int steps, lines, beams, eos, pad;
     int group, segs, chunk, splits;
+    bool fours;  // parents can be read four at a time
 };
 
-constexpr int kTraceLoads = 8;  // loads in flight a thread
+constexpr int kTraceLoads = 4;  // loads in flight a thread
+
+// A thread's walk over [major][minor] in strides, without a division a step.
+struct Index {
+    int major, minor, minors, up, right;
+    __device__ __forceinline__ Index(int first, int minors_, int stride)
+        : major(first / minors_), minor(first % minors_), minors(minors_), up(stride / minors_), right(stride % minors_) {}
+    __device__ __forceinline__ void next() {
+        major += up;
+        minor += right;
+        if (minor >= minors) {
+            minor -= minors;
+            ++major;
+        }
+    }
+};
+// The first slot of a slot's line.
+__device__ __forceinline__ int line_of(int k, int beams) { return k - k % beams; }
+
 
 __global__ void __launch_bounds__(1024) beam_sequences_kernel(const Trace a) {
-    extern __shared__ uint8_t tr_smem[];
+    extern __shared__ __align__(16) uint8_t tr_smem[];
     const int threads = blockDim.x;
     const int gk = a.group * a.beams;  // slots of the CTA's lines
     uint8_t *par = tr_smem;            // [chunk][gk]
@@ -734,18 +753,39 @@ __global__ void __launch_bounds__(1024) beam_sequences_kernel(const Trace a) {
     for (int hi = a.steps; hi > 0; hi -= a.chunk) {  // the steps [lo, hi)
         const int lo = max(0, hi - a.chunk), c = hi - lo;
         __syncthreads();
-        for (int e0 = threadIdx.x; e0 < c * slots; e0 += threads * kTraceLoads) {
-            int p[kTraceLoads], at[kTraceLoads];
+        // (unsigned: what is out of range, below 0 too, is no slot)
+        const auto slot_of = [&](int p) { return (unsigned)p < (unsigned)a.beams ? (unsigned)p : (unsigned)kLost; };
+        const int32_t *row = parents + lo * n;
+        if (a.fours) {  // four slots at a time
+            Index at(threadIdx.x, slots >> 2, threads);  // step, slot / 4
+            for (int e0 = threadIdx.x; e0 < c * (slots >> 2); e0 += threads * 4) {
+                int4 p[4];
+                int to[4];
 #pragma unroll
-            for (int u = 0; u < kTraceLoads; ++u) {
-                const int e = e0 + u * threads, t = e / slots, k = e - t * slots;
-                at[u] = t * gk + k;
-                p[u] = e < c * slots && lo + t ? parents[(lo + t) * n + k] : 0;  // step 0 has no parents
+                for (int u = 0; u < 4; ++u, at.next()) {
+                    to[u] = at.major < c ? at.major * gk + at.minor * 4 : -1;
+                    p[u] = make_int4(0, 0, 0, 0);  // step 0 has no parents
+                    if (to[u] >= 0 && lo + at.major) p[u] = *reinterpret_cast<const int4 *>(row + at.major * n + at.minor * 4);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (to[u] >= 0)
+                        *reinterpret_cast<unsigned *>(par + to[u]) = slot_of(p[u].x) | slot_of(p[u].y) << 8 |
+                                                                     slot_of(p[u].z) << 16 | slot_of(p[u].w) << 24;
             }
+        } else {
+            Index at(threadIdx.x, slots, threads);  // step, slot
+            for (int e0 = threadIdx.x; e0 < c * slots; e0 += threads * kTraceLoads) {
+                int p[kTraceLoads], to[kTraceLoads];
 #pragma unroll
-            for (int u = 0; u < kTraceLoads; ++u)
-                if (e0 + u * threads < c * slots)
-                    par[at[u]] = (unsigned)p[u] < (unsigned)a.beams ? (uint8_t)p[u] : kLost;
+                for (int u = 0; u < kTraceLoads; ++u, at.next()) {
+                    to[u] = at.major < c ? at.major * gk + at.minor : -1;
+                    p[u] = to[u] >= 0 && lo + at.major ? row[at.major * n + at.minor] : 0;
+                }
+#pragma unroll
+                for (int u = 0; u < kTraceLoads; ++u)
+                    if (to[u] >= 0) par[to[u]] = (uint8_t)slot_of(p[u]);
+            }
         }
         __syncthreads();
         const int per = (c + a.segs - 1) / a.segs;
@@ -779,18 +819,18 @@ __global__ void __launch_bounds__(1024) beam_sequences_kernel(const Trace a) {
             }
         }
         __syncthreads();
+        Index it(threadIdx.x, c, threads);  // slot, step
         for (int e0 = threadIdx.x; e0 < c * own; e0 += threads * kTraceLoads) {
             int tok[kTraceLoads], k[kTraceLoads], t[kTraceLoads], x[kTraceLoads];
 #pragma unroll
-            for (int u = 0; u < kTraceLoads; ++u) {
-                const int e = min(e0 + u * threads, c * own - 1), q = e / c;
-                t[u] = e - q * c, k[u] = k0 + q;
-                x[u] = path[t[u] * gk + k[u]];
-                tok[u] = x[u] == kLost ? a.pad : tokens[(lo + t[u]) * n + k[u] - k[u] % a.beams + x[u]];
+            for (int u = 0; u < kTraceLoads; ++u, it.next()) {
+                k[u] = it.major < own ? k0 + it.major : -1, t[u] = it.minor;
+                x[u] = k[u] >= 0 ? path[t[u] * gk + k[u]] : kLost;
+                tok[u] = x[u] == kLost ? a.pad : tokens[(lo + t[u]) * n + line_of(k[u], a.beams) + x[u]];
             }
 #pragma unroll
             for (int u = 0; u < kTraceLoads; ++u) {
-                if (e0 + u * threads >= c * own) break;
+                if (k[u] < 0) break;
                 if (x[u] == kLost) atomicMin(&len[k[u]], -1);
                 else if (tok[u] == a.eos) atomicMin(&len[k[u]], lo + t[u]);
                 a.seq[(base + k[u]) * a.steps + lo + t[u]] = tok[u];
@@ -1023,6 +1063,7 @@ int trba_beam_sequences(const int32_t *tokens, const int32_t *parents, int steps
     while (steps >= 128 && a.group == 1 && a.splits < 8 && 2 * a.splits <= beams && 2 * a.splits * lines <= sm_count())
         a.splits *= 2;
     const int gk = a.group * beams;
+    a.fours = beams % 4 == 0 && reinterpret_cast<uintptr_t>(parents) % 16 == 0;
     a.chunk = kTraceSmem / (2 * gk);
     if (a.chunk > steps) a.chunk = steps;
     if (a.chunk < a.segs) a.chunk = a.segs;  // (the entry slots pass through the path's rows)
