@@ -82,10 +82,15 @@ trba_linear_int4 *trba_linear_int4_create(int in_features, int out_features, int
  * even input's code in the low half, row stride ld_codes bytes; scales [out,
  * ceil(in / group)], f32 or f16 (scale_dtype: TRBA_F32 or TRBA_F16 of
  * trba_decode.h), row stride ld_scales elements; bias f32 [out] or NULL.
- * Reads them in `stream`'s order and returns when they may be freed. */
+ * storage: NULL, and the layer allocates what it keeps, reads the rest in
+ * `stream`'s order and returns when it may be freed; or a device buffer of
+ * trba_linear_int4_bytes(...) bytes, aligned to 16, that the caller keeps for
+ * the layer's life, and everything is only queued on `stream`. */
+long long trba_linear_int4_bytes(int in_features, int out_features, int group, int scale_dtype);
 trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_features, int group, const uint8_t *codes,
                                                 long long ld_codes, const void *scales, int scale_dtype,
-                                                long long ld_scales, const float *bias, void *stream);
+                                                long long ld_scales, const float *bias, void *storage,
+                                                long long storage_bytes, void *stream);
 void trba_linear_int4_destroy(trba_linear_int4 *l);
 /* x [rows, in] and y [rows, out] on the device, both of `dtype` (TRBA_F32,
  * TRBA_BF16, TRBA_F16), row strides ldx >= in and ldy >= out in elements; y

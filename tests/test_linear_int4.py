@@ -45,10 +45,15 @@ def test_c_refusals(lib):
     p = C.c_void_p(64)
     for ins, outs, group in ((0, 4, 32), (4, 0, 32), (4, (1 << 30) + 1, 32), ((1 << 30) + 1, 4, 32), (4, 4, 0), (4, 4, 16), (4, 4, 48), (4, 4, 129), (4, 4, -32)):
         refused(lib.trba_linear_int4_create(ins, outs, group, p, None), b"bad arguments")
-        refused(lib.trba_linear_int4_create_codes(ins, outs, group, p, 1 << 20, p, 0, 1 << 20, None, None), b"bad arguments")
+        refused(lib.trba_linear_int4_create_codes(ins, outs, group, p, 1 << 20, p, 0, 1 << 20, None, None, 0, None), b"bad arguments")
+        assert lib.trba_linear_int4_bytes(ins, outs, group, 0) == -1
     refused(lib.trba_linear_int4_create(4, 4, 32, None, None), b"bad arguments")
     for bad in ((None, 2, p, 0, 1), (p, 1, p, 0, 1), (p, 2, None, 0, 1), (p, 2, p, 1, 1), (p, 2, p, 0, 0)):
-        refused(lib.trba_linear_int4_create_codes(4, 4, 32, *bad, None, None), b"bad arguments")
+        refused(lib.trba_linear_int4_create_codes(4, 4, 32, *bad, None, None, 0, None), b"bad arguments")
+    need = lib.trba_linear_int4_bytes(4, 4, 32, 0)
+    assert need == 1024 + 4 * 16 * 4 + 16
+    for at, size in ((64, need - 1), (72, need)):
+        refused(lib.trba_linear_int4_create_codes(4, 4, 32, p, 2, p, 0, 1, None, C.c_void_p(at), size, None), b"storage")
     refused(lib.trba_linear_int4_forward(None, p, 0, 4, 1, p, 4, None, 0, None), b"bad arguments")
     assert lib.trba_linear_int4_workspace(None, 0, 9) == 0
     assert lib.trba_linear_int4_get(None, None, None, None) == -1 and lib.trba_linear_int4_param_count(None) == -1
@@ -191,6 +196,23 @@ def test_quantised_layer(lib, cuda):
     codes[:, -1] = (codes[:, -1] & 15) | (st["codes"][:, -1] & 0xF0)  # behind the last input: no code
     assert np.array_equal(st["codes"], codes) and np.array_equal(st["scales"], s.float().cpu().numpy())
     assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_layer_with_its_own_memory(lib, cuda):
+    """create_codes without storage owns a copy: what it was made from may go."""
+    lin, q, s, b = layer(37, 211, 64, "f16", 3)
+    h = lib.trba_linear_int4_create_codes(211, 37, 64, C.c_void_p(q.data_ptr()), q.shape[1], C.c_void_p(s.data_ptr()), 2, s.shape[1],
+                                          C.c_void_p(b.data_ptr()), None, 0, None)
+    x = torch.randn(3, 211, device="cuda").bfloat16()
+    want, y = lin.forward(x), torch.empty(3, 37, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    q.fill_(0), s.fill_(0)
+    torch.cuda.synchronize()
+    assert lib.trba_linear_int4_forward(h, C.c_void_p(x.data_ptr()), 1, 211, 3, C.c_void_p(y.data_ptr()), 37, None, 0, None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and torch.equal(lin.forward(x), want)
+    lib.trba_linear_int4_destroy(h)
 
 
 @pytest.mark.gpu

@@ -30,7 +30,8 @@ struct trba_linear_int4 {
     int tiles = 0, chunks = 0;
     int gpc = 0;                // scales of a row in a chunk (1 for groups of 128 and more)
     int block = 0;              // bytes of a block: 1024 + 16 gpc scales
-    uint8_t *base = nullptr;    // one allocation: blocks [tiles][chunks], bias
+    bool owned = true;          // base is this layer's own allocation
+    uint8_t *base = nullptr;    // blocks [tiles][chunks], bias
     float *bias = nullptr;      // [out]
 };
 
@@ -87,13 +88,23 @@ __global__ void __launch_bounds__(256) int4_layout_kernel(const uint8_t *__restr
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const int k0 = chunk * 128 + w * 32 + (lane & 3) * 8;
-                v[w] = 0;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const int k = k0 + c;
-                    const uint32_t q = n < out && k < in ? (codes[n * pitch + (k >> 1)] >> (4 * (k & 1))) & 15u : 8u;
-                    v[w] |= q << (4 * (c >> 1) + 16 * (c & 1));
+                uint32_t q = 0x88888888u;  // eight codes as they come, four bits each
+                if (n < out && k0 < in) {
+                    const uint8_t *src = codes + n * pitch + (k0 >> 1);
+                    if (k0 + 8 <= in) {
+                        q = (reinterpret_cast<uintptr_t>(src) & 3) == 0
+                                ? *reinterpret_cast<const uint32_t *>(src)
+                                : src[0] | (uint32_t)src[1] << 8 | (uint32_t)src[2] << 16 | (uint32_t)src[3] << 24;
+                    } else {
+                        for (int k = k0; k < in; ++k) {
+                            const int c = k - k0;
+                            q = (q & ~(15u << (4 * c))) | ((src[c >> 1] >> (4 * (c & 1))) & 15u) << (4 * c);
+                        }
+                    }
                 }
+                uint32_t even = q & 0x0f0f0f0fu, odd = (q >> 4) & 0x0f0f0f0fu;
+                even = (even | even >> 4) & 0x00ff00ffu, odd = (odd | odd >> 4) & 0x00ff00ffu;
+                v[w] = ((even | even >> 8) & 0xffffu) | (odd | odd >> 8) << 16;
             }
             reinterpret_cast<uint4 *>(out_block + half * 512)[lane] = make_uint4(v[0], v[1], v[2], v[3]);
         }
@@ -810,24 +821,30 @@ bool sizes_ok(int in, int out, int group) {
     return in > 0 && in <= (1 << 30) && out > 0 && out <= (1 << 30) && (group == 32 || group == 64 || (group >= 128 && group % 128 == 0));
 }
 
-trba_linear_int4 *allocate(int in, int out, int group, int scale_dtype) {
-    auto *l = new (std::nothrow) trba_linear_int4;
-    if (!l) return nullptr;
+void lay_out(trba_linear_int4 *l, int in, int out, int group, int scale_dtype) {
     l->in = in, l->out = out, l->group = group, l->groups = (in - 1) / group + 1;
     l->scale_dtype = scale_dtype;
     l->tiles = (out - 1) / 16 + 1;
     l->chunks = (in - 1) / 128 + 1;
     l->gpc = group >= 128 ? 1 : 128 / group;
     l->block = 1024 + 16 * l->gpc * (scale_dtype == TRBA_F32 ? 4 : 2);
-    const size_t nc = (size_t)l->tiles * l->chunks * l->block;
+}
+size_t blocks_bytes(const trba_linear_int4 *l) { return (size_t)l->tiles * l->chunks * l->block; }
+
+trba_linear_int4 *allocate(int in, int out, int group, int scale_dtype, void *storage) {
+    auto *l = new (std::nothrow) trba_linear_int4;
+    if (!l) return nullptr;
+    lay_out(l, in, out, group, scale_dtype);
+    l->owned = !storage;
+    l->base = static_cast<uint8_t *>(storage);
     if (cudaGetDevice(&l->device) != cudaSuccess ||
-        cudaMalloc(&l->base, nc + (size_t)out * 4) != cudaSuccess) {
+        (l->owned && cudaMalloc(&l->base, blocks_bytes(l) + (size_t)out * 4) != cudaSuccess)) {
         cudaGetLastError();
         report_error(__FILE__, __LINE__, "LinearInt4: device allocation failed", -1);
         delete l;
         return nullptr;
     }
-    l->bias = reinterpret_cast<float *>(l->base + nc);
+    l->bias = reinterpret_cast<float *>(l->base + blocks_bytes(l));
     return l;
 }
 
@@ -842,7 +859,7 @@ trba_linear_int4 *trba_linear_int4_create(int in_features, int out_features, int
                                           const float *bias) {
     TRBA_REQUIRE_RET(sizes_ok(in_features, out_features, group) && weight_f32, "trba_linear_int4_create: bad arguments",
                      nullptr);
-    trba_linear_int4 *l = allocate(in_features, out_features, group, TRBA_F32);
+    trba_linear_int4 *l = allocate(in_features, out_features, group, TRBA_F32, nullptr);
     if (!l) return nullptr;
     const size_t nw = (size_t)in_features * out_features, ns = (size_t)out_features * l->groups;
     const i64 pitch = (in_features + 1ll) / 2;
@@ -868,21 +885,32 @@ trba_linear_int4 *trba_linear_int4_create(int in_features, int out_features, int
     return l;
 }
 
+long long trba_linear_int4_bytes(int in_features, int out_features, int group, int scale_dtype) {
+    if (!sizes_ok(in_features, out_features, group) || (scale_dtype != TRBA_F32 && scale_dtype != TRBA_F16)) return -1;
+    trba_linear_int4 l;
+    lay_out(&l, in_features, out_features, group, scale_dtype);
+    return (long long)(blocks_bytes(&l) + (size_t)out_features * 4);
+}
+
 trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_features, int group, const uint8_t *codes,
                                                 long long ld_codes, const void *scales, int scale_dtype,
-                                                long long ld_scales, const float *bias, void *stream) {
+                                                long long ld_scales, const float *bias, void *storage,
+                                                long long storage_bytes, void *stream) {
     TRBA_REQUIRE_RET(sizes_ok(in_features, out_features, group) && codes && scales &&
                          (scale_dtype == TRBA_F32 || scale_dtype == TRBA_F16) && ld_codes >= (in_features + 1ll) / 2 &&
                          ld_scales >= (in_features - 1) / group + 1,
                      "trba_linear_int4_create_codes: bad arguments", nullptr);
-    trba_linear_int4 *l = allocate(in_features, out_features, group, scale_dtype);
+    TRBA_REQUIRE_RET(!storage || (storage_bytes >= trba_linear_int4_bytes(in_features, out_features, group, scale_dtype) &&
+                                  reinterpret_cast<uintptr_t>(storage) % 16 == 0),
+                     "trba_linear_int4_create_codes: storage too small or not aligned to 16 bytes", nullptr);
+    trba_linear_int4 *l = allocate(in_features, out_features, group, scale_dtype, storage);
     if (!l) return nullptr;
     cudaStream_t st = as_stream(stream);
     bool ok = (scale_dtype == TRBA_F16 ? layout<__half>(l, codes, ld_codes, scales, ld_scales, st)
                                        : layout<float>(l, codes, ld_codes, scales, ld_scales, st)) == 0;
     ok = ok && (bias ? cudaMemcpyAsync(l->bias, bias, (size_t)out_features * 4, cudaMemcpyDeviceToDevice, st)
                      : cudaMemsetAsync(l->bias, 0, (size_t)out_features * 4, st)) == cudaSuccess;
-    if (cudaStreamSynchronize(st) != cudaSuccess) ok = false;
+    if (!storage && cudaStreamSynchronize(st) != cudaSuccess) ok = false;
     if (!ok) {
         report_error(__FILE__, __LINE__, "trba_linear_int4_create_codes: copying the weights failed", -1);
         trba_linear_int4_destroy(l);
@@ -893,7 +921,7 @@ trba_linear_int4 *trba_linear_int4_create_codes(int in_features, int out_feature
 
 void trba_linear_int4_destroy(trba_linear_int4 *l) {
     if (!l) return;
-    cudaFree(l->base);
+    if (l->owned) cudaFree(l->base);
     delete l;
 }
 

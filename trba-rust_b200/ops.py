@@ -148,7 +148,8 @@ class LinearInt4:
         """From quantised weights on the GPU: codes [out, ceil(in / 2)] uint8,
         the even input's code in the low half; scales [out, ceil(in / group)]
         float32 or float16; bias [out] float32 or None.  W = (code - 8) *
-        scale.  The tensors are copied."""
+        scale.  The tensors are copied, in the order of torch's current stream;
+        a layer used on another stream is made there or waited for first."""
         import torch
         from .decode import DTYPE_CODES, _check_cuda, _check_tensors, _on, _raw_stream
         _check_tensors(codes=codes, scales=scales, bias=bias)
@@ -169,16 +170,22 @@ class LinearInt4:
         with _on(device, None):
             codes, scales = codes.contiguous(), scales.contiguous()
             bias = None if bias is None else bias.contiguous()
+            need = lib().trba_linear_int4_bytes(in_features, out_features, group, DTYPE_CODES[scales.dtype])
+            storage = torch.empty(need, dtype=torch.uint8, device=device)
+            self.home = _raw_stream(device.index)  # the stream the storage belongs to
             self._own(in_features, out_features, group, lib().trba_linear_int4_create_codes(
                 in_features, out_features, group, codes.data_ptr(), codes.shape[1], scales.data_ptr(),
                 DTYPE_CODES[scales.dtype], scales.shape[1], None if bias is None else bias.data_ptr(),
-                _raw_stream(device.index)))
+                storage.data_ptr(), need, self.home))
+            self.storage = storage
         return self
+
+    storage = None  # torch's memory of a layer made by from_codes
 
     def close(self):
         if getattr(self, "h", None):
             self.L.trba_linear_int4_destroy(self.h)
-            self.h = None
+            self.h = self.storage = None
 
     def __del__(self):
         try:
@@ -229,11 +236,13 @@ class LinearInt4:
         if rows > 1000000:
             raise ValueError("LinearInt4::forward: at most a million rows")
         if rows:
+            raw = decode._raw_stream(device.index)
+            if self.storage is not None and raw != self.home:
+                self.storage.record_stream(torch.cuda.current_stream(device))  # not to be reused before this call is done
             need = self.L.trba_linear_int4_workspace(self.h, code, rows) if rows > 2 else 0
             work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             rc = self.L.trba_linear_int4_forward(self.h, x.data_ptr(), code, x.stride(0) if rows > 1 else ins, rows,
-                                                 out.data_ptr(), ldy, work.data_ptr() if need else None, need,
-                                                 decode._raw_stream(device.index))
+                                                 out.data_ptr(), ldy, work.data_ptr() if need else None, need, raw)
             if rc:
                 raise _err(self.L, "LinearInt4::forward")
         return out
