@@ -55,7 +55,8 @@ extern "C" {
  * to the sum).  Where a row holds +inf, its +inf tokens share the
  * probability evenly.  A NaN score counts as a dead beam.  Scores are
  * formed and compared in f64 and rounded to f32 at the end (the exponentials
- * are f32, their sums f64).
+ * are f32, and so are their sums within a batch of 16 (f32) or 32 (16-bit) of
+ * a thread's elements; beyond that f64).
  *
  * beams 1 .. 32, vocab 1 .. 2^30, beams * vocab < 2^31, lines * beams <
  * 2^24, eos in [0, vocab) or -1 for "no end token" (then finished must be

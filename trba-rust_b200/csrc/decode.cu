@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <atomic>
 #include <type_traits>
@@ -137,7 +138,6 @@ struct Found {
     Key best[TRBA_MAX_BEAMS];
     float top;
 };
-
 
 template <class T>
 __device__ __forceinline__ float element(uint32_t w, int half) {
@@ -538,7 +538,11 @@ struct Line {
     }
 };
 
-// Short rows: a CTA a line, a warp a row.
+// Short rows: a CTA a line, a warp a row.  Bound by latency: a read of the row,
+// its sort, the logarithm and `beams` rounds of picking, one after the other
+// (one line of 5 beams over 130 f32: 6.4 us; 512 lines of 5: 8.4; a
+// launch of nothing takes about 2).  One kernel, because a second launch would
+// add half as much again.
 template <class T>
 __global__ void __launch_bounds__(512) select_line_kernel(const T *__restrict__ logits, i64 ld, const float *scores,
                                                           const uint8_t *finished, int beams, int vocab, int eos,
@@ -563,7 +567,12 @@ __global__ void __launch_bounds__(512) select_line_kernel(const T *__restrict__ 
 
 // Long rows, first part: a warp a segment of a row, to the workspace.  Warps
 // of dead and finished beams end at once; the others come and go, so that
-// some read while others pick their best.
+// some read while others pick their best.  64 lines of 10 beams over 65536 f32
+// (134 MB of live rows): 36 us with the merge, 3.7 TB/s of 6.5; what bounds it
+// is the instructions an element takes (a conversion, a maximum, a subtraction
+// and product, an exponential and an addition; issue slots 47% used with 22
+// warps a SM) and the second look's latency, not the bytes.  Seven CTAs a SM of
+// 64 registers a thread are what keeps enough reads in flight.
 constexpr int kScanWarps = 4;
 template <class T>
 __global__ void __launch_bounds__(kScanWarps * 32, 7) select_scan_kernel(
@@ -579,7 +588,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 7) select_scan_kernel(
     scan_segment<T>(logits + row * ld, c0, min(vocab, c0 + seg_len), beams, lane, scan[warp], found[u]);
 }
 
-// Second part: a CTA a line.
+// Second part: a CTA a line; bound by latency, as the short rows are (6 to 9
+// us for 64 lines of 10 beams, 16 segments each).
 __global__ void __launch_bounds__(512) select_merge_kernel(const Found *__restrict__ found, int segs,
                                                            const float *scores, const uint8_t *finished, int beams,
                                                            int eos, float *out_scores, int32_t *__restrict__ out_tokens,
@@ -665,8 +675,12 @@ __device__ __noinline__ void move_bytes(const char *src, char *dst, int bytes, i
     if (lane < bytes - done) dst[done + lane] = src[done + lane];
 }
 
+// 4 layer states of 5 MB: 10.9 us (3.8 TB/s read and written, the L2 cache
+// serving part); 8 cache tensors of 87 MB: 198 us (7.0 TB/s counting every row
+// as read, parents that repeat being read once from memory), which is what a
+// plain copy of as many bytes takes.
 // STREAM: more than stays in the L2 cache is moved, past it (203 us instead of
-// 214 for 0.7 GB).
+// 214 for 0.7 GB, both with 8 CTAs a SM).
 template <bool STREAM>
 __global__ void __launch_bounds__(256, 4) beam_reorder_kernel(const __grid_constant__ StateViews st,
                                                            const int32_t *__restrict__ parents, int rows, int beams) {
@@ -700,6 +714,9 @@ __global__ void __launch_bounds__(256, 4) beam_reorder_kernel(const __grid_const
 // maps are composed, and a second walk from the right slots notes the path.
 // A CTA takes `group` lines, or a part of one line's beams (all CTAs of a line
 // read its parents).  Steps that do not fit go in chunks, last first.
+// Bound by the latency of the reads and of the barriers between the walks: 512
+// lines of 5 beams, 21 steps 6.4 us; 16 lines of 16 beams, 2000 steps 17 us
+// (0.36 TB/s), where a thread a path over device memory took 1007.
 constexpr uint8_t kLost = 255;  // behind a parent out of range
 
 constexpr int kTraceSmem = 96 * 1024;
@@ -730,7 +747,6 @@ struct Index {
 };
 // The first slot of a slot's line.
 __device__ __forceinline__ int line_of(int k, int beams) { return k - k % beams; }
-
 
 __global__ void __launch_bounds__(1024) beam_sequences_kernel(const Trace a) {
     extern __shared__ __align__(16) uint8_t tr_smem[];
@@ -854,9 +870,11 @@ int launched() {
 // How a selection runs: rows of up to two batches whole (segs = 0), longer
 // ones in segments of whole batches: one round of warps on the device, but no
 // segment so short that picking its best (and joining them, with many beams)
-// costs more than reading it, and none much longer than the spans that are
-// remembered.  64 lines of 10 beams, 65536 f32: 72 us at 2 batches a segment,
-// 43 at 8, 38 at 24; 8 lines of 4 beams, 32000 f32: 12 us at 2, 19 at 24.
+// costs more than reading it, and none of more batches than there are spans to
+// remember, so that a second look is at one batch's groups.  With 2 / 4 / 8 /
+// 16 / 24 / 32 batches a segment, 64 lines of 10 beams, 65536 f32 take 68 / 50 /
+// 41 / 36 / 39 / 41 us, 16 lines of 32 beams, 20000 bf16 51 / 39 / 35 / 35 / 37 /
+// 37, one line of 5 beams, 32000 bf16 11 / 12 / 15 / 19 / 19 / 27.
 struct Plan {
     int segs, len;
     Plan(int lines, int beams, int vocab, int size) {
@@ -864,7 +882,7 @@ struct Plan {
         segs = len = 0;
         if (batches <= 2) return;
         const i64 all = (i64)lines * beams * batches, slots = (i64)sm_count() * 7 * kScanWarps;
-        const int least = beams > 8 ? beams / 4 : 2, most = 24;
+        const int least = beams > 8 ? beams / 4 : 2, most = 16;
         int per = all >= slots * most ? most : (int)(all / slots) + 1;
         if (per < least) per = least;
         if (per < (batches + 127) / 128) per = (batches + 127) / 128;
@@ -898,10 +916,14 @@ int select(const void *logits, i64 ld, const float *scores, const uint8_t *finis
            int eos, float *out_scores, int32_t *out_tokens, int32_t *out_parents, uint8_t *out_finished,
            void *workspace, cudaStream_t st) {
     const Plan plan(lines, beams, vocab, (int)sizeof(T));
-    const int warps = beams < 16 ? beams : 16;
     if (plan.segs == 0) {
         static std::atomic<unsigned long long> sized{0};
         if (const int e = allow_smem(select_line_kernel<T>, sized)) return e;
+        // More lines than SMs: 8 warps, so that several CTAs fit on a SM and one
+        // picks while others read (512 lines of 32 beams, 130 f32: 72 us with 8
+        // warps, 82 with 16; of 16 beams, 200 f16: 31 and 37); few lines are
+        // quickest with a warp for every row.
+        const int most = lines > sm_count() ? 8 : 16, warps = beams < most ? beams : most;
         const size_t smem = sizeof(Merge) + sizeof(Scan) * warps + sizeof(Found) * beams;
         select_line_kernel<T><<<lines, warps * 32, smem, st>>>(static_cast<const T *>(logits), ld, scores, finished,
                                                                beams, vocab, eos, out_scores, out_tokens, out_parents,
@@ -909,6 +931,7 @@ int select(const void *logits, i64 ld, const float *scores, const uint8_t *finis
         return launched();
     }
     static std::atomic<unsigned long long> sized{0};
+    const int warps = beams < 16 ? beams : 16;
     Found *found = static_cast<Found *>(workspace);
     const i64 units = (i64)lines * beams * plan.segs;
     select_scan_kernel<T><<<(unsigned)((units + kScanWarps - 1) / kScanWarps), kScanWarps * 32, 0, st>>>(

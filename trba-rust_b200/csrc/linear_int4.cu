@@ -42,7 +42,8 @@ namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
 
-// One warp a group: scale = max |w| / 7, code = 8 + round(w / scale).
+// One warp a group: scale = max |w| / 7, code = 8 + round(w / scale).  Runs
+// once a layer; bound by reading the f32 weights twice.
 __global__ void __launch_bounds__(256) int4_quantize_kernel(const float *__restrict__ w, int in, int out, int group,
                                                             int groups, uint8_t *__restrict__ codes, i64 pitch,
                                                             float *__restrict__ scales) {
@@ -69,7 +70,9 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const float *__restr
 }
 
 // Natural codes [out][pitch] and scales [out][groups] -> the layout above: a
-// warp a block, a lane 8 words of codes, then the scales.
+// warp a block, a lane 8 words of codes, then the scales.  Runs once a layer;
+// each word is one read where the rows allow it.  Making a 16384 x 16384 layer
+// takes 0.49 ms with the copies of its arguments.
 template <class S>
 __global__ void __launch_bounds__(256) int4_layout_kernel(const uint8_t *__restrict__ codes, i64 pitch,
                                                           const S *__restrict__ scales, i64 ld_scales, int in, int out,
@@ -130,10 +133,12 @@ __global__ void __launch_bounds__(256) int4_natural_kernel(const uint8_t *__rest
 }
 
 // ----------------------------------------------------------------- forward --
-constexpr int kPair = 2;  // blocks of a stage of the few-columns kernel
-// Few columns need few registers: 32 warps hide more latency; two stages of
-// two blocks each keep 64 KB in flight a SM.
-constexpr int kFewWarps = 32, kManyWarps = 16;
+// Few columns: 16 warps with three stages of two blocks each keep 64 KB in
+// flight a SM while they work on 32.  8 f16 rows through 16384 x 8192 take 31 us
+// so and 37 with 32 warps and two stages (one row: 25 and 27); a fourth stage,
+// or stages of one block, gain nothing.
+constexpr int kPair = 2, kFewStages = 3;
+constexpr int kFewWarps = 16, kManyWarps = 16;
 constexpr int many_depth(int nt) { return nt > 3 && nt <= 5 ? 4 : 3; }
 constexpr int many_blocks(int nt) { return nt <= 3 ? 2 : 1; }  // of a warp in a step
 
@@ -144,9 +149,12 @@ constexpr int many_blocks(int nt) { return nt <= 3 ? 2 : 1; }  // of a warp in a
 // exact in all types, and a group's sum is accumulated in f32 before its
 // scale multiplies it.
 //
-// What bounds it: at few rows, reading the codes (half a byte a weight).  The
-// warp-level mma is enough for that: a 1 KB block of codes costs 8 mma per
-// eight columns and about 75 integer and conversion instructions.
+// What bounds it: at few rows, reading the codes (half a byte a weight) and
+// turning them into floats.  The warp-level mma is enough for that: a 1 KB block
+// of codes costs 8 mma per eight columns and about 75 integer and conversion
+// instructions, which take as long as reading the block.  tcgen05 would take
+// the codes from shared memory as floats, four times as many bytes written
+// and read there, and its 128-row tiles would be one to eight columns wide.
 //
 // One CTA a SM for the whole product, its tiles a contiguous share of all of
 // them, its warps `wn` tiles side by side by `wk` parts of the inputs.  The
@@ -159,7 +167,7 @@ struct Args {
     uint4 *frags;  // [row block][chunk][word][column tile][lane]
     i64 ldx, ldy;
     int in, out, rows, dtype;
-    int tiles, chunks, gpc;
+    int tiles, chunks;
     int wn;              // wk = warps / wn
     int cs;              // many columns: CTAs that share a tile's chunks
     int slab;            // few columns: chunks whose activations are staged at once
@@ -307,7 +315,8 @@ __device__ __forceinline__ void store8(const Args &a, const Eight &v, uint8_t *d
 
 // The activations as B fragments: a thread eight of a row (three 16-byte
 // pieces for f32).  Columns go row by row, an f32 row's three next to each
-// other; what stands in the columns behind the last does not matter.
+// other; what stands in the columns behind the last does not matter.  2 to 4 us,
+// bound by its launch; the weights of the next kernel load meanwhile.
 __global__ void __launch_bounds__(256) int4_fragments_kernel(const __grid_constant__ Args a, int nt) {
     const int split = a.dtype == TRBA_F32 ? 3 : 1;
     const int row0 = blockIdx.y * a.block_rows, rows = min(a.block_rows, a.rows - row0);
@@ -403,6 +412,11 @@ __device__ __forceinline__ void write_tile(const Args &a, int tile, int row0, in
 // while activations are staged, sums are joined and outputs written.
 // Activations are staged in slabs of inputs, each once a CTA, all tiles
 // running over one slab before the next; sums wait in shared memory in between.
+// One bf16 row through 16384 x 16384, groups of 128: 31 us, 4.5 TB/s of codes
+// and scales, 0.68 of a copy's rate; one f16 row through 16384 x 8192, groups of
+// 32: 25 us.  With data, tensor pipe (26%) and issue slots (64%) all below their
+// limits, what is left is the wait of a warp for its own ring.  Sharing out the
+// tiles so that a CTA has all inputs of its outputs needs no sums in memory.
 template <bool F16, class S, int WG>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -414,7 +428,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
     const int rows = a.rows, split = a.dtype == TRBA_F32 ? 3 : 1;
     constexpr int kBlock = 1024 + 16 * (4 / WG) * (int)sizeof(S), kSlot = kPair * kBlock;
     const int pitch = a.slab * 256 + 64;  // 64 mod 128: eight lanes' 16-byte reads meet 32 different banks
-    const int ring = warp * 2 * kSlot;    // offsets in shared memory
+    const int ring = warp * kFewStages * kSlot;    // offsets in shared memory
 
     // the stream of this warp's stages: for each slab, for each of its tiles, its part of the chunks
     int ptile = t0 - a.wn, pslab = t0 < t1 ? 0 : a.chunks, left = 0;
@@ -434,17 +448,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
             psrc = a.blocks + ((i64)ptile * a.chunks + c) * kBlock + lane * 16;
         }
         if (left > 0) {
-            const int bytes = left > 1 ? kSlot : kBlock;
+            const int bytes = min(left, kPair) * kBlock;
 #pragma unroll
             for (int j = 0; j < (kSlot + 511) / 512; ++j)
                 if (lane * 16 < bytes - 512 * j) cp16(dst + 512 * j, psrc + 512 * j);
             psrc += kSlot;
             left -= kPair;
-            dst = 2 * ring_s + kSlot - dst;
+            dst = dst == ring_s + (kFewStages - 1) * kSlot ? ring_s : dst + kSlot;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    issue();
+#pragma unroll 1
+    for (int i = 0; i < kFewStages - 1; ++i) issue();
 
     // a column of mma depends on its own activations alone: lanes behind the
     // last column read it again
@@ -472,7 +487,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
         for (int u = t0; u < t1; u += a.wn, turn ^= 1) {
             float tot[NT][4] = {};
             for (int xo = cb * 256; xo < ce * 256; xo += kPair * 256) {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
                 __syncwarp();
                 issue();
 #pragma unroll
@@ -483,7 +498,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
                         [&](int w, int) { return *reinterpret_cast<const uint4 *>(smem + xcol + xo + p * 256 + w * 64); },
                         tot, lane);
                 }
-                blk = 2 * ring + kSlot - blk;
+                blk = blk == ring + (kFewStages - 1) * kSlot ? ring : blk + kSlot;
             }
             // join the wk_n warps of the tile; two buffers in turn, so that a
             // buffer is written again only after the next tile's barrier
@@ -518,7 +533,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
 // (read by all warps) and each warp's block.  Staging the activations as
 // fragments in memory first makes their copies plain and aligned; per SM and
 // step they are read once for wn tiles.  From about 24 columns on the tensor
-// pipe bounds it (a 16 x 8 x 16 mma takes 2.4 cycles a SM).
+// pipe's floor is above memory's (a 16 x 8 x 16 mma takes 2.4 cycles a SM).
+// 40 f16 rows through 50001 x 4099, groups of 32: 95 us with the fragments, 1.3
+// TB/s of codes and scales and 173 TFLOP/s; tensor pipe 37%, issue slots 48%: bound
+// by the shared-memory reads and conversions between the barriers of a step.  16
+// rows through 16384 x 8192: 35 us, 64 rows 80 us.
 template <bool F16, class S, int WG, int NT>
 __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -739,7 +758,7 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
     a.x = x, a.y = y, a.ldx = ldx, a.ldy = ldy;
     a.frags = static_cast<uint4 *>(workspace);
     a.in = l->in, a.out = l->out, a.rows = rows, a.dtype = dtype;
-    a.tiles = l->tiles, a.chunks = l->chunks, a.gpc = l->gpc;
+    a.tiles = l->tiles, a.chunks = l->chunks;
     const bool scale_f16 = l->scale_dtype == TRBA_F16;
     const int nt = shape.nt, blocks_y = shape.blocks;
     a.block_rows = shape.block_rows;
@@ -769,7 +788,7 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
         }
     } else {
         const int cols = rows * (dtype == TRBA_F32 ? 3 : 1);
-        const int ring = kFewWarps * 2 * kPair * l->block;
+        const int ring = kFewWarps * kFewStages * kPair * l->block;
         const auto x_bytes = [&](int chunks) { return ((i64)cols * (chunks * 256 + 64) + 127) & ~127ll; };
         for (ctas = a.tiles < sm_count() ? a.tiles : sm_count();; ctas = ctas * 2 < a.tiles ? ctas * 2 : a.tiles) {
             const int share = (a.tiles + ctas - 1) / ctas;  // tiles of a CTA, at most
@@ -778,7 +797,6 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
             i64 best = -1;
             int red = 0;
             for (int wn = kFewWarps; wn >= 1; wn >>= 1) {
-                if (wn == 16) continue;  // named barriers 1 + wn go up to 15
                 const int wk = kFewWarps / wn, bytes = 2 * wn * (wk - 1) * 512;
                 const i64 steps = (share + wn - 1) / wn;
                 const i64 cost = steps * (4 * ((a.chunks + wk - 1) / wk) + (wk > 1 ? 4 + wk : 0));
