@@ -412,9 +412,9 @@ __device__ __forceinline__ void write_tile(const Args &a, int tile, int row0, in
 // while activations are staged, sums are joined and outputs written.
 // Activations are staged in slabs of inputs, each once a CTA, all tiles
 // running over one slab before the next; sums wait in shared memory in between.
-// One bf16 row through 16384 x 16384, groups of 128: 31 us, 4.5 TB/s of codes
-// and scales, 0.68 of a copy's rate; one f16 row through 16384 x 8192, groups of
-// 32: 25 us.  With data, tensor pipe (26%) and issue slots (64%) all below their
+// One bf16 row through 16384 x 16384, groups of 128: 31.5 us, 4.4 TB/s of codes
+// and scales, 0.67 of a copy's rate; one f16 row through 16384 x 8192, groups of
+// 32: 20 us.  With data, tensor pipe (25%) and issue slots (57%) all below their
 // limits, what is left is the wait of a warp for its own ring.  Sharing out the
 // tiles so that a CTA has all inputs of its outputs needs no sums in memory.
 template <bool F16, class S, int WG>
