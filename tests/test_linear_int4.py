@@ -216,6 +216,29 @@ def test_layer_with_its_own_memory(lib, cuda):
 
 
 @pytest.mark.gpu
+def test_layer_dropped_while_another_stream_reads_it(cuda):
+    """The memory of a layer made on one stream is not handed out again before
+    a call on another is done with it."""
+    made, used = torch.cuda.Stream(), torch.cuda.Stream()
+    kept, q, s, b = layer(2000, 4096, 128, "f16", 5)
+    x = torch.randn(24, 4096, device="cuda").half()
+    want = kept.forward(x)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(made):
+            lin = LinearInt4.from_codes(q, s, in_features=4096, group=128, bias=b)
+            size = lin.storage.numel()
+        used.wait_stream(made)
+        ys = [lin.forward(x, stream=used) for _ in range(20)]
+        del lin
+        with torch.cuda.stream(made):
+            junk = torch.empty(size, dtype=torch.uint8, device="cuda").fill_(0x77)
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in ys)
+        del junk
+
+
+@pytest.mark.gpu
 def test_forward_refusals(lib, cuda):
     lin, *_ = layer(8, 40, 32, "f32", 0)
     x = torch.zeros(2, 40, device="cuda")
