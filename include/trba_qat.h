@@ -103,8 +103,11 @@ int trba_model_infer_host(trba_model *m, const int8_t *img, int batch, int32_t *
  * tokens before eos, then pad, best beam first; lengths (device, [batch,
  * beams]); scores (device, [batch, beams] f32 log probabilities, or NULL); a
  * slot that holds no sequence has score -inf.  The model keeps the search's
- * buffers; the first call that needs more than any before allocates (and
- * waits), so make it before a capture. */
+ * buffers: a call that needs more than any before allocates them, so make one
+ * of that size before a capture (inside one it returns -4, and nothing has
+ * run).  Buffers are kept until the model is destroyed; a graph that holds
+ * this call may be replayed whatever calls follow its capture, in their
+ * stream order. */
 int trba_model_infer_beam(trba_model *m, const int8_t *img, int batch, int beams, int32_t *sequences,
                           int32_t *lengths, float *scores, void *stream);
 /* The same with host buffers.  Synchronises. */

@@ -105,3 +105,38 @@ def test_expert_runner_decodes_with_beams(lib, cuda):
     with pytest.raises(RuntimeError, match="infer_beam"):
         run.model.infer_beam(dev, 2)  # more lines than the model was made for
     run.close()
+
+
+def test_captured_search_outlives_growth(lib, cuda):
+    """A search captured into a graph replays on buffers of its own size after
+    calls that needed more; the first call of a size is refused in a capture."""
+    import torch
+    ocfg, _, gm = _pair(dict(img_w=64, max_len=4), 8, seed=78, train_steps=1)
+    imgs = [torch.from_numpy(np.ascontiguousarray(so.make_batch(ocfg, 8, seed=s)[0])).cuda() for s in (5, 6)]
+    held = lambda: int(lib.trba_model_device_bytes(gm.h))  # noqa: E731
+    none = held()
+    want = [gm.infer_beam(x[:4], 3) for x in imgs]
+    small = held()
+    torch.cuda.synchronize()
+    buf = imgs[0][:4].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gm.infer_beam(buf, 3)
+    assert held() == small
+    wide = gm.infer_beam(imgs[1], 8)
+    # the small call's block is still there, beside one for (8 x 8) / (4 x 3) as many beams
+    assert small > none and held() - small >= 5 * (small - none)
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other):
+        kept = buf + 0
+        with pytest.raises(RuntimeError, match="before its capture"):
+            gm.infer_beam(imgs[0], 32)
+    for x, w in zip(imgs, want):
+        buf.copy_(x[:4])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, w))
+    other.replay()
+    assert torch.equal(kept, buf)
+    assert all(torch.equal(a, b) for a, b in zip(gm.infer_beam(imgs[1], 8), wide))
+    assert lib.trba_last_error() == 0, lib.trba_last_error_string()

@@ -268,8 +268,11 @@ struct trba_model {
     int gkey_batch = 0, gkey_probe = -1;
     long long graph_kernels = 0;  // kernel launches recorded in the step graph
     Probe probe;
-    uint8_t *beam_mem = nullptr;  // buffers of the beam search, grown when a call needs more
-    size_t beam_bytes = 0;
+    // Buffers of the beam search: a call that needs more than the last block
+    // has gets another, at least twice as large.  Earlier blocks stay, because
+    // captured graphs hold their addresses.
+    std::vector<uint8_t *> beam_mem;
+    size_t beam_bytes = 0, beam_total = 0;  // of the last block, of all
 };
 
 namespace {
@@ -1632,7 +1635,7 @@ void trba_model_destroy(trba_model *m) {
     if (m->gstream) cudaStreamDestroy(m->gstream);
     for (cudaEvent_t e : m->probe.ev) cudaEventDestroy(e);
     if (m->probe.stamps) cudaFree(m->probe.stamps);
-    cudaFree(m->beam_mem);
+    for (uint8_t *p : m->beam_mem) cudaFree(p);
     delete m;
 }
 
@@ -1688,7 +1691,7 @@ const float *trba_model_loss_dev(const trba_model *m) { return m ? m->loss.get()
 const int32_t *trba_model_step_tokens_dev(const trba_model *m) { return m ? m->step_tokens.get() : nullptr; }
 long long trba_model_step_count(const trba_model *m) { return m ? m->t : -1; }
 long long trba_model_device_bytes(const trba_model *m) {
-    return m ? (long long)(m->arena.used + m->zarena.used) : -1;
+    return m ? (long long)(m->arena.used + m->zarena.used + m->beam_total) : -1;
 }
 
 long long trba_model_running_stats_count(const trba_model *m) {
@@ -1761,23 +1764,27 @@ int trba_model_infer_beam(trba_model *m, const int8_t *img, int batch, int beams
     cudaStream_t st = as_stream(stream);
     const size_t need = BeamBuffers(nullptr, m, batch, beams).used;
     if (need > m->beam_bytes) {
-        cudaFree(m->beam_mem);  // waits for what still uses it
-        m->beam_mem = nullptr;
-        m->beam_bytes = 0;
-        const cudaError_t e = cudaMalloc(&m->beam_mem, need);
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        TRBA_CHECK(cudaStreamIsCapturing(st, &capturing));
+        if (capturing != cudaStreamCaptureStatusNone) return -4;
+        const size_t bytes = std::max(need, 2 * m->beam_bytes);
+        uint8_t *mem = nullptr;
+        const cudaError_t e = cudaMalloc(&mem, bytes);
         if (e != cudaSuccess) {
             cudaGetLastError();
             report_error(__FILE__, __LINE__, "trba_model_infer_beam: device allocation failed", (int)e);
             return (int)e;
         }
-        m->beam_bytes = need;
+        m->beam_mem.push_back(mem);
+        m->beam_bytes = bytes;
+        m->beam_total += bytes;
     }
     Ctx c{m, st, batch, m->P.get(), m->G.get()};
     c.eval = true;
     m->last_B = batch;
     TRBA_CHECK(cudaMemsetAsync(m->zarena.base, 0, m->zarena.used, st));
     cnn_forward(c, img);
-    const int rc = head_infer_beam(c, BeamBuffers(m->beam_mem, m, batch, beams), beams, sequences, lengths, scores);
+    const int rc = head_infer_beam(c, BeamBuffers(m->beam_mem.back(), m, batch, beams), beams, sequences, lengths, scores);
     return rc ? rc : cuda_status();
 }
 

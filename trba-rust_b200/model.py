@@ -212,8 +212,10 @@ class QatModel:
         seq = torch.empty((b, beams, self.cfg.steps), dtype=torch.int32, device=img.device)
         lengths = torch.empty((b, beams), dtype=torch.int32, device=img.device)
         scores = torch.empty((b, beams), dtype=torch.float32, device=img.device)
-        self._check(self.L.trba_model_infer_beam(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lengths), _ptr(scores),
-                                                 stream), "infer_beam")
+        rc = self.L.trba_model_infer_beam(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lengths), _ptr(scores), stream)
+        if rc == -4:
+            raise RuntimeError("infer_beam: a call of this size has to come before its capture (it allocates buffers)")
+        self._check(rc, "infer_beam")
         return seq, lengths, scores
 
     def infer_beam_host(self, img, beams: int, stream=None) -> list:
