@@ -140,3 +140,17 @@ def test_captured_search_outlives_growth(lib, cuda):
     assert torch.equal(kept, buf)
     assert all(torch.equal(a, b) for a, b in zip(gm.infer_beam(imgs[1], 8), wide))
     assert lib.trba_last_error() == 0, lib.trba_last_error_string()
+
+
+def test_search_keeps_no_more_than_it_uses(lib, cuda):
+    """Device memory of a first search: two sets of h and c, logits, scores,
+    the history's tokens and parents, finished (parts of 256 bytes; 130 classes
+    need no workspace)."""
+    import torch
+    ocfg, _, gm = _pair(dict(img_w=64, max_len=4), 8, seed=78, train_steps=0)
+    before = int(lib.trba_model_device_bytes(gm.h))
+    img = torch.from_numpy(np.ascontiguousarray(so.make_batch(ocfg, 8, seed=5)[0])).cuda()
+    gm.infer_beam(img[:4], 3)
+    rows = 4 * 3
+    parts = [rows * ocfg.hidden * 4] * 4 + [rows * ocfg.classes * 4, rows * 4] + [rows * ocfg.steps * 4] * 2 + [rows]
+    assert int(lib.trba_model_device_bytes(gm.h)) - before == sum(-(-p // 256) * 256 for p in parts)

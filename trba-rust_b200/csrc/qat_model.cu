@@ -1321,7 +1321,7 @@ __global__ void beam_start_kernel(float *scores, uint8_t *finished, int n, int b
 struct BeamBuffers {
     size_t used = 0;
     float *h[2], *c[2], *logits, *scores;
-    int32_t *tokens, *parents, *sequences, *lengths;
+    int32_t *tokens, *parents;
     uint8_t *finished;
     void *work;
     long long work_bytes;
@@ -1336,7 +1336,7 @@ struct BeamBuffers {
         const auto i = [&](i64 n) { return reinterpret_cast<int32_t *>(take(n * 4)); };
         for (int k = 0; k < 2; ++k) h[k] = f(rows * H), c[k] = f(rows * H);
         logits = f(rows * V), scores = f(rows);
-        tokens = i(S * rows), parents = i(S * rows), sequences = i(S * rows), lengths = i(rows);
+        tokens = i(S * rows), parents = i(S * rows);
         finished = take(rows);
         work_bytes = trba_beam_select_workspace(TRBA_F32, lines, beams, (int)V);
         work = take(work_bytes);
