@@ -154,3 +154,58 @@ def test_search_keeps_no_more_than_it_uses(lib, cuda):
     rows = 4 * 3
     parts = [rows * ocfg.hidden * 4] * 4 + [rows * ocfg.classes * 4, rows * 4] + [rows * ocfg.steps * 4] * 2 + [rows]
     assert int(lib.trba_model_device_bytes(gm.h)) - before == sum(-(-p // 256) * 256 for p in parts)
+
+
+def test_search_on_another_stream(lib, cuda):
+    """Results belong to the stream that writes them: their memory, once
+    dropped, is not handed to the current one."""
+    import ctypes as C
+    import torch
+    ocfg, _, gm = _pair(dict(img_w=64, max_len=4), 8, seed=78, train_steps=1)
+    img = torch.from_numpy(np.ascontiguousarray(so.make_batch(ocfg, 8, seed=5)[0])).cuda()
+    want = gm.infer_beam(img, 3)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    for handle in (st.cuda_stream, C.c_void_p(st.cuda_stream)):
+        got = gm.infer_beam(img, 3, stream=handle)
+        st.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        torch.cuda.synchronize()
+        like, ptrs = [(t.shape, t.dtype) for t in got], {t.data_ptr() for t in got}
+        del got
+        kept = [torch.empty(s, dtype=d, device="cuda") for _ in range(40) for s, d in like]
+        assert not ptrs & {t.data_ptr() for t in kept}
+        with torch.cuda.stream(st):
+            assert ptrs & {torch.empty(s, dtype=d, device="cuda").data_ptr() for s, d in like}
+    got = gm.infer_beam(img, 3, stream=0)  # the default stream's handle
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert lib.trba_last_error() == 0
+
+
+def test_expert_runner_on_another_stream(lib, cuda):
+    """The stream waits for images that the current one is still to write."""
+    import torch
+    import trba_b200.mope as mp
+    run = mp.ExpertRunner(mp.default_experts()[1], batch=5, seed=11)
+    ocfg = so.Config(img_w=96, max_len=5)
+    img = torch.from_numpy(np.ascontiguousarray(so.make_batch(ocfg, 12, seed=31)[0])).cuda()
+    search, seen = run.model.infer_beam, []
+
+    def scores(imgs, stream=None):  # (an untrained model's tokens hardly depend on the images; its scores do)
+        seen.clear()
+        lists = run.decode_beam(imgs, 4, stream=stream)
+        return lists, torch.cat([r[2] for r in seen]).cpu().numpy()
+
+    run.model.infer_beam = lambda *a, **k: seen.append(search(*a, **k)) or seen[-1]
+    want, want_s = scores(img)
+    _, zero_s = scores(torch.zeros_like(img))
+    assert (zero_s != want_s).all()  # what it would read otherwise
+    st = torch.cuda.Stream()
+    late, busy = torch.zeros_like(img), torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(20):  # several ms of work ahead of the images
+        busy = torch.tanh(busy @ busy)
+    late.copy_(img)
+    got, got_s = scores(late, st.cuda_stream)
+    assert got == want and np.array_equal(got_s, want_s)
+    run.close()

@@ -66,6 +66,15 @@ def _ptr(a):
     return C.c_void_p(a.data_ptr())  # torch tensor
 
 
+def _torch_stream(handle, device):
+    """torch's view of a raw stream handle; None: the current stream."""
+    import torch
+    if handle is None:
+        return torch.cuda.current_stream(device)
+    raw = handle.value if isinstance(handle, C.c_void_p) else int(handle)
+    return torch.cuda.ExternalStream(raw, device) if raw else torch.cuda.default_stream(device)
+
+
 class QatModel:
     def __init__(self, cfg: Config):
         self.cfg = cfg
@@ -202,17 +211,19 @@ class QatModel:
         """Beam search over device images [B, 3, H, W] int8: (sequences [B,
         beams, max_len+1] int32 with pad behind each one's end, lengths [B,
         beams], scores [B, beams] float32) as device tensors, best beam first.
-        Runs on torch's current stream unless a stream handle is given; the
-        caller then orders its use of the results after that stream."""
+        Runs on torch's current stream, or on a raw stream handle, to which the
+        results then belong; the caller makes that stream wait for the images,
+        keeps them, and orders its use of the results after it."""
         import torch
         self._check_beams(beams)
-        if stream is None:
-            stream = torch.cuda.current_stream(img.device).cuda_stream
+        st = _torch_stream(stream, img.device)
         b = int(img.shape[0])
-        seq = torch.empty((b, beams, self.cfg.steps), dtype=torch.int32, device=img.device)
-        lengths = torch.empty((b, beams), dtype=torch.int32, device=img.device)
-        scores = torch.empty((b, beams), dtype=torch.float32, device=img.device)
-        rc = self.L.trba_model_infer_beam(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lengths), _ptr(scores), stream)
+        with torch.cuda.stream(st):
+            seq = torch.empty((b, beams, self.cfg.steps), dtype=torch.int32, device=img.device)
+            lengths = torch.empty((b, beams), dtype=torch.int32, device=img.device)
+            scores = torch.empty((b, beams), dtype=torch.float32, device=img.device)
+        rc = self.L.trba_model_infer_beam(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lengths), _ptr(scores),
+                                          st.cuda_stream)
         if rc == -4:
             raise RuntimeError("infer_beam: a call of this size has to come before its capture (it allocates buffers)")
         self._check(rc, "infer_beam")

@@ -119,8 +119,13 @@ class ExpertRunner:
 
     def decode_beam(self, imgs, beams: int, stream=None) -> list[list[int]]:
         """Token lists of device images, the best of `beams` beams of each line
-        (which do not depend on the decoding batch, unlike the greedy rule's)."""
+        (which do not depend on the decoding batch, unlike the greedy rule's).
+        A raw `stream` handle waits for what torch's current stream has queued."""
         out = []
+        if stream is not None:
+            import torch
+            from .model import _torch_stream
+            _torch_stream(stream, imgs.device).wait_stream(torch.cuda.current_stream(imgs.device))
         for s in range(0, imgs.shape[0], self.batch):
             seq, lengths, _ = self.model.infer_beam(imgs[s:s + self.batch], beams, stream=stream)
             if stream is not None:
