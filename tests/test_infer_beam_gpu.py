@@ -209,3 +209,22 @@ def test_expert_runner_on_another_stream(lib, cuda):
     got, got_s = scores(late, st.cuda_stream)
     assert got == want and np.array_equal(got_s, want_s)
     run.close()
+
+
+def test_images_that_are_views(lib, cuda):
+    """Every other image of a batch, images with a gap between rows, and the
+    lines as plain rows of bytes."""
+    import torch
+    ocfg, _, gm = _pair(dict(img_w=64, max_len=4), 8, seed=78, train_steps=1)
+    img = torch.from_numpy(np.ascontiguousarray(so.make_batch(ocfg, 8, seed=5)[0])).cuda().view(8, 3, 32, 64)
+    want = gm.infer_beam(img[::2].clone(), 3)
+    room = torch.zeros(4, 3, 32, 80, dtype=torch.int8, device="cuda")
+    room[..., :64] = img[::2]
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for view in (img[::2], room[..., :64], img[::2].reshape(4, -1)):
+        assert all(torch.equal(a, b) for a, b in zip(gm.infer_beam(view, 3), want))
+        torch.cuda.synchronize()
+        got = gm.infer_beam(view, 3, stream=st.cuda_stream)
+        st.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

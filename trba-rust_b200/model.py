@@ -207,6 +207,12 @@ class QatModel:
         if not 1 <= beams <= 32:
             raise ValueError(f"1 to 32 beams are supported, got {beams}")
 
+    def _check_images(self, img):
+        per, shape = 3 * self.cfg.img_h * self.cfg.img_w, tuple(img.shape)
+        if not shape or int(np.prod(shape[1:])) != per:
+            raise ValueError(f"images {shape} do not have 3 x {self.cfg.img_h} x {self.cfg.img_w} values a line")
+        return shape[0]
+
     def infer_beam(self, img, beams: int, stream=None):
         """Beam search over device images [B, 3, H, W] int8: (sequences [B,
         beams, max_len+1] int32 with pad behind each one's end, lengths [B,
@@ -216,9 +222,14 @@ class QatModel:
         keeps them, and orders its use of the results after it."""
         import torch
         self._check_beams(beams)
+        if not isinstance(img, torch.Tensor) or img.dtype != torch.int8:
+            raise TypeError("images must be an int8 torch tensor")
+        b = self._check_images(img)
+        if not img.is_cuda or img.device.index != torch.cuda.current_device():
+            raise ValueError(f"images are on {img.device}, not on the current CUDA device")
         st = _torch_stream(stream, img.device)
-        b = int(img.shape[0])
         with torch.cuda.stream(st):
+            img = img.contiguous()
             seq = torch.empty((b, beams, self.cfg.steps), dtype=torch.int32, device=img.device)
             lengths = torch.empty((b, beams), dtype=torch.int32, device=img.device)
             scores = torch.empty((b, beams), dtype=torch.float32, device=img.device)
@@ -234,7 +245,7 @@ class QatModel:
         score), best first, without the slots that hold no sequence."""
         self._check_beams(beams)
         img = np.ascontiguousarray(img, np.int8)
-        b = int(img.shape[0])
+        b = self._check_images(img)
         seq = np.empty((b, beams, self.cfg.steps), np.int32)
         lens, scores = np.empty((b, beams), np.int32), np.empty((b, beams), np.float32)
         self._check(self.L.trba_model_infer_beam_host(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lens), _ptr(scores),
