@@ -84,6 +84,8 @@ class QatModel:
         if not self.h:
             raise RuntimeError("trba_model_create failed: " + self.L.trba_last_error_string().decode())
         self.n_params = int(self.L.trba_model_param_count(self.h))
+        import torch
+        self.device = torch.cuda.current_device()  # the model's memory is there
 
     def close(self):
         if getattr(self, "h", None):
@@ -225,8 +227,11 @@ class QatModel:
         if not isinstance(img, torch.Tensor) or img.dtype != torch.int8:
             raise TypeError("images must be an int8 torch tensor")
         b = self._check_images(img)
-        if not img.is_cuda or img.device.index != torch.cuda.current_device():
-            raise ValueError(f"images are on {img.device}, not on the current CUDA device")
+        if img.device != torch.device("cuda", self.device):
+            raise ValueError(f"images are on {img.device}, the model is on cuda:{self.device}")
+        if torch.cuda.current_device() != self.device:
+            with torch.cuda.device(self.device):
+                return self.infer_beam(img, beams, stream)
         st = _torch_stream(stream, img.device)
         with torch.cuda.stream(st):
             img = img.contiguous()
@@ -243,13 +248,15 @@ class QatModel:
     def infer_beam_host(self, img, beams: int, stream=None) -> list:
         """Beam search over host images: for every line a list of (tokens,
         score), best first, without the slots that hold no sequence."""
+        import torch
         self._check_beams(beams)
         img = np.ascontiguousarray(img, np.int8)
         b = self._check_images(img)
         seq = np.empty((b, beams, self.cfg.steps), np.int32)
         lens, scores = np.empty((b, beams), np.int32), np.empty((b, beams), np.float32)
-        self._check(self.L.trba_model_infer_beam_host(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lens), _ptr(scores),
-                                                      stream), "infer_beam_host")
+        with torch.cuda.device(self.device):
+            rc = self.L.trba_model_infer_beam_host(self.h, _ptr(img), b, beams, _ptr(seq), _ptr(lens), _ptr(scores), stream)
+        self._check(rc, "infer_beam_host")
         return [[(seq[i, k, :lens[i, k]].tolist(), float(scores[i, k])) for k in range(beams)
                  if scores[i, k] > -np.inf] for i in range(b)]
 
