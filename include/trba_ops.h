@@ -68,9 +68,9 @@ long long trba_linear_int8_param_count(const trba_linear_int8 *l);
  * enter them with all their bits) and y is rounded once, to the type of x.
  *
  * A layer keeps its weights on the device that was current when it was
- * created; forward is refused on another one.  forward only launches kernels:
- * it may be captured into CUDA graphs and, each call with a workspace of its
- * own, run on several streams at once. */
+ * created; forward and get are refused on another one.  forward only
+ * launches kernels: it may be captured into CUDA graphs and, each call with a
+ * workspace of its own, run on several streams at once. */
 typedef struct trba_linear_int4 trba_linear_int4;
 /* in and out are 1 .. 2^30.  From f32 weights [out, in] row-major and bias [out] (NULL = zeros), both on
  * the host.  scale = max |w| of the group / 7 (1 when all are zero), code - 8

@@ -968,6 +968,9 @@ int trba_linear_int4_forward(const trba_linear_int4 *l, const void *x, int dtype
 
 int trba_linear_int4_get(const trba_linear_int4 *l, uint8_t *codes, float *scales, float *bias) {
     if (!l) return -1;
+    int dev = -1;
+    cudaGetDevice(&dev);
+    TRBA_REQUIRE_RET(dev == l->device, "trba_linear_int4_get: the layer is on another device", -1);
     cudaError_t e = cudaDeviceSynchronize();
     if (codes && e == cudaSuccess) {
         const size_t n = (size_t)l->out * (((size_t)l->in + 1) / 2);

@@ -253,7 +253,9 @@ class LinearInt4:
         n, g = self.out_features, -(-self.in_features // self.group)
         q, s = np.empty((n, -(-self.in_features // 2)), np.uint8), np.empty((n, g), np.float32)
         b = np.empty(n, np.float32)
-        if self.L.trba_linear_int4_get(self.h, _p(q), _p(s), _p(b)) != 0:
+        with self.torch.cuda.device(self.device):
+            rc = self.L.trba_linear_int4_get(self.h, _p(q), _p(s), _p(b))
+        if rc != 0:
             raise _err(self.L, "LinearInt4 state")
         return {"codes": q, "scales": s, "bias": b}
 
