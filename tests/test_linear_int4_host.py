@@ -47,3 +47,21 @@ def test_state_is_read_on_the_layers_device(monkeypatch):
     lin.in_features, lin.out_features, lin.group = 8, 4, 32
     monkeypatch.setattr(torch.cuda, "device", Device)
     assert lin.state()["codes"].shape == (4, 4) and used == [1] and now == [0]
+
+
+def test_a_closed_layer_is_refused():
+    """Before the library is called, which ends the process on a bad argument
+    unless it was told not to."""
+    class Lib:
+        def trba_linear_int4_destroy(self, h):
+            pass
+
+    from trba_b200 import decode
+    lin = LinearInt4.__new__(LinearInt4)
+    lin.L, lin.torch, lin.decode, lin.h = Lib(), torch, decode, 1
+    lin.device, lin.in_features, lin.out_features, lin.group = torch.device("cpu"), 8, 4, 32
+    lin.close()
+    lin.close()
+    for call in (lambda: lin.forward(torch.zeros(2, 8)), lin.state):
+        with pytest.raises(RuntimeError, match="closed"):
+            call()

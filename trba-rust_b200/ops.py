@@ -198,6 +198,8 @@ class LinearInt4:
         float16); leading dimensions of x are rows.  Runs on torch's current
         stream, or on `stream` (a torch.cuda.Stream)."""
         torch, decode = self.torch, self.decode
+        if not self.h:
+            raise RuntimeError("LinearInt4::forward: the layer is closed")
         if not isinstance(x, torch.Tensor) or out is not None:
             decode._check_tensors(x=x, out=out)
         code = decode.DTYPE_CODES.get(x.dtype)
@@ -250,6 +252,8 @@ class LinearInt4:
     def state(self) -> dict:
         """Host copies: codes [out, ceil(in / 2)] uint8, scales [out, groups]
         float32, bias [out] float32."""
+        if not self.h:
+            raise RuntimeError("LinearInt4 state: the layer is closed")
         n, g = self.out_features, -(-self.in_features // self.group)
         q, s = np.empty((n, -(-self.in_features // 2)), np.uint8), np.empty((n, g), np.float32)
         b = np.empty(n, np.float32)
