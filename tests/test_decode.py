@@ -125,6 +125,23 @@ def test_state_views():
         decode._state(torch.zeros(6, 4, 8, 6)[:, :, :5, ::2], torch.zeros(6, 4, 5, 3), 0)
 
 
+def test_too_many_states_are_refused_before_any_is_moved(lib):
+    """A state of too many parts behind a launch's worth of others."""
+    lib.trba_clear_error()
+    good, bad = (64, 1 << 20, 16, 16, 16, 1, 0, 0, 1, 0, 0), (64, 1 << 30, 1, 1 << 24, 1 << 23, 1 << 24, 2, 1, 1, 0, 0)
+    launches = lib.trba_launch_count()
+    for n, state in ((0, bad), (16, bad), (20, bad), (16, (64, 64, -1, 8, 8, 1, 0, 0, 1, 0, 0))):
+        views = (C.c_int64 * (11 * (n + 1)))(*good * n, *state)
+        assert lib.trba_beam_reorder(views, n + 1, C.c_void_p(64), 256, 1, None) == -1
+        assert lib.trba_launch_count() == launches
+        lib.trba_clear_error()
+    big, half = (torch.empty(256, n, dtype=torch.int8, device="meta") for n in (1 << 24, 1 << 23))
+    with pytest.raises(ValueError, match="too large"):
+        decode._state(big[:, ::2], half, 0)
+    assert decode._state(big[:, ::2][:100], half[:100], 0)[5] == 1 << 23
+    assert decode._state(big, big, 0)[2] == 1 << 24
+
+
 # --------------------------------------------------------------- GPU: select --
 # A score is off by at most: half a step of f32 (2^-24 of it); the f32
 # exponentials, whose relative error is 2^-22 (the function) + 2^-23 |t| (t

@@ -911,6 +911,19 @@ int allow_smem(K kernel, std::atomic<unsigned long long> &done) {
     return 0;
 }
 
+// The widest unit that every address of a state is a multiple of (0: none).
+int unit_of(const trba_beam_state &s) {
+    i64 bits = (i64)reinterpret_cast<uintptr_t>(s.src) | (i64)reinterpret_cast<uintptr_t>(s.dst) | s.bytes | s.src_row |
+               s.dst_row;
+    if (s.mid > 1) bits |= s.src_mid | s.dst_mid;
+    if (s.outer > 1) bits |= s.src_outer | s.dst_outer;
+    return !(bits & 15) ? 16 : !(bits & 7) ? 8 : !(bits & 3) ? 4 : 0;
+}
+// Pieces of a part of a row of a state, and the most that a launch counts: a
+// warp's next piece is still below 2^31.
+i64 pieces_of(const trba_beam_state &s, int vec) { return (s.bytes - 1) / (moves_of(vec) * 32 * (vec ? vec : 4)) + 1; }
+constexpr i64 kMostPieces = 2147483647ll - (1 << 20);
+
 template <class T>
 int select(const void *logits, i64 ld, const float *scores, const uint8_t *finished, int lines, int beams, int vocab,
            int eos, float *out_scores, int32_t *out_tokens, int32_t *out_parents, uint8_t *out_finished,
@@ -1011,6 +1024,9 @@ int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t
         TRBA_REQUIRE_RET((s.src && s.dst) || s.bytes == 0 || s.mid == 0 || s.outer == 0,
                          "trba_beam_reorder: null state", -1);
         TRBA_REQUIRE_RET(s.mid < (1ll << 31) && s.outer < (1ll << 31), "trba_beam_reorder: bad sizes", -1);
+        if (s.bytes == 0 || s.mid == 0 || s.outer == 0) continue;
+        const double all = (double)pieces_of(s, unit_of(s)) * (double)s.mid * (double)s.outer * (double)rows;
+        TRBA_REQUIRE_RET(all <= (double)kMostPieces, "trba_beam_reorder: a state is too large for one launch", -1);
     }
     int i = 0;
     while (i < n_states) {
@@ -1019,18 +1035,10 @@ int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t
         for (; i < n_states && v.n < kMaxStates; ++i) {
             const trba_beam_state &s = states[i];
             if (s.bytes == 0 || s.mid == 0 || s.outer == 0) continue;
-            // the widest unit that every address of the view is a multiple of
-            i64 bits = (i64)reinterpret_cast<uintptr_t>(s.src) | (i64)reinterpret_cast<uintptr_t>(s.dst) | s.bytes |
-                       s.src_row | s.dst_row;
-            if (s.mid > 1) bits |= s.src_mid | s.dst_mid;
-            if (s.outer > 1) bits |= s.src_outer | s.dst_outer;
             StateView &d = v.s[v.n];
-            d.vec = !(bits & 15) ? 16 : !(bits & 7) ? 8 : !(bits & 3) ? 4 : 0;
-            const i64 piece = moves_of(d.vec) * 32 * (d.vec ? d.vec : 4), per_row = (s.bytes - 1) / piece + 1;
-            const double all = (double)per_row * (double)s.mid * (double)s.outer * (double)rows;
-            TRBA_REQUIRE_RET(all < 2147483647.0, "trba_beam_reorder: a state is too large for one launch", -1);
-            const i64 mine = per_row * s.mid * s.outer * rows;
-            if (pieces + mine > 2147483647ll - (1 << 20)) break;  // the next launch takes it
+            d.vec = unit_of(s);
+            const i64 per_row = pieces_of(s, d.vec), mine = per_row * s.mid * s.outer * rows;
+            if (pieces + mine > kMostPieces) break;  // the next launch takes it
             d.first = (int)pieces;
             pieces += mine;
             bytes += s.bytes * s.mid * s.outer * rows;
@@ -1042,10 +1050,7 @@ int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t
             d.src_outer = s.src_outer, d.dst_outer = s.dst_outer;
             ++v.n;
         }
-        if (v.n == 0) {
-            TRBA_REQUIRE_RET(i >= n_states, "trba_beam_reorder: a state is too large for one launch", -1);
-            break;
-        }
+        if (v.n == 0) break;  // only empty states were left
         v.pieces = (int)pieces;
         // Rounds of CTAs even out the SMs' shares: 0.7 GB moved by 3 / 8 / 64
         // CTAs a SM takes 213 / 219 / 195 us, 21 MB 10.8 us up to 32 and 14 at 64.

@@ -22,6 +22,7 @@ import torch
 from .ffi import lib
 
 MAX_BEAMS = 32
+MOST_PARTS = 2 ** 31 - 1 - 2 ** 20  # contiguous parts of a state's rows (of at most 1024 bytes each)
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -198,6 +199,9 @@ def _state(src, dst, dim):
         raise ValueError(f"state of shape {tuple(shape)} and strides {src.stride()}: at most one gap before and one "
                          "after the beam dimension are supported; make it contiguous")
     o, om = outer[0] if outer else (1, 0, 0), inner[0] if inner else (1, 0, 0)
+    if ((nbytes - 1) // 1024 + 1) * om[0] * o[0] * shape[dim] > MOST_PARTS:
+        raise ValueError(f"state of shape {tuple(shape)} and strides {src.stride()} is too large: its rows fall into "
+                         f"more than {MOST_PARTS} contiguous parts")
     return (src.data_ptr(), dst.data_ptr(), nbytes, src.stride(dim) * size, dst.stride(dim) * size, *om, *o)
 
 
