@@ -142,6 +142,31 @@ def test_too_many_states_are_refused_before_any_is_moved(lib):
     assert decode._state(big, big, 0)[2] == 1 << 24
 
 
+def test_outputs_that_share_memory():
+    """The rule that outputs are checked by, on the host."""
+    m = torch.zeros(60)
+    apart = lambda w, r=(), same=(): decode._check_apart({f"w{i}": t for i, t in enumerate(w)}, {f"r{i}": t for i, t in enumerate(r)}, same)  # noqa: E731
+    apart([m[:10], m[10:20]], [m[20:], m[20:]])  # inputs may be anything
+    apart([m[:0], m[5:5]], [m])
+    apart([m[:10]], [m[:10]], {("w0", "r0")})
+    apart([m[:40].view(4, 10)[:, :5]], [m[40:]])
+    for w, r, word in (([m[:10], m[9:20]], [], "w0 overlaps w1"), ([m[30:], m[:31]], [], "overlaps"), ([m[:10]], [m[:10]], "w0 overlaps r0"),
+                       ([m[:10]], [m], "w0 overlaps r0"), ([m], [m[7:8]], "w0 overlaps r0"), ([m[:1].expand(4)], [], "broadcast"),
+                       ([m.as_strided((4, 5), (4, 1))], [], "itself"), ([m.as_strided((5, 5), (1, 1))], [], "itself")):
+        with pytest.raises(ValueError, match=word):
+            apart(w, r)
+    for w, r in (([m[:10]], [m[:11]]), ([m[:10]], [m[1:11]])):
+        with pytest.raises(ValueError, match="overlaps"):
+            apart(w, r, {("w0", "r0")})
+    p, t = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(6, 4)
+    o = torch.zeros(6, 4)
+    for states, out in (([t, t], [o, o]), ([t[:, :2], t], [o[:, 2:], o])):
+        with pytest.raises(ValueError, match="overlaps"):
+            decode.beam_reorder(states, p, out=out)
+    with pytest.raises(ValueError, match="overlaps parents"):
+        decode.beam_reorder([torch.zeros(6, 1, dtype=torch.int32)], p, out=[p.view(6, 1)])
+
+
 # --------------------------------------------------------------- GPU: select --
 # A score is off by at most: half a step of f32 (2^-24 of it); the f32
 # exponentials, whose relative error is 2^-22 (the function) + 2^-23 |t| (t
@@ -502,3 +527,25 @@ def test_captured_and_on_other_streams(lib, cuda):
     streams[0].synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
     assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_overlapping_outputs_are_refused(cuda):
+    x, s, f = make(3, 4, 50, "f32", 1)
+    new = decode.beam_select(x, s, f, eos=2)
+    room = torch.zeros(24, device="cuda")
+    bad = [new._replace(parents=new.tokens), new._replace(tokens=s.view(torch.int32)), new._replace(scores=x.view(-1)[6:18].view(3, 4)),
+           new._replace(tokens=new.scores.view(torch.int32)), new._replace(finished=room.view(torch.bool)[:12].view(3, 4), scores=room[1:13].view(3, 4))]
+    for out in bad:
+        with pytest.raises(ValueError, match="overlaps"):
+            decode.beam_select(x, s, f, eos=2, out=out)
+    shifted = room[4:16].view(3, 4).copy_(s)  # the scores one line further down in one buffer
+    with pytest.raises(ValueError, match="out.scores overlaps scores"):
+        decode.beam_select(x, shifted, f, eos=2, out=new._replace(scores=room[:12].view(3, 4)))
+    tok, par = torch.zeros(2, 5, 3, 4, dtype=torch.int32, device="cuda").unbind()
+    seq, n = decode.beam_sequences(tok, par)
+    for out in ((tok.view(3, 4, 5), n), (seq, seq.view(-1)[:12].view(3, 4)), (seq, par.view(-1)[:12].view(3, 4))):
+        with pytest.raises(ValueError, match="overlaps"):
+            decode.beam_sequences(tok, par, out=out)
+    decode.beam_select(x, s, f, eos=2, out=decode.BeamStep(s, tok[0], par[0], f))  # in place, into a history
+    assert torch.equal(s, new.scores) and torch.equal(tok[0], new.tokens) and torch.equal(f, new.finished)

@@ -84,6 +84,9 @@ def _check_out(name, t, shape, dtype, device):
                          f"{tuple(t.shape)}")
 
 
+_IN_PLACE = {("out.scores", "scores"), ("out.finished", "finished")}
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None, *, eos: int = -1,
                 out: BeamStep | None = None, stream=None) -> BeamStep:
     """The best `beams` continuations of every line by running score plus log
@@ -94,8 +97,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     beam; finished [lines, beams] bool or uint8, or None.  A finished beam
     continues with `eos` at an unchanged score.  A line with too few
     continuations above -inf fills up with score -inf, token eos, parent = the
-    slot.  A NaN logit counts as -inf.  `out`: buffers to write into; its
-    scores and finished may be the inputs'."""
+    slot.  A NaN logit counts as -inf.  `out`: buffers to write into, apart
+    from each other and the inputs; its scores and finished may be exactly the
+    inputs'."""
     if not (isinstance(scores, Tensor) and isinstance(logits, Tensor)
             and (finished is None or isinstance(finished, Tensor))):
         _check_tensors(scores=scores, logits=logits, finished=finished)
@@ -155,6 +159,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         out = BeamStep(*out)
         for name, t, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32, torch.bool)):
             _check_out(f"out.{name}", t, (lines, beams), dtype, device)
+        read = {"logits": logits, "scores": scores}
+        if finished is not None:
+            read["finished"] = finished
+        _check_apart({f"out.{n}": t for n, t in zip(out._fields, out)}, read, _IN_PLACE)
     if lines:
         L = lib()
         need = _select_workspace(code, lines, beams, vocab, device.index)
@@ -213,8 +221,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
     instance h and c [lines * beams, hidden], stacked layers [layers, lines *
     beams, hidden] (dim=1) or the filled part of a cache, cache[:, :, :n];
     parents [lines, beams] int32 as beam_select returns them.  Returns new
-    tensors, or writes into `out` (the same shapes and types, not overlapping
-    any state: keep two sets and use them in turn)."""
+    tensors, or writes into `out` (the same shapes and types, apart from the
+    states and each other: keep two sets and use them in turn)."""
     states = list(states)
     if not (isinstance(parents, Tensor) and all(isinstance(t, Tensor) for t in states)):
         _check_tensors(parents=parents, **{f"states[{i}]": t for i, t in enumerate(states)})
@@ -239,7 +247,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
             _check_tensors(**{f"out[{i}]": o})
             if o.shape != t.shape or o.dtype != t.dtype:
                 raise ValueError(f"out[{i}] must have the shape and type of states[{i}]")
-        _check_apart(states, out)
+        _check_apart({f"out[{i}]": o for i, o in enumerate(out)},
+                     {"parents": parents, **{f"states[{i}]": t for i, t in enumerate(states)}})
     _check_cuda("parents", parents)
     for i, t in enumerate(states):
         if t.device != device:
@@ -273,17 +282,36 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _check_apart(states, out):
-    spans = [(_span(t), f"states[{i}]") for i, t in enumerate(states) if t.numel()]
-    for i, o in enumerate(out):
-        if not o.numel():
-            continue
-        if any(st == 0 and n > 1 for n, st in zip(o.shape, o.stride())):
-            raise ValueError(f"out[{i}] is a broadcast view")
-        lo, hi = _span(o)
-        for (a, b), name in spans:
-            if lo < b and a < hi:
-                raise ValueError(f"out[{i}] overlaps {name}: reordering in place is not supported")
+def _check_apart(written, read, same=()):
+    """Refuses outputs that share memory with themselves, each other or an
+    input; `same`: (output, input) names that may be one buffer."""
+    spans = []
+    for group, is_out in ((written, True), (read, False)):
+        for name, t in group.items():
+            n = t.numel()
+            if not n:
+                continue
+            if t.is_contiguous():
+                lo = t.data_ptr()
+                spans.append((lo, lo + n * t.element_size(), is_out, name))
+                continue
+            if is_out:
+                reach = 1
+                for st, m in sorted(zip(t.stride(), t.shape)):
+                    if m > 1 and st < reach:
+                        raise ValueError(f"{name} is a broadcast view, or overlaps itself")
+                    reach += (m - 1) * st
+            spans.append((*_span(t), is_out, name))
+    spans.sort()
+    for i, (lo, hi, is_out, name) in enumerate(spans):
+        for lo2, hi2, is_out2, name2 in spans[i + 1:]:
+            if lo2 >= hi:
+                break
+            if not (is_out or is_out2):
+                continue
+            a, b = (name, name2) if is_out else (name2, name)
+            if not ((a, b) in same and (lo, hi) == (lo2, hi2)):
+                raise ValueError(f"{a} overlaps {b}")
 
 
 def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1, pad: int = 0, out=None,
@@ -291,7 +319,8 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1
     """(sequences [lines, beams, steps] int32, lengths [lines, beams] int32) of
     the paths that end in the last step's slots, from the [steps, lines,
     beams] int32 tokens and parents of all steps: each path's tokens before
-    its first `eos`, then `pad`."""
+    its first `eos`, then `pad`.  `out`: the two to write into, apart from the
+    inputs and each other."""
     if not (isinstance(tokens, Tensor) and isinstance(parents, Tensor)):
         _check_tensors(tokens=tokens, parents=parents)
     if tokens.dim() != 3 or tokens.dtype != torch.int32 or parents.shape != tokens.shape or parents.dtype != torch.int32:
@@ -317,6 +346,7 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1
         seq, lengths = out
         _check_out("out[0]", seq, (lines, beams, steps), torch.int32, device)
         _check_out("out[1]", lengths, (lines, beams), torch.int32, device)
+        _check_apart({"out[0]": seq, "out[1]": lengths}, {"tokens": tokens, "parents": parents})
         out = (seq, lengths)
     if lines:
         L = lib()
