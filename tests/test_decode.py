@@ -167,6 +167,36 @@ def test_outputs_that_share_memory():
         decode.beam_reorder([torch.zeros(6, 1, dtype=torch.int32)], p, out=[p.view(6, 1)])
 
 
+def test_interleaved_tensors():
+    """Side by side in a wider row, or not: by the addresses of all elements."""
+    def bytes_of(t):
+        at = np.zeros((), np.int64)
+        for n, st in zip(t.shape, t.stride()):
+            at = at[..., None] + np.arange(n) * st * t.element_size()
+        return set((at.ravel()[:, None] + t.data_ptr() + np.arange(t.element_size())).ravel().tolist())
+
+    rng = np.random.default_rng(0)
+    base = torch.zeros(4000, dtype=torch.uint8)
+    seen = [0, 0]
+    for _ in range(3000):
+        ts = []
+        for _ in range(2):
+            dtype = (torch.uint8, torch.int16, torch.int32)[rng.integers(3)]
+            size = torch.empty(0, dtype=dtype).element_size()
+            strides = [int(st) for st in rng.choice([1, 2, 8, 12, 24, 48, 96], 3)]
+            shape = [int(n) for n in rng.integers(1, 5, 3)]
+            ts.append(base.view(dtype).as_strided(shape, strides, int(rng.integers(60 // size))))
+        share = bool(bytes_of(ts[0]) & bytes_of(ts[1]))
+        assert not (decode._interleaved(*ts) and share)
+        assert decode._interleaved(*ts) == decode._interleaved(*ts[::-1])
+        seen[decode._interleaved(*ts)] += not share
+    assert min(seen) > 50
+    w = torch.zeros(6, 2, 8)
+    assert decode._interleaved(w[:, 0], w[:, 1]) and not decode._interleaved(w[:, 0], w[:, 0])
+    assert decode._interleaved(w[:, 0, :5], w[:, 1]) and not decode._interleaved(w[:, 0], w.view(6, 16)[:, 7:])
+    assert decode._interleaved(w[:, 0], w.view(96)[88:].view(1, 8)) is False  # (no stride in common; their ranges decide)
+
+
 # --------------------------------------------------------------- GPU: select --
 # A score is off by at most: half a step of f32 (2^-24 of it); the f32
 # exponentials, whose relative error is 2^-22 (the function) + 2^-23 |t| (t
@@ -384,6 +414,20 @@ def test_reorder_many_states_and_outputs(cuda):
     assert decode.beam_reorder([torch.empty(30, 0, device="cuda")], par)[0].shape == (30, 0)
     none = decode.beam_reorder([torch.empty(0, 3, device="cuda")], par[:0])[0]
     assert none.shape == (0, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,W", [(torch.float32, 8), (torch.int8, 3), (torch.bfloat16, 255)])
+def test_reorder_between_halves_of_one_buffer(dtype, W, cuda):
+    """Two sets of states in one allocation, used in turn."""
+    par = torch.tensor([[2, 0, 2], [1, 1, 0]], dtype=torch.int32, device="cuda")
+    both = torch.randint(0, 100, (6, 2, W), device="cuda").to(dtype)
+    want, layers = both[:, 0][rows_of(par)], torch.randint(0, 100, (4, 2, 6, W), device="cuda").to(dtype)
+    keep, want_l = both[:, 0].clone(), layers[:, 1][:, rows_of(par)]
+    decode.beam_reorder([both[:, 0]], par, out=[both[:, 1]])
+    assert torch.equal(both[:, 1], want) and torch.equal(both[:, 0], keep)
+    decode.beam_reorder([layers[:, 1]], par, dim=1, out=[layers[:, 0]])
+    assert torch.equal(layers[:, 0], want_l)
 
 
 @pytest.mark.gpu

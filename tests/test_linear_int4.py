@@ -327,3 +327,18 @@ def test_beam_search_through_the_layer(lib, cuda):
                                ([s.tokens for s in hist], [s.parents for s in hist])), eos, 0)
     assert np.array_equal(seq.cpu().numpy(), want[0]) and np.array_equal(n.cpu().numpy(), want[1])
     assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_output_beside_its_input(dtype, cuda):
+    """x and y as columns of one buffer, as layers that append to their input keep them."""
+    for rows, ins, outs in ((1, 40, 24), (5, 203, 70), (20, 203, 70)):
+        lin, q, s, b = layer(outs, ins, 32, "f32", rows)
+        buf = torch.randn(rows, ins + outs + 3, device="cuda").to(DTYPES[dtype])
+        x, rest = buf[:, :ins].clone(), buf[:, ins + outs:].clone()
+        lin.forward(buf[:, :ins], out=buf[:, ins:ins + outs])
+        check(buf[:, ins:ins + outs], x, q, s, b, ins, 32)
+        assert torch.equal(buf[:, :ins], x) and torch.equal(buf[:, ins + outs:], rest)
+        with pytest.raises(ValueError, match="overlaps"):
+            lin.forward(buf[:, :ins], out=buf[:, ins - 1:ins - 1 + outs])

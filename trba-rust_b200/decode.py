@@ -282,6 +282,19 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _interleaved(a, b):
+    """Whether two tensors share no byte although their ranges of memory do:
+    both lie side by side within every period of a stride that they have in
+    common (halves of the same wider rows, for instance)."""
+    dims = [[(n - 1, st * t.element_size()) for n, st in zip(t.shape, t.stride()) if n > 1] for t in (a, b)]
+    apart = b.data_ptr() - a.data_ptr()
+    for period in {st for _, st in dims[0]} & {st for _, st in dims[1]} - {0}:
+        wide = [t.element_size() + sum(n * st for n, st in d if st % period) for t, d in zip((a, b), dims)]
+        if apart % period >= wide[0] and -apart % period >= wide[1]:
+            return True
+    return False
+
+
 def _check_apart(written, read, same=()):
     """Refuses outputs that share memory with themselves, each other or an
     input; `same`: (output, input) names that may be one buffer."""
@@ -293,7 +306,7 @@ def _check_apart(written, read, same=()):
                 continue
             if t.is_contiguous():
                 lo = t.data_ptr()
-                spans.append((lo, lo + n * t.element_size(), is_out, name))
+                spans.append((lo, lo + n * t.element_size(), is_out, name, t))
                 continue
             if is_out:
                 reach = 1
@@ -301,16 +314,16 @@ def _check_apart(written, read, same=()):
                     if m > 1 and st < reach:
                         raise ValueError(f"{name} is a broadcast view, or overlaps itself")
                     reach += (m - 1) * st
-            spans.append((*_span(t), is_out, name))
-    spans.sort()
-    for i, (lo, hi, is_out, name) in enumerate(spans):
-        for lo2, hi2, is_out2, name2 in spans[i + 1:]:
+            spans.append((*_span(t), is_out, name, t))
+    spans.sort(key=lambda span: span[:4])
+    for i, (lo, hi, is_out, name, t) in enumerate(spans):
+        for lo2, hi2, is_out2, name2, t2 in spans[i + 1:]:
             if lo2 >= hi:
                 break
             if not (is_out or is_out2):
                 continue
             a, b = (name, name2) if is_out else (name2, name)
-            if not ((a, b) in same and (lo, hi) == (lo2, hi2)):
+            if not ((a, b) in same and (lo, hi) == (lo2, hi2)) and not _interleaved(t, t2):
                 raise ValueError(f"{a} overlaps {b}")
 
 

@@ -231,10 +231,7 @@ class LinearInt4:
             ldy = out.stride(0) if out.dim() == 2 and rows > 1 else outs
             if ldy < outs or (outs > 1 and out.stride(-1) != 1):
                 raise ValueError("LinearInt4::forward: the rows of out must be contiguous and apart")
-            if rows:
-                (a, b), (c, d) = decode._span(x), decode._span(out)
-                if a < d and c < b:
-                    raise ValueError("LinearInt4::forward: out overlaps x")
+            decode._check_apart({"LinearInt4::forward: out": out}, {"x": x})
         if rows > 1000000:
             raise ValueError("LinearInt4::forward: at most a million rows")
         if rows:
