@@ -593,3 +593,31 @@ def test_overlapping_outputs_are_refused(cuda):
             decode.beam_sequences(tok, par, out=out)
     decode.beam_select(x, s, f, eos=2, out=decode.BeamStep(s, tok[0], par[0], f))  # in place, into a history
     assert torch.equal(s, new.scores) and torch.equal(tok[0], new.tokens) and torch.equal(f, new.finished)
+
+
+@pytest.mark.gpu
+def test_negated_and_conjugated_views(cuda):
+    """torch's lazy views are read as the values they stand for."""
+    par = torch.tensor([[1, 1, 0]], dtype=torch.int32, device="cuda")
+    z = torch.randn(3, 5, dtype=torch.complex64, device="cuda")
+    neg = torch._neg_view(torch.randn(3, 5, device="cuda"))
+    assert z.conj().is_conj() and neg.is_neg()
+    got = decode.beam_reorder([z.conj(), neg, z.conj().imag, torch._neg_view(z.conj())], par)
+    for g, t in zip(got, (z.conj(), neg, z.conj().imag, -z.conj())):
+        assert torch.equal(g.resolve_conj().resolve_neg(), t.resolve_conj().resolve_neg()[par[0].long()])
+    for t, o in ((z, z.clone().conj()), (neg, torch._neg_view(torch.zeros(3, 5, device="cuda")))):
+        with pytest.raises(ValueError, match="view"):
+            decode.beam_reorder([t], par, out=[o])
+    x, s, f = make(2, 3, 70, "f32", 4)
+    want = decode.beam_select(x, s, f, eos=2)
+    got = decode.beam_select(torch._neg_view(-x), torch._neg_view(-s), f, eos=2)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    wide = torch.full((6, 80), 1e4, device="cuda")
+    wide[:, :70] = -x
+    got = decode.beam_select(torch._neg_view(wide[:, :70]), s, f, eos=2)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(ValueError, match="out.scores"):
+        decode.beam_select(x, s, f, eos=2, out=want._replace(scores=torch._neg_view(s.clone())))
+    t, p = (torch.randint(0, 3, (4, 2, 3), dtype=torch.int32, device="cuda") for _ in range(2))
+    got, want = decode.beam_sequences(torch._neg_view(-t), torch._neg_view(-p)), decode.beam_sequences(t, p)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

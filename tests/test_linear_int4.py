@@ -342,3 +342,16 @@ def test_output_beside_its_input(dtype, cuda):
         assert torch.equal(buf[:, :ins], x) and torch.equal(buf[:, ins + outs:], rest)
         with pytest.raises(ValueError, match="overlaps"):
             lin.forward(buf[:, :ins], out=buf[:, ins - 1:ins - 1 + outs])
+
+
+@pytest.mark.gpu
+def test_negated_views(cuda):
+    """torch's lazily negated views are read as the values they stand for."""
+    lin, q, s, b = layer(30, 100, 32, "f32", 2)
+    x = torch.randn(4, 100, device="cuda")
+    want = lin.forward(x)
+    assert torch.equal(lin.forward(torch._neg_view(-x)), want)
+    other = LinearInt4.from_codes(q, torch._neg_view(-s), in_features=100, group=32, bias=torch._neg_view(-b))
+    assert torch.equal(other.forward(x), want)
+    with pytest.raises(ValueError, match="out must be"):
+        lin.forward(x, out=torch._neg_view(torch.zeros(4, 30, device="cuda")))

@@ -66,6 +66,11 @@ def _check_cuda(name, t, device=None):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+def _plain(t):
+    """t itself, or the values of a view that torch negates or conjugates as it is read."""
+    return t.resolve_conj().resolve_neg() if t.is_neg() or t.is_conj() else t
+
+
 @functools.lru_cache(maxsize=256)
 def _select_workspace(code, lines, beams, vocab, device_index):
     return lib().trba_beam_select_workspace(code, lines, beams, vocab)
@@ -79,7 +84,7 @@ def _check_beams(beams):
 def _check_out(name, t, shape, dtype, device):
     _check_tensors(**{name: t})
     _check_cuda(name, t, device)
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.is_neg():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} "
                          f"{tuple(t.shape)}")
 
@@ -147,6 +152,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     if stream is not None or device.index != _current_device():
         with _on(device, stream):
             return beam_select(logits, scores, finished, eos=eos, out=out)
+    if logits.is_neg():  # (the copy's strides are others)
+        return beam_select(_plain(logits), scores, finished, eos=eos, out=out)
+    scores = _plain(scores)
     if not scores.is_contiguous():
         scores = scores.contiguous()
     if finished is not None and not finished.is_contiguous():
@@ -247,6 +255,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
             _check_tensors(**{f"out[{i}]": o})
             if o.shape != t.shape or o.dtype != t.dtype:
                 raise ValueError(f"out[{i}] must have the shape and type of states[{i}]")
+            if o.is_neg() or o.is_conj():
+                raise ValueError(f"out[{i}] is a negated or conjugated view")
         _check_apart({f"out[{i}]": o for i, o in enumerate(out)},
                      {"parents": parents, **{f"states[{i}]": t for i, t in enumerate(states)}})
     _check_cuda("parents", parents)
@@ -258,6 +268,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
     if stream is not None or device.index != _current_device():
         with _on(device, stream):
             return beam_reorder(states, parents, dim=dim, out=out)
+    parents, states = _plain(parents), [_plain(t) for t in states]
     if not parents.is_contiguous():
         parents = parents.contiguous()
     if out is None:
@@ -351,7 +362,7 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1
     if stream is not None or device.index != _current_device():
         with _on(device, stream):
             return beam_sequences(tokens, parents, eos=eos, pad=pad, out=out)
-    tokens, parents = tokens.contiguous(), parents.contiguous()
+    tokens, parents = _plain(tokens).contiguous(), _plain(parents).contiguous()
     if out is None:
         out = (torch.empty((lines, beams, steps), dtype=torch.int32, device=device),
                torch.empty((lines, beams), dtype=torch.int32, device=device))

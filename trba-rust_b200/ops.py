@@ -151,7 +151,7 @@ class LinearInt4:
         scale.  The tensors are copied, in the order of torch's current stream;
         a layer used on another stream is made there or waited for first."""
         import torch
-        from .decode import DTYPE_CODES, _check_cuda, _check_tensors, _on, _raw_stream
+        from .decode import DTYPE_CODES, _check_cuda, _check_tensors, _on, _plain, _raw_stream
         _check_tensors(codes=codes, scales=scales, bias=bias)
         if in_features < 1 or codes.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[1] != -(-in_features // 2):
             raise ValueError(f"codes must be a uint8 tensor [out, {-(-in_features // 2)}]")
@@ -168,8 +168,8 @@ class LinearInt4:
                 _check_cuda(name, t, device)
         self = cls.__new__(cls)
         with _on(device, None):
-            codes, scales = codes.contiguous(), scales.contiguous()
-            bias = None if bias is None else bias.contiguous()
+            codes, scales = _plain(codes).contiguous(), _plain(scales).contiguous()
+            bias = None if bias is None else _plain(bias).contiguous()
             need = lib().trba_linear_int4_bytes(in_features, out_features, group, DTYPE_CODES[scales.dtype])
             storage = torch.empty(need, dtype=torch.uint8, device=device)
             self.home = _raw_stream(device.index)  # the stream the storage belongs to
@@ -214,6 +214,7 @@ class LinearInt4:
         if stream is not None or device.index != decode._current_device():
             with decode._on(device, stream):
                 return self.forward(x, out)
+        x = decode._plain(x)
         if x.dim() != 2:
             x = x.reshape(-1, ins)
         rows = x.shape[0]
@@ -224,7 +225,7 @@ class LinearInt4:
             ldy = outs
         else:
             decode._check_cuda("out", out, device)
-            if out.shape != shape or out.dtype != x.dtype:
+            if out.shape != shape or out.dtype != x.dtype or out.is_neg():
                 raise ValueError(f"LinearInt4::forward: out must be {x.dtype} {tuple(shape)}")
             if out.dim() != 2 and not out.is_contiguous():
                 raise ValueError("LinearInt4::forward: out must be contiguous")
