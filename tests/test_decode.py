@@ -621,3 +621,36 @@ def test_negated_and_conjugated_views(cuda):
     t, p = (torch.randint(0, 3, (4, 2, 3), dtype=torch.int32, device="cuda") for _ in range(2))
     got, want = decode.beam_sequences(torch._neg_view(-t), torch._neg_view(-p)), decode.beam_sequences(t, p)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,L,K,V", [("f32", 1, 2, 1300003), ("bf16", 1, 1, 2300001), ("f16", 2, 1, 2100007)])
+def test_select_rows_of_millions(dtype, L, K, V, cuda):
+    """Segments of more batches than there are spans to remember: several
+    batches a span are looked at again.  Scores as everywhere: E|t| <= log V +
+    1 < 16 here, so 2^-22 + 16 * 2^-23 is still below 2^-18."""
+    x, s, f = make(L, K, V + 3, dtype, V & 7, mask=0.3)
+    for off in (0, 1, 3):
+        view = x[:, off:off + V]
+        got = [t.cpu().numpy() for t in decode.beam_select(view, s, eos=2)]
+        rows = view.double().view(L, K, V)
+        total = s.double()[:, :, None] + rows - torch.logsumexp(rows, -1, keepdim=True)
+        best = torch.sort(total.view(L, K * V), dim=1, descending=True, stable=True)
+        want, at = best[0][:, :K].cpu().numpy(), best[1][:, :K].cpu().numpy()
+        tol18 = 2.0 ** -18 + 2.0 ** -24 * np.abs(want)
+        assert (np.abs(got[0] - want) <= tol18).all()
+        flat = got[2].astype(np.int64) * V + got[1]
+        chosen = np.take_along_axis(total.view(L, K * V).cpu().numpy(), flat, 1)
+        assert (np.abs(chosen - want) <= 2 * tol18).all() and all(len(set(r)) == K for r in flat.tolist())
+        # within one beam the order is that of the logits, exactly: ties to the lowest token
+        if K == 1:
+            assert np.array_equal(flat, at)
+    # a single largest element anywhere in a span of several batches, ties to the lowest
+    y = torch.zeros(L * K, V, dtype=DTYPES[dtype], device="cuda")
+    for at in (0, 511, 8191, 8192, 8704, 16383, 1050624, V // 2 + 1, V - 1):
+        y.zero_()
+        y[:, at] = 1.0
+        y[:, V - 1] = 1.0
+        step = decode.beam_select(y, torch.zeros(L, K, device="cuda"))
+        want = [(k, v) for k in range(K) for v in sorted({at, V - 1})][:K]
+        assert list(zip(step.parents[-1].tolist(), step.tokens[-1].tolist())) == want

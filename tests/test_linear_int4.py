@@ -355,3 +355,110 @@ def test_negated_views(cuda):
     assert torch.equal(other.forward(x), want)
     with pytest.raises(ValueError, match="out must be"):
         lin.forward(x, out=torch._neg_view(torch.zeros(4, 30, device="cuda")))
+
+
+# ------------------------------------------------- GPU: what large sizes do --
+def check_rows(y, x, q, s, ins, group, at):
+    """check() for the outputs `at` alone."""
+    check(y[:, at].contiguous(), x, q[at], s[at], None, ins, group)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("outs,ins,group", [(50001, 300, 32), (40000, 643, 128)])
+def test_many_tiles_a_block(outs, ins, group, dtype, lib, cuda):
+    """More than eight columns through more tiles than the device has blocks for
+    at once: stages and partial sums go on from one group of tiles to the next."""
+    for rows in (9, 17, 24, 40, 61):
+        lin, q, s, b = layer(outs, ins, group, ("f32", "f16")[rows & 1], rows)
+        g = torch.Generator(device="cuda").manual_seed(rows)
+        x = torch.randn(rows, ins, generator=g, device="cuda").to(DTYPES[dtype])
+        check(lin.forward(x), x, q, s, b, ins, group)
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows", [("f16", 8), ("bf16", 7), ("f32", 2)])
+@pytest.mark.parametrize("outs,ins,group", [(5000, 16384, 128), (40001, 16001, 32)])
+def test_tiles_and_slabs(outs, ins, group, dtype, rows, lib, cuda):
+    """Few columns, several tiles a block, and more inputs than are staged at
+    once: sums of all its tiles wait between the slabs."""
+    lin, q, s, _ = layer(outs, ins, group, "f16", rows, bias=False)
+    x = torch.randn(rows, ins, generator=torch.Generator(device="cuda").manual_seed(rows), device="cuda").to(DTYPES[dtype])
+    y = lin.forward(x)
+    at = torch.cat([torch.arange(0, outs, 37), torch.arange(40), torch.arange(outs - 40, outs)]).cuda()
+    check_rows(y, x, q, s, ins, group, at)
+    assert torch.equal(y, lin.forward(x))
+    # every output: by the same layer in parts that have a tile or two a block
+    for n0 in range(0, outs, 4096):
+        n1 = min(outs, n0 + 4096)
+        part = LinearInt4.from_codes(q[n0:n1], s[n0:n1], in_features=ins, group=group)
+        size = (x.double().abs() @ torch.full((ins, 1), 8 * float(s.max()), dtype=torch.float64, device="cuda")).max()
+        tol = 2 * ((ins / 16 + 20) * 2.0 ** -23 * size + torch.finfo(x.dtype).eps / 2 * y.double().abs().max())
+        assert (part.forward(x).double() - y[:, n0:n1].double()).abs().max() <= tol
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_more_blocks_than_processors(lib, cuda):
+    """So many outputs that their sums leave no room for a slab: the grid grows."""
+    outs, ins, group, rows = 600007, 8500, 128, 8
+    lin, q, s, _ = layer(outs, ins, group, "f16", 3, bias=False)
+    x = torch.randn(rows, ins, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").half()
+    y = lin.forward(x)
+    at = torch.cat([torch.arange(0, outs, 997), torch.arange(outs - 20, outs)]).cuda()
+    check_rows(y, x, q, s, ins, group, at)
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_codes_and_scales_with_wider_rows(lib, cuda):
+    """create_codes with row strides above the rows' sizes, at an odd address of the codes."""
+    outs, ins, group = 45, 211, 64
+    wide = torch.randint(0, 256, (outs * 130 + 7,), dtype=torch.uint8, device="cuda")
+    for dtype, off, ld, lds in ((torch.float32, 0, 106, 4), (torch.float16, 3, 113, 7), (torch.float16, 4, 128, 5), (torch.float32, 1, 130, 9)):
+        q = wide[off:off + outs * ld].view(outs, ld)[:, :106]
+        s = (torch.rand(outs, lds, device="cuda") * 0.1 + 0.01).to(dtype)
+        h = lib.trba_linear_int4_create_codes(ins, outs, group, C.c_void_p(q.data_ptr()), ld, C.c_void_p(s.data_ptr()),
+                                              0 if dtype == torch.float32 else 2, lds, None, None, 0, None)
+        lin = LinearInt4.from_codes(q.contiguous(), s[:, :4].contiguous(), in_features=ins, group=group)
+        x = torch.randn(3, ins, device="cuda").bfloat16()
+        want, y = lin.forward(x), torch.empty(3, outs, dtype=torch.bfloat16, device="cuda")
+        assert lib.trba_linear_int4_forward(h, C.c_void_p(x.data_ptr()), 1, ins, 3, C.c_void_p(y.data_ptr()), outs, None, 0, None) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        check(y, x, q, s[:, :4], None, ins, group)
+        lib.trba_linear_int4_destroy(h)
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_memory_of_a_dropped_layer_waits_for_the_reading_stream(cuda):
+    """While calls on another stream are pending, the memory of the layer that
+    they read is not handed out again on the stream that made it."""
+    made, used = torch.cuda.Stream(), torch.cuda.Stream()
+    kept, q, s, b = layer(2000, 4096, 128, "f16", 5)
+    x = torch.randn(24, 4096, device="cuda").half()
+    want = kept.forward(x)
+    busy = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for read in (False, True):
+        with torch.cuda.stream(made):
+            lin = LinearInt4.from_codes(q, s, in_features=4096, group=128, bias=b)
+        size, ptr = lin.storage.numel(), lin.storage.data_ptr()
+        used.wait_stream(made)
+        with torch.cuda.stream(used):
+            for _ in range(40):  # tens of ms ahead of the layer's calls
+                busy = torch.tanh(busy @ busy)
+        ys = [lin.forward(x, stream=used) for _ in range(20)] if read else []
+        done = torch.cuda.Event()
+        done.record(used)
+        del lin
+        with torch.cuda.stream(made):
+            again = [torch.empty(size, dtype=torch.uint8, device="cuda").fill_(0x77) for _ in range(3)]
+        assert not done.query()
+        # (without a reader the block comes back at once: the check below can fail)
+        assert (ptr in [t.data_ptr() for t in again]) == (not read)
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in ys)
+        del again
