@@ -462,3 +462,27 @@ def test_memory_of_a_dropped_layer_waits_for_the_reading_stream(cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(y, want) for y in ys)
         del again
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 9])
+def test_tiny_activations(rows, cuda):
+    """Subnormal activations count in all types; of an f32 activation only what
+    lies below 2^-133 (the last place of a bf16) is dropped."""
+    outs, ins = 24, 256
+    lin, q, s, _ = layer(outs, ins, 32, "f32", 9, bias=False)
+    k = torch.randint(-500, 500, (rows, ins), generator=torch.Generator().manual_seed(rows)).cuda()
+    w = do.int4_weights(q.cpu().numpy(), s.cpu().numpy(), ins, 32)
+    for dtype, unit, dropped in ((torch.float16, 2.0 ** -24, 0.0), (torch.bfloat16, 2.0 ** -133, 0.0), (torch.float32, 2.0 ** -133, 0.0),
+                                 (torch.float32, 2.0 ** -143, 2.0 ** -133), (torch.float32, 2.0 ** -149, 2.0 ** -133)):
+        x = (k.double() * unit).to(dtype)
+        xx = x.double().cpu().numpy()
+        want, size = xx @ w.T, np.abs(xx) @ np.abs(w).T
+        # check()'s rule, what is dropped times its weight, and half a step of the
+        # output's and the sums' subnormals (ins / 16 + 20 additions, 2^-150 each)
+        lost = dropped * np.abs(w).sum(1) + (ins / 16 + 20) * 2.0 ** -149 + {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}.get(dtype, 2.0 ** -150)
+        tol = (ins / 16 + 20) * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * np.abs(want) + lost
+        err = np.abs(lin.forward(x).double().cpu().numpy() - want)
+        assert (err <= tol).all(), (dtype, unit, (err / tol).max())
+        if dtype != torch.float16 and unit == 2.0 ** -133:
+            assert np.abs(want).max() > 100 * np.max(lost)  # (values that would show if they were taken as zero)
