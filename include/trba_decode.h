@@ -12,9 +12,11 @@
  * All pointers are device pointers of the current device.  The functions
  * only launch kernels on `stream`, without allocation or synchronisation, so
  * they may be captured into CUDA graphs and, each with a workspace of its
- * own, run on several streams at once.  They return 0, -1 for a bad argument or a CUDA error
- * code; errors also follow the library policy (trba_last_error / abort on
- * error).  Zero lines is an empty call and returns 0. */
+ * own, run on several streams at once.  They return 0, -1 for a bad argument
+ * (then nothing has run) or a CUDA error code; errors also follow the library
+ * policy (trba_last_error / abort on error).  Zero lines is an empty call and
+ * returns 0.  Outputs must not overlap the inputs or each other, except where
+ * the same buffer is said to do. */
 #ifndef TRBA_DECODE_H
 #define TRBA_DECODE_H
 
@@ -48,8 +50,7 @@ extern "C" {
  * token is eos or the parent was finished).  A line with fewer than `beams`
  * continuations above -inf fills the remaining slots with score -inf, token
  * eos (0 when eos < 0), parent = the slot itself, finished 1 (0 when eos <
- * 0).  out_scores / out_finished may be the same buffers as scores /
- * finished.
+ * 0).  out_scores / out_finished may be exactly the buffers scores / finished.
  *
  * A logit of NaN counts as -inf (its token is never chosen and adds nothing
  * to the sum).  Where a row holds +inf, its +inf tokens share the
@@ -85,8 +86,9 @@ typedef struct {
 
 /* dst row (l, k) = src row (l, parents[l, k]) for every state, for each of
  * its outer and mid parts, in one launch for up to 16 states.  `states` is a
- * host array, read before the call returns.  dst must not overlap any src:
- * use two buffers in turn.  A parent outside [0, beams) leaves its dst row as
+ * host array, read before the call returns.  No dst may overlap a src or
+ * another dst: use two buffers in turn (they may be halves of wider rows).  A
+ * state's rows may have up to 2^31 - 2^20 parts of at most 1024 bytes.  A parent outside [0, beams) leaves its dst row as
  * it was. */
 int trba_beam_reorder(const trba_beam_state *states, int n_states, const int32_t *parents, int lines, int beams,
                       void *stream);

@@ -65,7 +65,9 @@ long long trba_linear_int8_param_count(const trba_linear_int8 *l);
  * time: W[n, k] = (code[n, k] - 8) * scale[n, k / group], 4-bit codes with one
  * scale per `group` consecutive inputs.  group is 32, 64 or a multiple of
  * 128; the last group of a row may be short.  Sums are f32 (f32 activations
- * enter them with all their bits) and y is rounded once, to the type of x.
+ * enter them with all their bits down to 2^-133; a group's sum of (code - 8) *
+ * x has to fit, before its scale) and y is rounded once, to the type of x.  It
+ * is an operator for serving: no gradients.
  *
  * A layer keeps its weights on the device that was current when it was
  * created; forward and get are refused on another one.  forward only

@@ -606,9 +606,11 @@ __global__ void __launch_bounds__(512) select_merge_kernel(const Found *__restri
 
 // -------------------------------------------------------------- reordering --
 // A copy, bound by memory.  A warp moves a piece of a row at a time, 4 units of
-// 16 bytes or 8 smaller ones a lane in flight.  Rows whose addresses are all multiples of
-// 4, 8 or 16 bytes go in such units; others in 4-byte words of the
-// destination, each put together from the two source words it lies in.
+// 16 bytes or 8 smaller ones a lane in flight.  Rows whose addresses are all
+// multiples of 4, 8 or 16 bytes go in such units; others in 4-byte words of the
+// destination, each put together from the two source words it lies in.  (Wider
+// units, put together from aligned ones as the selection's scan does, were not
+// tried.)
 constexpr int kMaxStates = 16;
 __host__ __device__ constexpr int moves_of(int vec) { return vec == 16 ? 4 : 8; }
 struct StateView {
@@ -714,9 +716,13 @@ __global__ void __launch_bounds__(256, 4) beam_reorder_kernel(const __grid_const
 // maps are composed, and a second walk from the right slots notes the path.
 // A CTA takes `group` lines, or a part of one line's beams (all CTAs of a line
 // read its parents).  Steps that do not fit go in chunks, last first.
-// Bound by the latency of the reads and of the barriers between the walks: 512
-// lines of 5 beams, 21 steps 6.4 us; 16 lines of 16 beams, 2000 steps 17 us
-// (0.36 TB/s), where a thread a path over device memory took 1007.
+// 512 lines of 5 beams, 21 steps 6.4 us, most of it launch and latency.  16 lines
+// of 16 beams, 2000 steps 16.5 us (0.36 TB/s), where a thread a path over device
+// memory took 1007: with a line's beams shared by 1 / 2 / 4 / 8 CTAs it takes
+// 30.8 / 22.6 / 18.5 / 16.5 us, so about 2 us of the second walk and the writing
+// are left, and 14 that sharing by beams does not divide: the launch, reading
+// all parents of the line, the first walk (63 dependent reads) and the
+// composition (32), in every CTA.
 constexpr uint8_t kLost = 255;  // behind a parent out of range
 
 constexpr int kTraceSmem = 96 * 1024;
@@ -870,8 +876,9 @@ int launched() {
 // How a selection runs: rows of up to two batches whole (segs = 0), longer
 // ones in segments of whole batches: one round of warps on the device, but no
 // segment so short that picking its best (and joining them, with many beams)
-// costs more than reading it, and none of more batches than there are spans to
-// remember, so that a second look is at one batch's groups.  With 2 / 4 / 8 /
+// costs more than reading it, and up to 128 segments (1 Mi f32 tokens) none of
+// more batches than there are spans to remember, so that a second look is at
+// one batch's groups.  With 2 / 4 / 8 /
 // 16 / 24 / 32 batches a segment, 64 lines of 10 beams, 65536 f32 take 68 / 50 /
 // 41 / 36 / 39 / 41 us, 16 lines of 32 beams, 20000 bf16 51 / 39 / 35 / 35 / 37 /
 // 37, one line of 5 beams, 32000 bf16 11 / 12 / 15 / 19 / 19 / 27.

@@ -139,22 +139,34 @@ __global__ void __launch_bounds__(256) int4_natural_kernel(const uint8_t *__rest
 // or stages of one block, gain nothing.
 constexpr int kPair = 2, kFewStages = 3;
 constexpr int kFewWarps = 16, kManyWarps = 16;
+// More columns, in tiles of eight: the stages of a step, and the blocks that a
+// warp takes in one.  Four stages instead of three gain a little at 4 and 5
+// tiles (16384 x 8192: 49.3 and 50.4 us at 32 rows, 53.6 and 54.3 at 40) and
+// nothing at 2 and 6; at 3 and 8 they leave room for fewer warps side by side
+// (50001 x 4099: 65.7 -> 76.3 us at 24 rows, 135 -> 163 at 64).  Two blocks a
+// step halve the barriers: 31.5 us instead of 37.0 at 16 rows through 16384 x
+// 8192, 65.7 instead of 71.9 at 24 through 50001 x 4099 (but 14.1 instead of
+// 12.3 through 4096 x 4096); from 5 tiles on their fragments take the room (40
+// rows through 50001 x 4099: 96 -> 107 us, 64: 135 -> 153; at 4 tiles 84 -> 78
+// there and 14.4 -> 16.4 through 4096 x 4096).
 constexpr int many_depth(int nt) { return nt > 3 && nt <= 5 ? 4 : 3; }
-constexpr int many_blocks(int nt) { return nt <= 3 ? 2 : 1; }  // of a warp in a step
+constexpr int many_blocks(int nt) { return nt <= 3 ? 2 : 1; }
 
 // y^T = W x^T on the tensor cores: A is a 16-output tile of the weights, the
 // codes turned into exact bf16 or f16 integers in registers, B the
 // activations, eight columns at a time.  An f32 activation enters as three
-// bf16 columns whose sum it is exactly, so its products with the codes are
-// exact in all types, and a group's sum is accumulated in f32 before its
-// scale multiplies it.
+// bf16 columns whose sum it is exactly (down to 2^-133, a bf16's last place),
+// so its products with the codes are exact in all types, and a group's sum is
+// accumulated in f32 before its scale multiplies it.
 //
 // What bounds it: at few rows, reading the codes (half a byte a weight) and
 // turning them into floats.  The warp-level mma is enough for that: a 1 KB block
 // of codes costs 8 mma per eight columns and about 75 integer and conversion
-// instructions, which take as long as reading the block.  tcgen05 would take
-// the codes from shared memory as floats, four times as many bytes written
-// and read there, and its 128-row tiles would be one to eight columns wide.
+// instructions, which take as long as reading the block.  tcgen05 was not
+// built, so not measured either: its weights, as floats, would pass through
+// tensor memory on the way, a group's sum would need columns of its own to be
+// scaled from, and its 128-row tiles would be one to eight columns wide at the
+// rows of a decoding step.
 //
 // One CTA a SM for the whole product, its tiles a contiguous share of all of
 // them, its warps `wn` tiles side by side by `wk` parts of the inputs.  The
@@ -207,7 +219,10 @@ __device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_
 __device__ __forceinline__ uint32_t bf162_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t *>(&v); }
 
 // The four pairs of a word (codes at bits 4 j and 4 j + 16) as floats, exact,
-// with one shift a word.
+// with one shift a word.  Or-ing a small integer into the mantissa of a power of
+// two, instead of converting it, is a published method (Kim et al., "Who Says
+// Elephants Can't Run", 2022, for 4-bit weights in f16); the bf16 form is this
+// file's own.
 // f16: the code is or-ed into the mantissa of 1024 at either of two places,
 // the upper one worth 16 times as much: code - 8.
 // bf16 has room for one place behind 128.  The place above it needs no
@@ -414,9 +429,11 @@ __device__ __forceinline__ void write_tile(const Args &a, int tile, int row0, in
 // running over one slab before the next; sums wait in shared memory in between.
 // One bf16 row through 16384 x 16384, groups of 128: 31.5 us, 4.4 TB/s of codes
 // and scales, 0.67 of a copy's rate; one f16 row through 16384 x 8192, groups of
-// 32: 20 us.  With data, tensor pipe (25%) and issue slots (57%) all below their
-// limits, what is left is the wait of a warp for its own ring.  Sharing out the
-// tiles so that a CTA has all inputs of its outputs needs no sums in memory.
+// 32: 20 us.  In the first of these a CTA has seven tiles for eight pairs of
+// warps, so an eighth of them has nothing to do; the others wait for their own
+// rings, with data, tensor pipe (25%) and issue slots (57%) all below their
+// limits.  Sharing out the tiles so that a CTA has all inputs of its outputs
+// needs no sums in memory.
 template <bool F16, class S, int WG>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -536,8 +553,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) int4_few_kernel(const __gri
 // pipe's floor is above memory's (a 16 x 8 x 16 mma takes 2.4 cycles a SM).
 // 40 f16 rows through 50001 x 4099, groups of 32: 95 us with the fragments, 1.3
 // TB/s of codes and scales and 173 TFLOP/s; tensor pipe 37%, issue slots 48%: bound
-// by the shared-memory reads and conversions between the barriers of a step.  16
-// rows through 16384 x 8192: 35 us, 64 rows 80 us.
+// by the shared-memory reads and conversions between the barriers of a step (a
+// warp has one tile of 16 outputs, and reads all fragments for it).  16 rows
+// through 16384 x 8192: 32 to 35 us, 64 rows 76 to 80 us.  Beyond 64 columns a
+// row block follows the other, each reading and unpacking the whole layer: 128
+// rows 147 us, 512 rows 498 us.
 template <bool F16, class S, int WG, int NT>
 __global__ void __launch_bounds__(kManyWarps * 32, 1) int4_many_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(128) uint8_t smem[];

@@ -8,7 +8,9 @@ Work is queued on torch's current stream of the tensors' device, or on
 ``stream`` (a torch.cuda.Stream); outputs and workspaces belong to that
 stream.  As with torch's own operators, inputs that another stream writes have
 to be waited for, and kept, by the caller.  Arguments are checked here: a
-ValueError or TypeError means that nothing ran.
+ValueError or TypeError means that nothing ran.  These are operators for
+serving: they record no graph, and what they return for inputs that require
+gradients requires none.
 """
 from __future__ import annotations
 

@@ -115,7 +115,8 @@ class LinearInt4:
         lin = LinearInt4(in_features, out_features, weight_f32, bias, group=128)
         y = lin.forward(x)     # torch CUDA tensors, [rows, in] -> [rows, out]
 
-    No counterpart in the reference."""
+    An operator for serving: forward records no graph, and y requires no
+    gradient although x may.  No counterpart in the reference."""
 
     def __init__(self, in_features: int, out_features: int, weight_f32: np.ndarray, bias: np.ndarray | None = None,
                  group: int = 128):
@@ -196,7 +197,8 @@ class LinearInt4:
     def forward(self, x, out=None, stream=None):
         """[rows, in] -> [rows, out] of the same type (float32, bfloat16 or
         float16); leading dimensions of x are rows.  Runs on torch's current
-        stream, or on `stream` (a torch.cuda.Stream)."""
+        stream, or on `stream` (a torch.cuda.Stream).  `out` must share no
+        memory with x."""
         torch, decode = self.torch, self.decode
         if not self.h:
             raise RuntimeError("LinearInt4::forward: the layer is closed")
