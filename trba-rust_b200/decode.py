@@ -156,7 +156,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
             return beam_select(logits, scores, finished, eos=eos, out=out)
     if logits.is_neg():  # (the copy's strides are others)
         return beam_select(_plain(logits), scores, finished, eos=eos, out=out)
-    scores = _plain(scores)
+    if scores.is_neg():
+        scores = _plain(scores)
     if not scores.is_contiguous():
         scores = scores.contiguous()
     if finished is not None and not finished.is_contiguous():
@@ -244,11 +245,17 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
     if rows >= 1 << 24:
         raise ValueError("lines * beams must be below 2**24")
     device = parents.device
+    elsewhere, lazy = False, parents.is_neg()
     for i, t in enumerate(states):
-        if not -t.dim() <= dim < t.dim():
+        n = t.dim()
+        if not -n <= dim < n:
             raise ValueError(f"states[{i}] has no dimension {dim}")
         if t.shape[dim] != rows:
             raise ValueError(f"states[{i}]: dimension {dim} is {t.shape[dim]}, expected lines * beams = {rows}")
+        if t.device != device:
+            elsewhere = True
+        if t.is_neg() or t.is_conj():
+            lazy = True
     if out is not None:
         out = list(out)
         if len(out) != len(states):
@@ -261,16 +268,18 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, dim: 
                 raise ValueError(f"out[{i}] is a negated or conjugated view")
         _check_apart({f"out[{i}]": o for i, o in enumerate(out)},
                      {"parents": parents, **{f"states[{i}]": t for i, t in enumerate(states)}})
-    _check_cuda("parents", parents)
-    for i, t in enumerate(states):
-        if t.device != device:
+        for i, o in enumerate(out):
+            _check_cuda(f"out[{i}]", o, device)
+    if not parents.is_cuda:
+        _check_cuda("parents", parents)
+    if elsewhere:
+        for i, t in enumerate(states):
             _check_cuda(f"states[{i}]", t, device)
-    for i, t in enumerate(out or ()):
-        _check_cuda(f"out[{i}]", t, device)
     if stream is not None or device.index != _current_device():
         with _on(device, stream):
             return beam_reorder(states, parents, dim=dim, out=out)
-    parents, states = _plain(parents), [_plain(t) for t in states]
+    if lazy:
+        parents, states = _plain(parents), [_plain(t) for t in states]
     if not parents.is_contiguous():
         parents = parents.contiguous()
     if out is None:
@@ -364,7 +373,9 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, *, eos: int = -1
     if stream is not None or device.index != _current_device():
         with _on(device, stream):
             return beam_sequences(tokens, parents, eos=eos, pad=pad, out=out)
-    tokens, parents = _plain(tokens).contiguous(), _plain(parents).contiguous()
+    if tokens.is_neg() or parents.is_neg():
+        tokens, parents = _plain(tokens), _plain(parents)
+    tokens, parents = tokens.contiguous(), parents.contiguous()
     if out is None:
         out = (torch.empty((lines, beams, steps), dtype=torch.int32, device=device),
                torch.empty((lines, beams), dtype=torch.int32, device=device))

@@ -216,7 +216,8 @@ class LinearInt4:
         if stream is not None or device.index != decode._current_device():
             with decode._on(device, stream):
                 return self.forward(x, out)
-        x = decode._plain(x)
+        if x.is_neg():
+            x = decode._plain(x)
         if x.dim() != 2:
             x = x.reshape(-1, ins)
         rows = x.shape[0]
