@@ -654,3 +654,43 @@ def test_select_rows_of_millions(dtype, L, K, V, cuda):
         step = decode.beam_select(y, torch.zeros(L, K, device="cuda"))
         want = [(k, v) for k in range(K) for v in sorted({at, V - 1})][:K]
         assert list(zip(step.parents[-1].tolist(), step.tokens[-1].tolist())) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_select_largest_vocabulary(dtype, lib, cuda):
+    """2^30 tokens: zeros, a few of them higher.  |t| is at most 12 here, and a
+    thread's partial sum takes 5 additions: 2^-22 + 12 * 2^-23 + 5 * 2^-24 < 2^-18."""
+    tol = lambda s: 2.0 ** -18 + 2.0 ** -24 * abs(s)  # noqa: E731
+    V = 1 << 30
+    x = torch.zeros(1, V, dtype=DTYPES[dtype], device="cuda")
+    s = torch.tensor([[-1.5]], device="cuda")
+    step = decode.beam_select(x, s)
+    assert step.tokens.item() == 0 and abs(step.scores.item() + 1.5 + np.log(V)) <= tol(22.3)
+    for at in (V - 1, V // 2 + 12345, 777):  # each higher than the one before
+        x[0, at] = x.max() + 4
+        step = decode.beam_select(x, s, torch.zeros(1, 1, dtype=torch.bool, device="cuda"), eos=V - 1)
+        n = int(round(x.max().item() / 4))
+        want = -1.5 + 4 * n - np.log(V - n + sum(np.exp(4.0 * k) for k in range(1, n + 1)))
+        assert step.tokens.item() == at and abs(step.scores.item() - want) <= tol(want)
+        assert step.finished.item() == (at == V - 1)
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K", [(300001, 2), (70000, 32)])
+def test_sequences_of_many_steps(T, K, lib, cuda):
+    """Many chunks of steps, the last first."""
+    rng = np.random.default_rng(K)
+    tok, par = rng.integers(3, 60, (T, 1, K)).astype(np.int32), rng.integers(0, K, (T, 1, K)).astype(np.int32)
+    tok[T // 3 * 2] = 2
+    par[0] = 0
+    slot, path = np.arange(K), np.empty((T, K), np.int32)
+    for t in range(T - 1, -1, -1):
+        path[t] = tok[t, 0, slot]
+        slot = par[t, 0, slot]
+    seq, n = decode.beam_sequences(torch.from_numpy(tok).cuda(), torch.from_numpy(par).cuda(), eos=2, pad=-1)
+    assert (n == T // 3 * 2).all()
+    path[T // 3 * 2:] = -1
+    assert np.array_equal(seq[0].cpu().numpy(), path.T)
+    assert lib.trba_last_error() == 0

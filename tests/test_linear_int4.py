@@ -486,3 +486,41 @@ def test_tiny_activations(rows, cuda):
         assert (err <= tol).all(), (dtype, unit, (err / tol).max())
         if dtype != torch.float16 and unit == 2.0 ** -133:
             assert np.abs(want).max() > 100 * np.max(lost)  # (values that would show if they were taken as zero)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ins", [1 << 30, (1 << 30) - 129])
+def test_most_inputs(ins, lib, cuda):
+    """The most inputs that a layer takes: the staged activations of a row are
+    counted in 64 bits.  Three inputs count, the rest are zero."""
+    outs, rows = 3, 2
+    q = torch.full((outs, -(-ins // 2)), 0x88, dtype=torch.uint8, device="cuda")
+    s = torch.ones(outs, 1, device="cuda")
+    at = [0, ins // 2 + 77, ins - 1]
+    code = torch.randint(0, 16, (outs, 3), generator=torch.Generator().manual_seed(1), dtype=torch.uint8).cuda()
+    for j, k in enumerate(at):
+        q[:, k // 2] = (0x80 | code[:, j]) if k % 2 == 0 else (8 | code[:, j] << 4)
+    lin = LinearInt4.from_codes(q, s, in_features=ins, group=1 << 30)
+    del q
+    x = torch.zeros(rows, ins, dtype=torch.bfloat16, device="cuda")
+    x[:, at] = torch.tensor([[1.0, 2.0, -3.0], [0.5, -4.0, 8.0]], device="cuda").bfloat16()
+    want = x[:, at].float() @ (code.float() - 8).T
+    assert torch.equal(lin.forward(x).float(), want.bfloat16().float())
+    assert torch.equal(lin.forward(x[:1]).float(), want[:1].bfloat16().float())
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_most_rows(dtype, lib, cuda):
+    outs, ins, rows = 40, 64, 1000000
+    lin, q, s, b = layer(outs, ins, 32, "f32", 1)
+    x = torch.randn(rows, ins, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(DTYPES[dtype])
+    y = lin.forward(x)
+    w = torch.from_numpy(do.int4_weights(q.cpu().numpy(), s.cpu().numpy(), ins, 32)).cuda()
+    want, size = x.double() @ w.T + b, x.double().abs() @ w.abs().T + b.abs()
+    tol = (ins / 16 + 20) * 2.0 ** -23 * size + torch.finfo(y.dtype).eps / 2 * want.abs() + 2.0 ** -25  # as in check()
+    assert ((y.double() - want).abs() <= tol).all()
+    with pytest.raises(ValueError, match="million"):
+        lin.forward(x[:1].expand(rows + 1, ins))
+    assert lib.trba_last_error() == 0

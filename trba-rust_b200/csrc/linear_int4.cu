@@ -809,7 +809,7 @@ int forward(const trba_linear_int4 *l, const void *x, int dtype, i64 ldx, int ro
     } else {
         const int cols = rows * (dtype == TRBA_F32 ? 3 : 1);
         const int ring = kFewWarps * kFewStages * kPair * l->block;
-        const auto x_bytes = [&](int chunks) { return ((i64)cols * (chunks * 256 + 64) + 127) & ~127ll; };
+        const auto x_bytes = [&](int chunks) { return (cols * ((i64)chunks * 256 + 64) + 127) & ~127ll; };
         for (ctas = a.tiles < sm_count() ? a.tiles : sm_count();; ctas = ctas * 2 < a.tiles ? ctas * 2 : a.tiles) {
             const int share = (a.tiles + ctas - 1) / ctas;  // tiles of a CTA, at most
             // Tiles of a CTA that run side by side: the fewest steps of (chunks a
