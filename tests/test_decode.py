@@ -167,6 +167,12 @@ def test_outputs_that_share_memory():
         decode.beam_reorder([torch.zeros(6, 1, dtype=torch.int32)], p, out=[p.view(6, 1)])
 
 
+def test_streams_are_torchs():
+    for stream in (0, C.c_void_p(64), "0"):
+        with pytest.raises(TypeError, match="torch.cuda.Stream"):
+            decode._on(torch.device("cuda", 0), stream)
+
+
 def test_interleaved_tensors():
     """Side by side in a wider row, or not: by the addresses of all elements."""
     def bytes_of(t):
@@ -693,4 +699,34 @@ def test_sequences_of_many_steps(T, K, lib, cuda):
     assert (n == T // 3 * 2).all()
     path[T // 3 * 2:] = -1
     assert np.array_equal(seq[0].cpu().numpy(), path.T)
+    assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+def test_long_rows_captured(lib, cuda):
+    """The two launches of long rows in two graphs that run at once, on new inputs."""
+    L, K, V = 3, 5, 30011
+    inputs = [make(L, K, V, "bf16", 70 + i) for i in range(4)]
+    want = [decode.beam_select(*i, eos=2) for i in inputs]
+    graphs = []
+    for q in range(2):
+        buf = [t.clone() for t in inputs[q]]
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = decode.beam_select(*buf, eos=2)
+            for _ in range(3):  # a step on the scores of the last, in one graph
+                again = decode.beam_select(buf[0], out.scores, out.finished, eos=2)
+        graphs.append((g, buf, out, again, torch.cuda.Stream()))
+    for r in range(2):
+        for q, (g, buf, _, _, st) in enumerate(graphs):
+            with torch.cuda.stream(st):
+                for b, t in zip(buf, inputs[2 * r + q]):
+                    b.copy_(t)
+                for _ in range(5):
+                    g.replay()
+        torch.cuda.synchronize()
+        for q, (_, buf, out, again, _) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[2 * r + q]))
+            check_step(again, buf[0], out.scores, out.finished, 2)
     assert lib.trba_last_error() == 0

@@ -524,3 +524,30 @@ def test_most_rows(dtype, lib, cuda):
     with pytest.raises(ValueError, match="million"):
         lin.forward(x[:1].expand(rows + 1, ins))
     assert lib.trba_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,outs,ins", [("f16", 40, 1000, 4000), ("bf16", 16, 3000, 1111), ("f32", 9, 130, 2048)])
+def test_many_columns_captured_on_two_streams(dtype, rows, outs, ins, cuda):
+    """As test_captured_on_two_streams, for the two launches of many columns
+    (inputs split over clusters in the first and the last)."""
+    lin, q, s, b = layer(outs, ins, 64, "f16", 8)
+    xs = [torch.randn(rows, ins, device="cuda").to(DTYPES[dtype]) for _ in range(4)]
+    want = [lin.forward(x) for x in xs]
+    graphs = []
+    for k in range(2):
+        buf = xs[k].clone()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ys = [lin.forward(buf) for _ in range(4)]
+        graphs.append((g, buf, ys, torch.cuda.Stream()))
+    for r in range(2):
+        for k, (g, buf, _, st) in enumerate(graphs):
+            with torch.cuda.stream(st):
+                buf.copy_(xs[2 * r + k])
+                for _ in range(5):
+                    g.replay()
+        torch.cuda.synchronize()
+        for k, (_, _, ys, _) in enumerate(graphs):
+            assert all(torch.equal(y, want[2 * r + k]) for y in ys)

@@ -50,6 +50,8 @@ def _on(device: torch.device, stream):
     """Context in which `stream` (None: the device's current one) and `device` are current."""
     if stream is None:
         return torch.cuda.device(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        raise TypeError(f"stream must be a torch.cuda.Stream, got {type(stream).__name__}")
     if stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
     return torch.cuda.stream(stream)
