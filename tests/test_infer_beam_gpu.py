@@ -228,3 +228,24 @@ def test_images_that_are_views(lib, cuda):
         got = gm.infer_beam(view, 3, stream=st.cuda_stream)
         st.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_growth_while_another_stream_captures(lib, cuda):
+    """The default stream's call that allocates meanwhile leaves the capture as it was."""
+    import torch
+    ocfg, _, gm = _pair(dict(img_w=64, max_len=4), 4, seed=78, train_steps=0)
+    img = torch.from_numpy(np.ascontiguousarray(so.make_batch(ocfg, 4, seed=5)[0])).cuda()
+    seq = torch.empty(4, 3, ocfg.steps, dtype=torch.int32, device="cuda")
+    lengths, x = torch.empty(4, 3, dtype=torch.int32, device="cuda"), torch.ones(8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        y = x + 1
+        rc = lib.trba_model_infer_beam(gm.h, img.data_ptr(), 4, 3, seq.data_ptr(), lengths.data_ptr(), None, None)
+        y = y * 2
+    assert rc == 0 and lib.trba_last_error() == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (y == 4).all()
+    want = gm.infer_beam(img, 3)
+    assert torch.equal(want[0], seq) and torch.equal(want[1], lengths)

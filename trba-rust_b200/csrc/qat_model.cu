@@ -1765,11 +1765,17 @@ int trba_model_infer_beam(trba_model *m, const int8_t *img, int batch, int beams
     const size_t need = BeamBuffers(nullptr, m, batch, beams).used;
     if (need > m->beam_bytes) {
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        TRBA_CHECK(cudaStreamIsCapturing(st, &capturing));
+        if (cudaStreamIsCapturing(st, &capturing) != cudaSuccess) {  // the default stream while another one captures
+            cudaGetLastError();
+            return -4;
+        }
         if (capturing != cudaStreamCaptureStatusNone) return -4;
         const size_t bytes = std::max(need, 2 * m->beam_bytes);
         uint8_t *mem = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // another stream may capture meanwhile
+        cudaThreadExchangeStreamCaptureMode(&mode);
         const cudaError_t e = cudaMalloc(&mem, bytes);
+        cudaThreadExchangeStreamCaptureMode(&mode);
         if (e != cudaSuccess) {
             cudaGetLastError();
             report_error(__FILE__, __LINE__, "trba_model_infer_beam: device allocation failed", (int)e);
